@@ -216,7 +216,7 @@ def _plain_tables(s):
     n, width = table.shape
     want = (s["lens"] + page - 1) // page
     back = (have - want).clamp(min=0)
-    need = (want - have).clamp(min=0)
+    need = torch.where(want <= width, (want - have).clamp(min=0), 0)
     column = torch.arange(width, device=table.device)
     # pages given back go on the stack, request by request
     gone = (column >= want[:, None]) & (column < have[:, None])
@@ -342,7 +342,10 @@ def exact(case, seed):
         granted = np.ones(n, np.int32)
         for r in range(n):
             need = max(0, want[r] - int(have[r]))
-            if need > count or want[r] > width:
+            if want[r] > width:
+                granted[r] = 0
+                continue
+            if need > count:  # the rest of those that grow gets nothing either
                 granted[r:] = [0 if want[i] > have[i] else 1 for i in range(r, n)]
                 break
             for j in range(need):
