@@ -226,6 +226,74 @@ int sb200_kv_cache_slots(int64_t* slots, const int32_t* batch_indices, const int
 int sb200_kv_cache_append(void* cache, const void* k, int64_t ldk, const void* v, int64_t ldv, const int64_t* slots,
                           int64_t n, int num_kv_heads, int head_dim, int page_size, int dtype, sb200_stream_t stream);
 
+/* Most requests of a step in the three calls below. */
+#define SB200_MAX_REQUESTS 8192
+
+/* Block tables from request lengths.  Afterwards request r owns ceil(seq_lens[r] / page_size) pages: entries
+ * [0, num_blocks[r]) of row r of block_tables ([num_requests, width] int32, rows ld apart).  Pages that a request no longer
+ * needs are pushed on free_blocks[0 .. *num_free) (`capacity` entries) first, requests in order; then the requests that grow
+ * pop theirs from its top, in order.  A request that wants more than `width` pages gets none and costs none; one that the
+ * remaining pages do not suffice for gets none, nor do those that grow after it: granted[r] is 1 where request r has what it
+ * asked for and 0 where it was left as it was.  A negative length leaves a request alone (granted).  Pages whose push would
+ * pass `capacity` stay with their request (granted 0).  Entries beyond num_blocks / *num_free keep what they held.  Rows must
+ * not overlap.  Nothing is read on the host.  Counterpart in the reference: the block manager's lists
+ * (sarathi/core/block_space_manager), host code. */
+int sb200_resize_block_tables(int32_t* block_tables, int64_t ld, int32_t* num_blocks, const int32_t* seq_lens,
+                              int32_t* free_blocks, int32_t* num_free, int32_t* granted, int num_requests, int width,
+                              int64_t capacity, int page_size, sb200_stream_t stream);
+
+/* Index arrays of a step from its lengths: request r has context_lens[r] tokens in the cache and adds query_lens[r]; the new
+ * tokens of all requests lie one after the other in a batch padded to num_tokens rows.
+ *   qo_indptr [n + 1]: first row of every request;  kv_lens [n]: context + new tokens;  kv_indptr [n + 1], kv_indices
+ *   [kv_capacity >= n * width]: its pages, from block_tables, -1 behind the last;  last_page_len [n]: tokens in its last page;
+ *   per row: batch_indices (request, -1 for padding), positions (int64, 0 for padding), kv_slots as sb200_kv_cache_slots
+ *   (-1 for padding and for pages outside [0, num_pages)).
+ * Negative lengths count as zero; a context is cut to what the table has room for, and new tokens to what is then left in the
+ * table and in num_tokens.  Replaces the host loops of begin_forward
+ * (sarathi/model_executor/attention/flashinfer_attention_wrapper.py). */
+int sb200_batch_layout(const int32_t* query_lens, const int32_t* context_lens, const int32_t* block_tables, int64_t ld,
+                       int num_requests, int width, int page_size, int64_t num_pages, int64_t num_tokens, int32_t* qo_indptr,
+                       int32_t* kv_lens, int32_t* kv_indptr, int32_t* kv_indices, int64_t kv_capacity, int32_t* last_page_len,
+                       int32_t* batch_indices, int64_t* positions, int64_t* kv_slots, sb200_stream_t stream);
+
+/* ------------------------------------------------- attention over the paged cache */
+
+/* What a plan is made for. */
+typedef struct sb200_attention_shape {
+  int num_heads, num_kv_heads;  /* of this rank; num_heads a multiple of num_kv_heads */
+  int head_dim;                 /* 64, 128 or 256 */
+  int page_size;
+  int dtype;                    /* of q, out and the cache */
+  int window;                   /* a token sees itself and the window - 1 tokens before it; 0: all before it */
+  int max_requests, max_tokens;
+} sb200_attention_shape;
+
+/* Causal attention of a step's new tokens: row i of request r stands at position kv_lens[r] - (rows of r) + i and sees the
+ * cached keys up to that position (its own and its neighbours' have been appended before).  Prompt chunks and single decoded
+ * tokens share one call.
+ * sb200_attention_plan divides the work of a step over the SMs, on the device, from qo_indptr / kv_lens / kv_indptr as
+ * sb200_batch_layout makes them: once a step, for all layers of this shape.  `plan` (sb200_attention_plan_bytes bytes) is
+ * read by every sb200_paged_attention of the step.
+ * sb200_paged_attention: out[t, h, :] = sum_j softmax_j(scale q[t, h] . k[j]) v[j].  q and out: [num_tokens, num_heads *
+ * head_dim], rows ldq / ldo elements apart (views of the fused qkv buffer are fine); cache: [num_pages, 2, page_size,
+ * num_kv_heads, head_dim]; kv_indices as planned.  lse: NULL or fp32 [num_tokens, num_heads], the natural logarithm of
+ * sum_j exp(scale q . k[j]).  Scores, maxima, sums and outputs are fp32 until the one rounding at the end; fp16 / bf16
+ * round the probabilities once more, for the second product.  A row that sees no key is zero (lse -inf).  Rows that belong to no
+ * request are left as they were, or cleared if zero_rows_behind.  Pages outside [0, num_pages) read as zeros.
+ * workspace (sb200_attention_workspace_bytes): parts of rows whose keys are shared out; written before it is read in every
+ * call.  A plan and a workspace serve one call at a time: not two streams at once.  `status` (device word): as sb200_gemm_colpar.
+ * Replaces: BatchPrefillWithPagedKVCacheWrapper.plan / run,
+ * sarathi/model_executor/attention/flashinfer_attention_wrapper.py:240-299. */
+int64_t sb200_attention_plan_bytes(const sb200_attention_shape* shape);
+int64_t sb200_attention_workspace_bytes(const sb200_attention_shape* shape);
+int sb200_attention_plan(void* plan, int64_t plan_bytes, const sb200_attention_shape* shape, const int32_t* qo_indptr,
+                         const int32_t* kv_lens, const int32_t* kv_indptr, int num_requests, int64_t num_kv_indices,
+                         sb200_stream_t stream);
+int sb200_paged_attention(void* out, int64_t ldo, float* lse, const void* q, int64_t ldq, int64_t num_tokens, const void* cache,
+                          int64_t num_pages, const void* plan, const sb200_attention_shape* shape, const int32_t* kv_indices,
+                          int64_t num_kv_indices, float scale, int zero_rows_behind, void* workspace, int64_t workspace_bytes,
+                          uint32_t* status, sb200_stream_t stream);
+
 /* The tile shape and schedule of the general tensor-core kernel (epilogue 3 = the row-parallel
  * kernel, which always is that one; sb200_gemm_launch says which kernel a column-parallel call
  * takes): out[0..11] = cta_pairs, accumulators, BN, scheduling units, tiles handed out whole,

@@ -38,7 +38,14 @@ class RotaryArgs(ctypes.Structure):
                 ("kv_cache", c_void_p), ("kv_slots", c_void_p), ("kv_page_size", c_int), ("num_kv_heads", c_int)]
 
 
+class AttentionShape(ctypes.Structure):
+    """Mirror of ``sb200_attention_shape`` (include/sarathi_b200.h)."""
+    _fields_ = [(n, c_int) for n in ("num_heads", "num_kv_heads", "head_dim", "page_size", "dtype", "window", "max_requests",
+                                     "max_tokens")]
+
+
 _PP = ctypes.POINTER(c_void_p)
+_SHAPE = ctypes.POINTER(AttentionShape)
 _GEMM_SIGS: dict = {
     "sb200_gemm_colpar": (_I, [_P, _L, _P, _L, _P, _L, _P, _P, _L, _L, _L, _L, _I, _I, ctypes.POINTER(RotaryArgs), _P, _I,
                                _P, _L, _P]),
@@ -53,6 +60,12 @@ _GEMM_SIGS: dict = {
     "sb200_gemm_choices_made": (_L, []),
     "sb200_kv_cache_slots": (_I, [_P, _P, _P, _P, _P, _L, _I, _P]),
     "sb200_kv_cache_append": (_I, [_P, _P, _L, _P, _L, _P, _L, _I, _I, _I, _I, _P]),
+    "sb200_resize_block_tables": (_I, [_P, _L, _P, _P, _P, _P, _P, _I, _I, _L, _I, _P]),
+    "sb200_batch_layout": (_I, [_P, _P, _P, _L, _I, _I, _I, _L, _L, _P, _P, _P, _P, _L, _P, _P, _P, _P, _P]),
+    "sb200_attention_plan_bytes": (_L, [_SHAPE]),
+    "sb200_attention_workspace_bytes": (_L, [_SHAPE]),
+    "sb200_attention_plan": (_I, [_P, _L, _SHAPE, _P, _P, _P, _I, _L, _P]),
+    "sb200_paged_attention": (_I, [_P, _L, _P, _P, _L, _L, _P, _L, _P, _SHAPE, _P, _L, _F, _I, _P, _L, _P, _P]),
     "sb200_diag_mma_rate": (_I, [_I, _I, _I, _P, _P]),
     "sb200_comm_heap_bytes": (_L, [_L]),
     "sb200_comm_create": (_I, [_PP, _I, _I, _L]),
@@ -155,6 +168,15 @@ def require_cuda(*tensors: torch.Tensor) -> None:
     for t in tensors:
         if t is not None and not t.is_cuda:
             raise RuntimeError("sarathi_serve_b200 ops run on CUDA tensors only (no CPU fallback)")
+
+
+def require_current(*tensors: torch.Tensor) -> None:
+    """Kernels run on the current device and its current stream: refuse tensors that live on another one."""
+    require_cuda(*tensors)
+    here = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.get_device() != here:
+            raise RuntimeError(f"sarathi_serve_b200: a tensor is on cuda:{t.get_device()}, the current device is cuda:{here}")
 
 
 def ptr(t):

@@ -1,0 +1,399 @@
+// Attention of a step's new tokens over the paged KV cache: the plan kernel, the join of cut units, the C entry points.
+// attention.cuh has the division of the work, attention_simt.cu the fp32 kernel, attention_tc.cu the tensor-core kernel.
+//
+// Replaces the flashinfer calls of the reference's attention wrapper
+// (sarathi/model_executor/attention/flashinfer_attention_wrapper.py:240-299: one paged prefill wrapper for prompt chunks
+// and decodes, planned once a step in begin_forward and run by every layer).
+#include "attention.cuh"
+
+namespace sb200 {
+
+constexpr int kPlanThreads = 1024;
+
+struct PlanArgs {
+  AttnPlanView plan;
+  const int32_t *qo_indptr, *kv_lens, *kv_indptr;
+  int64_t num_kv_indices;
+  int n, workers, max_tokens;
+  AttnShape sh;
+};
+
+// What a block of keys, and a unit apart from its blocks, costs a CTA: see the measurements in attention_tc.cu.
+__device__ __forceinline__ void unit_cost(int kind, int nrows, int* block, int* fixed, int* least) {
+  if (kind == ATTN_MANY) { *block = nrows > 128 ? 8 : 6; *fixed = 12; *least = 2; }
+  else if (kind == ATTN_FEW) { *block = 8; *fixed = 4; *least = 2; }
+  else { *block = 8; *fixed = 2; *least = 1; }
+}
+
+__device__ __forceinline__ long long scan_block(long long v, long long* red, long long* total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  long long x = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
+  }
+  __syncthreads();
+  if (lane == 31) red[warp] = x;
+  __syncthreads();
+  if (warp == 0) {
+    long long s = red[lane];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long y = __shfl_up_sync(0xffffffffu, s, o);
+      if (lane >= o) s += y;
+    }
+    red[lane] = s;
+  }
+  __syncthreads();
+  *total = red[31];
+  return x - v + (warp ? red[warp - 1] : 0);
+}
+
+// One CTA: tiles per request (prefix sum over the requests), then the tiles and their costs (prefix sum over the tiles,
+// 1024 at a time), then the start of every worker's share (binary search).  Made once a step, read by every layer.
+__global__ void __launch_bounds__(kPlanThreads)
+attn_plan_kernel(const PlanArgs a) {
+  grid_dependency_begin();
+  extern __shared__ int smem_i[];
+  int* first = smem_i;  // [n + 1] first tile of every request
+  __shared__ long long red[33];
+  const AttnShape& sh = a.sh;
+  const int per = (a.n + kPlanThreads - 1) / kPlanThreads, r0 = min(a.n, (int)threadIdx.x * per), r1 = min(a.n, r0 + per);
+  auto span = [&](int r, int* q0) {
+    const int b = max(0, min(a.qo_indptr[r], a.max_tokens)), e = max(0, min(a.qo_indptr[r + 1], a.max_tokens));
+    *q0 = b;
+    return max(0, e - b);
+  };
+  auto kind_of = [&](int qlen, int* rows) {
+    const long long all = (long long)qlen * sh.group;
+    if (sh.few_limit < 0) { *rows = sh.rows_many; return (int)ATTN_SIMT; }
+    if (all <= sh.few_limit) { *rows = sh.rows_few; return (int)ATTN_FEW; }
+    *rows = sh.rows_many;
+    return (int)ATTN_MANY;
+  };
+  auto tiles_of = [&](int r) {
+    int q0, rows;
+    const int q = span(r, &q0);
+    kind_of(q, &rows);
+    return ((long long)q * sh.group + rows - 1) / rows;
+  };
+  long long s = 0, total;
+  for (int r = r0; r < r1; ++r) s += tiles_of(r);
+  long long p = scan_block(s, red, &total);
+  for (int r = r0; r < r1; ++r) {
+    first[r] = (int)min(p, (long long)a.plan.tiles_cap);
+    p += tiles_of(r);
+  }
+  const int tiles = (int)min(total, (long long)a.plan.tiles_cap);
+  if (threadIdx.x == 0) first[a.n] = tiles;
+  __syncthreads();
+
+  long long carry = 0;
+  for (int base = 0; base < tiles; base += kPlanThreads) {
+    const int t = base + threadIdx.x;
+    long long c = 0;
+    if (t < tiles) {
+      int lo = 0, hi = a.n;
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (first[mid] <= t) lo = mid;
+        else hi = mid - 1;
+      }
+      AttnTile d;
+      int rows;
+      const int q = span(lo, &d.q_row);
+      d.kind = kind_of(q, &rows);
+      d.row0 = (t - first[lo]) * rows;
+      d.nrows = (int)min((long long)rows, (long long)q * sh.group - d.row0);
+      // no more tokens than the listed pages have room for, whatever the length says
+      const long long at0 = min((long long)max(0, a.kv_indptr[lo]), (long long)a.num_kv_indices);
+      const long long at1 = min((long long)max(0, a.kv_indptr[lo + 1]), (long long)a.num_kv_indices);
+      const long long room = min(max(0ll, at1 - at0) * sh.page_size, 1ll << 30);
+      const int len = (int)min((long long)max(0, a.kv_lens[lo]), room);
+      d.pos0 = len - q;
+      d.page_at = (int)at0;
+      const int tok0 = d.row0 / sh.group, tok1 = (d.row0 + d.nrows - 1) / sh.group;
+      const int seen_hi = max(0, d.pos0 + tok1 + 1);
+      const int seen_lo = sh.window > 0 ? max(0, d.pos0 + tok0 + 1 - sh.window) : 0;
+      d.blk_lo = seen_lo / kAttnBlock;
+      d.nblk = max(0, (seen_hi + kAttnBlock - 1) / kAttnBlock - d.blk_lo);
+      int4* dst = reinterpret_cast<int4*>(a.plan.tiles + t);
+      dst[0] = make_int4(d.q_row, d.row0, d.nrows, d.kind);
+      dst[1] = make_int4(d.pos0, d.page_at, d.blk_lo, d.nblk);
+      int block, fixed, least;
+      unit_cost(d.kind, d.nrows, &block, &fixed, &least);
+      c = ((long long)d.nblk * block + fixed) * sh.kv_heads;
+    }
+    const long long at = carry + scan_block(c, red, &total);
+    if (t < tiles) a.plan.cost[t] = at;
+    carry += total;
+  }
+  if (threadIdx.x == 0) {
+    a.plan.cost[tiles] = carry;
+    a.plan.header[0] = tiles;
+    a.plan.header[1] = a.workers;
+    a.plan.header[2] = a.n ? max(0, min(a.qo_indptr[a.n], a.max_tokens)) : 0;
+  }
+  __syncthreads();
+  for (int w = threadIdx.x; w <= a.workers; w += kPlanThreads) {
+    int4 out = make_int4(tiles, 0, 0, 0);
+    if (w < a.workers && tiles > 0) {
+      const long long x = carry * w / a.workers;
+      int lo = 0, hi = tiles - 1;
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (a.plan.cost[mid] <= x) lo = mid;
+        else hi = mid - 1;
+      }
+      const AttnTile d = a.plan.tiles[lo];
+      int block, fixed, least;
+      unit_cost(d.kind, d.nrows, &block, &fixed, &least);
+      const long long unit = (long long)d.nblk * block + fixed, rem = x - a.plan.cost[lo];
+      int head = (int)(rem / unit);
+      const long long in = rem - head * unit;
+      int blk = in <= fixed / 2 ? 0 : (int)min((in - fixed / 2 + block / 2) / block, (long long)d.nblk);
+      // no piece of less than `least` blocks: the cut moves to the end of the unit it is near to
+      if (blk < least) blk = 0;
+      else if (d.nblk - blk < least) { blk = 0; ++head; }
+      out = head < sh.kv_heads ? make_int4(lo, head, blk, 0) : make_int4(lo + 1, 0, 0, 0);
+    }
+    a.plan.starts[w] = out;
+  }
+}
+
+// Joins the pieces of cut units: o = sum_p 2^(l_p - m) o_p / sum_p 2^(l_p - m) with l_p the log2 of piece p's sum, in the
+// order of the keys.  CTA (x, y): the unit that worker x's share begins inside of, if it is the first such worker, rows
+// y, y + gridDim.y ... of it, a warp per row.  Also clears the rows of q that belong to no request, when asked to.
+template <typename T, int HD>
+__global__ void __launch_bounds__(128)
+attn_join_kernel(const AttnArgs a) {
+  grid_dependency_begin();
+  constexpr int N = HD / 32;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int workers = a.plan.header[1];
+  T* out = reinterpret_cast<T*>(a.out);
+  if (a.zero_behind) {
+    const int rows0 = min(a.plan.header[2], a.num_tokens), per_row = a.kv_heads * a.group * HD;
+    const int ctas = gridDim.x * gridDim.y, cta = blockIdx.y * gridDim.x + blockIdx.x;
+    for (int t = rows0 + cta; t < a.num_tokens; t += ctas) {
+      for (int i = threadIdx.x; i < per_row; i += blockDim.x) out[t * a.ldo + i] = DT<T>::from_f(0.f);
+      if (a.lse)
+        for (int i = threadIdx.x; i < a.kv_heads * a.group; i += blockDim.x)
+          a.lse[(int64_t)t * (a.kv_heads * a.group) + i] = -INFINITY;
+    }
+  }
+  const int w = blockIdx.x + 1;
+  if (w >= workers) return;
+  const int4 at = a.plan.starts[w], before = a.plan.starts[w - 1];
+  if (at.z == 0 || (before.x == at.x && before.y == at.y && before.z > 0)) return;
+  int last = w;  // the workers w .. last begin inside this unit
+  while (last + 1 < workers) {
+    const int4 n = a.plan.starts[last + 1];
+    if (n.x != at.x || n.y != at.y) break;
+    ++last;
+  }
+  AttnPiece p;
+  p.t = a.plan.tiles[at.x];
+  p.head = at.y;
+  const int rows = (int)min((long long)p.t.nrows, max(0ll, ((long long)a.num_tokens - p.t.q_row) * a.group - p.t.row0));
+  for (int r = blockIdx.y * 4 + warp; r < rows; r += gridDim.y * 4) {
+    // piece 0 is the last of worker w - 1, piece i > 0 the first of worker w + i - 1 (none, if the next one begins there too)
+    const int pieces = last - w + 2;
+    auto slot = [&](int i) { return i == 0 ? 2 * (w - 1) + 1 : 2 * (w + i - 1); };
+    auto lse_of = [&](int i) {
+      if (i > 0 && i + 1 < pieces) {
+        const int4 x = a.plan.starts[w + i - 1], y = a.plan.starts[w + i];
+        if (x.x == y.x && x.y == y.y && x.z == y.z) return -INFINITY;
+      }
+      return a.part_l[(int64_t)slot(i) * a.slot_rows + r];
+    };
+    float m = -INFINITY;
+    for (int i = lane; i < pieces; i += 32) m = fmaxf(m, lse_of(i));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const float base = m == -INFINITY ? 0.f : m;
+    float acc[N] = {}, sum = 0.f;
+    for (int i0 = 0; i0 < pieces; i0 += 32) {
+      const float mine = i0 + lane < pieces ? exp2f(lse_of(i0 + lane) - base) : 0.f;
+      sum += warp_sum(mine);
+      const int n = min(32, pieces - i0);
+#pragma unroll 4
+      for (int i = 0; i < n; ++i) {
+        const float wt = __shfl_sync(0xffffffffu, mine, i);
+        if (wt == 0.f) continue;  // (a piece that this row sees nothing of)
+        const float* o = a.part_o + ((int64_t)slot(i0 + i) * a.slot_rows + r) * HD + lane * N;
+#pragma unroll
+        for (int j = 0; j < N; ++j) acc[j] += wt * o[j];
+      }
+    }
+    int token, head, pos;
+    attn_row(a, p, r, &token, &head, &pos);
+    const float inv = attn_inverse(sum, pos);
+    T* dst = out + token * a.ldo + head * HD + lane * N;
+#pragma unroll
+    for (int j = 0; j < N; ++j) dst[j] = DT<T>::from_f(acc[j] * inv);
+    if (a.lse && lane == 0) a.lse[(int64_t)token * (a.kv_heads * a.group) + head] = (base + log2f(sum)) * 0.69314718055994531f;
+  }
+}
+
+// ------------------------------------------------------------------ host
+static int attn_shape(const sb200_attention_shape* s, AttnShape* sh, const char* what) {
+  SB_CHECK_ARG(s, "%s: null shape", what);
+  SB_CHECK_ARG(s->num_heads > 0 && s->num_kv_heads > 0 && s->num_heads % s->num_kv_heads == 0,
+               "%s: %d heads cannot share %d kv heads evenly", what, s->num_heads, s->num_kv_heads);
+  SB_CHECK_ARG(s->page_size > 0 && s->page_size <= (1 << 20) && s->window >= 0 && s->max_requests >= 0 && s->max_tokens >= 0 &&
+                   s->max_tokens <= (1 << 28) && s->num_heads <= (1 << 16) &&
+                   (int64_t)s->max_tokens * (s->num_heads / s->num_kv_heads) <= (1 << 30),
+               "%s: bad sizes", what);
+  if (s->head_dim != 64 && s->head_dim != 128 && s->head_dim != 256) {
+    set_error("%s: head size %d is not supported (64, 128 or 256)", what, s->head_dim);
+    return SB200_ERR_UNSUPPORTED;
+  }
+  if (s->max_requests > SB200_MAX_REQUESTS) {
+    set_error("%s: %d requests, at most %d are supported", what, s->max_requests, SB200_MAX_REQUESTS);
+    return SB200_ERR_UNSUPPORTED;
+  }
+  if (s->dtype != SB200_F32 && s->dtype != SB200_F16 && s->dtype != SB200_BF16) {
+    set_error("%s: unsupported dtype id %d", what, s->dtype);
+    return SB200_ERR_UNSUPPORTED;
+  }
+  sh->heads = s->num_heads;
+  sh->kv_heads = s->num_kv_heads;
+  sh->group = s->num_heads / s->num_kv_heads;
+  sh->head_dim = s->head_dim;
+  sh->page_size = s->page_size;
+  sh->dtype = s->dtype;
+  sh->window = s->window;
+  sh->rows_many = 32;
+  sh->rows_few = 32;
+  sh->few_limit = -1;
+  return SB200_OK;
+}
+
+// Tiles of at most `rows` rows: every request may end in a partial one.
+static int64_t tiles_cap(const AttnShape& sh, const sb200_attention_shape* s) {
+  return (int64_t)s->max_tokens * sh.group / sh.rows_many + s->max_requests + 1;
+}
+
+static size_t align16(size_t v) { return (v + 15) & ~size_t(15); }
+
+static size_t plan_view(void* base, int64_t cap, AttnPlanView* v) {
+  uint8_t* p = reinterpret_cast<uint8_t*>(base);
+  size_t at = 0;
+  v->header = reinterpret_cast<int*>(p + at);
+  at += kAttnHeaderInts * sizeof(int);
+  v->starts = reinterpret_cast<int4*>(p + at);
+  at += (kAttnMaxWorkers + 1) * sizeof(int4);
+  v->cost = reinterpret_cast<long long*>(p + at);
+  at += align16((size_t)(cap + 1) * sizeof(long long));
+  v->tiles = reinterpret_cast<AttnTile*>(p + at);
+  at += (size_t)cap * sizeof(AttnTile);
+  v->tiles_cap = (int)cap;
+  return at;
+}
+
+static int attn_workers() {
+  const int n = sm_count();
+  return n < kAttnMaxWorkers ? n : kAttnMaxWorkers;
+}
+
+static int slot_rows(const AttnShape& sh) { return sh.rows_many > sh.rows_few ? sh.rows_many : sh.rows_few; }
+
+template <typename T>
+static cudaError_t launch_join(int head_dim, const AttnArgs& a, dim3 grid, cudaStream_t s) {
+  if (head_dim == 64) return launch_dependent(attn_join_kernel<T, 64>, grid, dim3(128), 0, s, a);
+  if (head_dim == 128) return launch_dependent(attn_join_kernel<T, 128>, grid, dim3(128), 0, s, a);
+  return launch_dependent(attn_join_kernel<T, 256>, grid, dim3(128), 0, s, a);
+}
+
+}  // namespace sb200
+
+using namespace sb200;
+
+extern "C" int64_t sb200_attention_plan_bytes(const sb200_attention_shape* shape) {
+  AttnShape sh;
+  if (attn_shape(shape, &sh, "attention_plan_bytes")) return -1;
+  AttnPlanView v;
+  return (int64_t)plan_view(nullptr, tiles_cap(sh, shape), &v);
+}
+
+extern "C" int64_t sb200_attention_workspace_bytes(const sb200_attention_shape* shape) {
+  AttnShape sh;
+  if (attn_shape(shape, &sh, "attention_workspace_bytes")) return -1;
+  return (int64_t)2 * kAttnMaxWorkers * slot_rows(sh) * (sh.head_dim + 1) * sizeof(float);
+}
+
+extern "C" int sb200_attention_plan(void* plan, int64_t plan_bytes, const sb200_attention_shape* shape, const int32_t* qo_indptr,
+                                    const int32_t* kv_lens, const int32_t* kv_indptr, int num_requests, int64_t num_kv_indices,
+                                    sb200_stream_t stream) {
+  AttnShape sh;
+  if (int rc = attn_shape(shape, &sh, "attention_plan")) return rc;
+  SB_CHECK_ARG(num_requests >= 0 && num_requests <= shape->max_requests, "attention_plan: %d requests, made for at most %d",
+               num_requests, shape->max_requests);
+  PlanArgs a;
+  const size_t need = plan_view(plan, tiles_cap(sh, shape), &a.plan);
+  SB_CHECK_ARG(plan && aligned16(plan) && plan_bytes >= (int64_t)need, "attention_plan: the plan buffer must be 16-byte aligned and hold %lld bytes",
+               (long long)need);
+  SB_CHECK_ARG(qo_indptr && (num_requests == 0 || (kv_lens && kv_indptr)) && num_kv_indices >= 0 && num_kv_indices <= INT32_MAX,
+               "attention_plan: null pointer or bad number of page entries");
+  a.qo_indptr = qo_indptr;
+  a.kv_lens = kv_lens;
+  a.kv_indptr = kv_indptr;
+  a.num_kv_indices = num_kv_indices;
+  a.n = num_requests;
+  a.workers = attn_workers();
+  a.max_tokens = shape->max_tokens;
+  a.sh = sh;
+  const size_t smem = (size_t)(num_requests + 1) * sizeof(int);
+  SB_CUDA(launch_dependent(attn_plan_kernel, dim3(1), dim3(kPlanThreads), smem, (cudaStream_t)stream, a));
+  return SB200_OK;
+}
+
+extern "C" int sb200_paged_attention(void* out, int64_t ldo, float* lse, const void* q, int64_t ldq, int64_t num_tokens,
+                                     const void* cache, int64_t num_pages, const void* plan, const sb200_attention_shape* shape,
+                                     const int32_t* kv_indices, int64_t num_kv_indices, float scale, int zero_rows_behind,
+                                     void* workspace, int64_t workspace_bytes, uint32_t* status, sb200_stream_t stream) {
+  AttnShape sh;
+  if (int rc = attn_shape(shape, &sh, "paged_attention")) return rc;
+  SB_CHECK_ARG(num_tokens >= 0 && num_tokens <= shape->max_tokens, "paged_attention: %lld tokens, the plan is made for at most %d",
+               (long long)num_tokens, shape->max_tokens);
+  if (num_tokens == 0) return SB200_OK;
+  const int64_t row = (int64_t)sh.heads * sh.head_dim;
+  const int64_t es = (int64_t)dtype_size(sh.dtype);
+  SB_CHECK_ARG(out && q && plan && (cache || num_pages == 0) && (kv_indices || num_kv_indices == 0), "paged_attention: null pointer");
+  SB_CHECK_ARG(ldq >= row && ldo >= row && aligned16(q) && aligned16(out) && aligned16(cache) && (ldq * es) % 16 == 0 && (ldo * es) % 16 == 0,
+               "paged_attention: rows of q and out must be 16-byte aligned and at least %lld elements apart", (long long)row);
+  SB_CHECK_ARG(num_pages >= 0 && num_kv_indices >= 0 && num_pages * 2 * sh.page_size <= INT32_MAX, "paged_attention: bad cache of %lld pages",
+               (long long)num_pages);
+  SB_CHECK_ARG(workspace && aligned16(workspace) && workspace_bytes >= sb200_attention_workspace_bytes(shape),
+               "paged_attention: the workspace must be 16-byte aligned and hold %lld bytes", (long long)sb200_attention_workspace_bytes(shape));
+  SB_CHECK_ARG(isfinite(scale), "paged_attention: the scale is not a finite number");
+  AttnArgs a = {};
+  plan_view(const_cast<void*>(plan), tiles_cap(sh, shape), &a.plan);
+  a.q = q; a.ldq = ldq; a.out = out; a.ldo = ldo; a.lse = lse; a.cache = cache;
+  a.kv_indices = kv_indices;
+  a.num_kv_indices = num_kv_indices;
+  a.num_pages = (int)num_pages;
+  a.num_tokens = (int)num_tokens;
+  a.kv_heads = sh.kv_heads;
+  a.group = sh.group;
+  a.page_size = sh.page_size;
+  a.page_shift = -1;
+  for (int b = 0; b < 31; ++b)
+    if ((1 << b) == sh.page_size) a.page_shift = b;
+  a.window = sh.window;
+  a.slot_rows = slot_rows(sh);
+  a.part_o = reinterpret_cast<float*>(workspace);
+  a.part_l = a.part_o + (size_t)2 * kAttnMaxWorkers * a.slot_rows * sh.head_dim;
+  a.status = status;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  a.zero_behind = zero_rows_behind;
+  const int workers = attn_workers();
+  cudaStream_t s = (cudaStream_t)stream;
+  if (int rc = run_attn_simt(sh.dtype, sh.head_dim, a, workers, s)) return rc;
+  // rows of a slot over four warps each
+  const dim3 grid((unsigned)workers, (unsigned)(a.slot_rows >= 128 ? 8 : a.slot_rows >= 32 ? 2 : 1));
+  SB_DISPATCH_FLOAT(sh.dtype, SB_CUDA(launch_join<scalar_t>(sh.head_dim, a, grid, s)));
+  return SB200_OK;
+}

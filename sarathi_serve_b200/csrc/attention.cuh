@@ -1,0 +1,130 @@
+// What the attention kernels share: the plan of a step (which CTA does which rows against which keys), the addressing of
+// the paged cache, and where a piece of work leaves its result.
+//
+//   o_i = sum_j p_ij v_j / sum_j p_ij,   p_ij = exp(scale q_i . k_j - m_i),   j <= pos_i  (and j > pos_i - window)
+//
+// A query row is a (token, q head) pair.  The `group` q heads that share a kv head also share its keys and values, so
+// the rows of a request for one kv head are (token, head of the group) pairs, token-major, and a TILE is a run of them.  A
+// UNIT is a tile for one kv head; its keys come in blocks of 128.  Units are laid end to end, tile by tile and head by
+// head, weighted by what a block costs, and every CTA (one per SM) gets an equal share of that line: long contexts are cut
+// wherever a share ends, short ones are not cut at all.  A PIECE is the part of a unit that one CTA does.  A piece that is
+// a whole unit writes the output; the others leave (o / l, log2-sum) in fp32 in a workspace, and a second kernel joins the
+// pieces of each cut unit in the order of their keys.  A CTA has at most two such pieces, its first and its last, so
+// the workspace has two slots per CTA, and the result does not depend on timing.
+#pragma once
+
+#include "common.cuh"
+#include "sm100_ptx.cuh"
+
+namespace sb200 {
+
+constexpr int kAttnBlock = 128;       // keys of a block
+constexpr int kAttnMaxWorkers = 256;  // (B200: 148 SMs)
+constexpr int kAttnHeaderInts = 16;
+
+// How the rows of a tile are computed.
+enum { ATTN_SIMT = 0, ATTN_FEW = 1, ATTN_MANY = 2 };
+
+struct AttnTile {
+  int q_row;    // first row of the request's tokens in q
+  int row0;     // first (token, head of the group) row of the tile
+  int nrows;
+  int kind;
+  int pos0;     // position of the request's first new token (negative: more new tokens than the cache is said to hold)
+  int page_at;  // first entry of the request's pages in kv_indices
+  int blk_lo, nblk;  // blocks of keys that some row sees
+};
+
+struct AttnPlanView {
+  int* header;       // number of tiles, workers, rows of q that belong to a request
+  int4* starts;      // [workers + 1] (tile, head, block): where each worker's share begins
+  long long* cost;   // [tiles + 1] start of every tile on the line
+  AttnTile* tiles;
+  int tiles_cap;
+};
+
+struct AttnShape {
+  int heads, kv_heads, group, head_dim, page_size, dtype, window;
+  int rows_many;   // rows of a tile, and up to how many rows a request takes the kernel for few rows
+  int rows_few;
+  int few_limit;   // -1: every tile is ATTN_SIMT
+};
+
+struct AttnArgs {
+  AttnPlanView plan;
+  const void* q; int64_t ldq;
+  void* out; int64_t ldo;
+  float* lse;
+  const void* cache;
+  const int32_t* kv_indices;
+  float* part_o;       // [2 workers][slot_rows][head_dim]
+  float* part_l;       // [2 workers][slot_rows]
+  uint32_t* status;
+  int64_t num_kv_indices;
+  int num_pages, num_tokens;
+  int kv_heads, group, page_size, window, slot_rows;
+  int page_shift;      // log2(page_size), or -1
+  float scale_log2;    // scale * log2(e): scores in powers of two
+  int zero_behind;
+};
+
+struct AttnPiece {
+  AttnTile t;
+  int head, b0, b1;   // blocks [b0, b1) of the tile's nblk
+  int slot;           // -1: the whole unit
+  int lo, hi;         // keys [lo, hi) that some row of the tile sees
+};
+
+// Walks a worker's share of the line.
+struct AttnWalk {
+  int4 cur, end;
+  int worker;
+  __device__ __forceinline__ AttnWalk(const AttnArgs& a, int w) : cur(a.plan.starts[w]), end(a.plan.starts[w + 1]), worker(w) {}
+  __device__ __forceinline__ bool next(const AttnArgs& a, AttnPiece* p) {
+    if (cur.x > end.x || (cur.x == end.x && (cur.y > end.y || (cur.y == end.y && cur.z >= end.z)))) return false;
+    const int4* src = reinterpret_cast<const int4*>(a.plan.tiles + cur.x);
+    const int4 u = src[0], v = src[1];
+    p->t = AttnTile{u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+    p->head = cur.y;
+    p->b0 = cur.z;
+    p->b1 = cur.x == end.x && cur.y == end.y ? end.z : p->t.nblk;
+    const bool head_cut = p->b0 > 0, tail_cut = p->b1 < p->t.nblk;
+    p->slot = head_cut ? 2 * worker : tail_cut ? 2 * worker + 1 : -1;
+    // q may have fewer rows than the plan was made for
+    p->t.nrows = min((long long)p->t.nrows, max(0ll, ((long long)a.num_tokens - p->t.q_row) * a.group - p->t.row0));
+    const int first = p->t.row0 / a.group, last = (p->t.row0 + max(p->t.nrows, 1) - 1) / a.group;
+    p->hi = max(0, p->t.pos0 + last + 1);
+    p->lo = a.window > 0 ? max(0, p->t.pos0 + first + 1 - a.window) : 0;
+    if (cur.y + 1 < a.kv_heads) cur = make_int4(cur.x, cur.y + 1, 0, 0);
+    else cur = make_int4(cur.x + 1, 0, 0, 0);
+    return true;
+  }
+};
+
+// Cache row (of kv_heads * head_dim elements) of a key, or -1 where its page is not one of the cache's: such a page reads
+// as zeros, so that a bad table cannot reach outside.  The value is page_size rows further.
+__device__ __forceinline__ int attn_key_row(const AttnArgs& a, int page_at, int key) {
+  const int p = a.page_shift >= 0 ? key >> a.page_shift : key / a.page_size;
+  const long long at = (long long)page_at + p;
+  const int page = at >= 0 && at < a.num_kv_indices ? a.kv_indices[at] : -1;
+  return (unsigned)page < (unsigned)a.num_pages ? page * 2 * a.page_size + (key - p * a.page_size) : -1;
+}
+
+// Where row r of a piece's tile goes: (token row, q head).
+__device__ __forceinline__ void attn_row(const AttnArgs& a, const AttnPiece& p, int r, int* token, int* head, int* pos) {
+  const int row = p.t.row0 + r, tok = row / a.group;
+  *token = p.t.q_row + tok;
+  *head = p.head * a.group + (row - tok * a.group);
+  *pos = p.t.pos0 + tok;
+}
+
+// Of a sum that came out as zero: nothing to see gives zeros, keys with scores of minus infinity only are 0 / 0.
+__device__ __forceinline__ float attn_inverse(float l, int pos) {
+  if (l > 0.f || l != l) return 1.f / l;
+  return pos < 0 ? 0.f : __int_as_float(0x7fc00000);
+}
+
+int run_attn_simt(int dtype, int head_dim, const AttnArgs& a, int workers, cudaStream_t s);
+int run_attn_tc(int dtype, int head_dim, const AttnArgs& a, const AttnShape& sh, int workers, cudaStream_t s);
+
+}  // namespace sb200

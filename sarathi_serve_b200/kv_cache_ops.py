@@ -5,10 +5,14 @@
 
 ``slots`` computes, once per step, the cache row of every token; ``append_paged_kv_cache`` copies
 strided k / v views (no ``.contiguous()``) there.  ``dense_ops.linear_rotary(..., kv_cache=, kv_slots=)``
-stores k and v from the qkv GEMM's epilogue instead, so that only ``slots`` remains as a launch."""
+stores k and v from the qkv GEMM's epilogue instead, so that only ``slots`` remains as a launch.
+
+``resize_block_tables`` and ``batch_layout`` make a step's block tables and index arrays on the GPU, from the lengths of
+its requests: what the reference's block manager and its wrapper's ``begin_forward`` do in host loops.  Neither reads
+anything back, so both can be captured into the CUDA graph of a step."""
 from __future__ import annotations
 
-from typing import Optional
+from typing import NamedTuple, Optional
 
 import torch
 
@@ -65,3 +69,99 @@ def append_paged_kv_cache(append_key: torch.Tensor, append_value: torch.Tensor, 
         raise RuntimeError("append_paged_kv_cache: only the NHD layout of the reference's cache is supported")
     s = slots(batch_indices, positions, kv_indices, kv_indptr, paged_kv_cache.shape[2])
     append_rows(paged_kv_cache, append_key, append_value, s)
+
+
+def _int32(name: str, t: torch.Tensor, n: int, what: str) -> None:
+    if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous() or (n >= 0 and t.numel() != n):
+        raise RuntimeError(f"{what}: {name} must be a contiguous int32 tensor" + (f" of {n} elements" if n >= 0 else ""))
+
+
+def _tables(block_tables: torch.Tensor, n: int, what: str) -> None:
+    if block_tables.dtype != torch.int32 or block_tables.dim() != 2 or block_tables.shape[0] != n:
+        raise RuntimeError(f"{what}: block_tables must be an int32 tensor [{n}, blocks]")
+    if (block_tables.shape[1] > 1 and block_tables.stride(1) != 1) or (n > 1 and block_tables.stride(0) < block_tables.shape[1]):
+        raise RuntimeError(f"{what}: the rows of block_tables must have unit inner stride and must not overlap")
+
+
+def _table_stride(block_tables: torch.Tensor) -> int:
+    return block_tables.stride(0) if block_tables.shape[0] > 1 else block_tables.shape[1]
+
+
+def resize_block_tables(block_tables: torch.Tensor, num_blocks: torch.Tensor, seq_lens: torch.Tensor, free_blocks: torch.Tensor,
+                        num_free: torch.Tensor, page_size: int, granted: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Make the block tables fit the requests' lengths, in place: afterwards request r owns ceil(seq_lens[r] / page_size)
+    pages, entries [0, num_blocks[r]) of ``block_tables`` [n, blocks].  A request that shrinks (``seq_lens[r] = 0``: it has
+    finished) pushes its last pages on the stack ``free_blocks[:num_free]``; then requests that grow pop theirs from its top,
+    in request order.  Returns ``granted`` int32 [n]: 0 where the stack (or the table's width) did not suffice and the request
+    was left as it was -- from the first such request on, none that needs pages gets any, unless it was its own table that was
+    too narrow.  A negative length leaves a request alone.  All tensors int32 on the GPU; ``num_free`` has one element."""
+    what = "resize_block_tables"
+    N.require_current(block_tables, num_blocks, seq_lens, free_blocks, num_free, granted)
+    n = num_blocks.numel()
+    _tables(block_tables, n, what)
+    for name, t, k in (("num_blocks", num_blocks, n), ("seq_lens", seq_lens, n), ("free_blocks", free_blocks, -1),
+                       ("num_free", num_free, 1)):
+        _int32(name, t, k, what)
+    if granted is None:
+        granted = torch.empty(n, dtype=torch.int32, device=num_blocks.device)
+    else:
+        _int32("granted", granted, n, what)
+    N.check(N.lib().sb200_resize_block_tables(N.ptr(block_tables), _table_stride(block_tables), N.ptr(num_blocks), N.ptr(seq_lens),
+                                              N.ptr(free_blocks), N.ptr(num_free), N.ptr(granted), n, block_tables.shape[1],
+                                              free_blocks.numel(), int(page_size), N.stream_ptr()), what)
+    return granted
+
+
+class BatchLayout(NamedTuple):
+    """Index arrays of a step (see ``batch_layout``)."""
+    qo_indptr: torch.Tensor      # int32 [n + 1]
+    kv_lens: torch.Tensor        # int32 [n]
+    kv_indptr: torch.Tensor      # int32 [n + 1]
+    kv_indices: torch.Tensor     # int32 [n * blocks]
+    last_page_len: torch.Tensor  # int32 [n]
+    batch_indices: torch.Tensor  # int32 [num_tokens]
+    positions: torch.Tensor      # int64 [num_tokens]
+    kv_slots: torch.Tensor       # int64 [num_tokens]
+
+
+def batch_layout(query_lens: torch.Tensor, context_lens: torch.Tensor, block_tables: torch.Tensor, page_size: int, num_pages: int,
+                 num_tokens: int, out: Optional[BatchLayout] = None) -> BatchLayout:
+    """Index arrays of a step in which request r adds ``query_lens[r]`` tokens to the ``context_lens[r]`` it has in the cache,
+    all new tokens one after the other in a batch padded to ``num_tokens`` rows: row offsets (``qo_indptr``), lengths
+    (``kv_lens``), page lists in the form of flashinfer's plan (``kv_indptr``, ``kv_indices``, ``last_page_len``; -1 behind the
+    last page), and for every row its request (-1: padding), position and cache slot (-1: padding, or a page outside
+    ``[0, num_pages)``).  ``positions`` goes to the rotary embedding, ``kv_slots`` to the append, everything to
+    ``attention_ops.AttentionPlan.update``.
+
+    Negative lengths count as zero.  A context is cut to what its block table has room for, and the new tokens to what is then
+    left of it and of ``num_tokens``.  ``out``: the result of an earlier call of the same sizes, written again (buffers of a CUDA
+    graph)."""
+    what = "batch_layout"
+    n = query_lens.numel()
+    N.require_current(query_lens, context_lens, block_tables)
+    _int32("query_lens", query_lens, n, what)
+    _int32("context_lens", context_lens, n, what)
+    _tables(block_tables, n, what)
+    T, width, dev = int(num_tokens), block_tables.shape[1], query_lens.device
+    if T < 0:
+        raise RuntimeError(f"{what}: num_tokens is negative")
+    if out is None:
+        # one allocation each for the two types; int32 parts one after the other
+        ints = torch.empty(4 * n + 2 + n * width + T, dtype=torch.int32, device=dev)
+        a, b, c, d, e, f = ints.split([n + 1, n, n + 1, n * width, n, T])
+        longs = torch.empty(2, T, dtype=torch.int64, device=dev)
+        out = BatchLayout(a, b, c, d, e, f, longs[0], longs[1])
+    else:
+        N.require_current(*out)
+        for name, t, k in zip(BatchLayout._fields, out, (n + 1, n, n + 1, -1, n, T)):
+            _int32("out." + name, t, k, what)
+        if out.kv_indices.numel() < n * width:
+            raise RuntimeError(f"{what}: out.kv_indices must hold {n * width} entries")
+        for t in out[6:]:
+            if t.dtype != torch.int64 or t.shape != (T,) or not t.is_contiguous():
+                raise RuntimeError(f"{what}: out.positions and out.kv_slots must be contiguous int64 tensors of {T} elements")
+    N.check(N.lib().sb200_batch_layout(N.ptr(query_lens), N.ptr(context_lens), N.ptr(block_tables), _table_stride(block_tables), n, width,
+                                       int(page_size), int(num_pages), T, N.ptr(out.qo_indptr), N.ptr(out.kv_lens),
+                                       N.ptr(out.kv_indptr), N.ptr(out.kv_indices), out.kv_indices.numel(), N.ptr(out.last_page_len),
+                                       N.ptr(out.batch_indices), N.ptr(out.positions), N.ptr(out.kv_slots), N.stream_ptr()), what)
+    return out
