@@ -265,9 +265,9 @@ static int attn_shape(const sb200_attention_shape* s, AttnShape* sh, const char*
   sh->page_size = s->page_size;
   sh->dtype = s->dtype;
   sh->window = s->window;
-  sh->rows_many = 32;
-  sh->rows_few = 32;
-  sh->few_limit = -1;
+  sh->rows_many = s->dtype == SB200_F32 ? 32 : 16;
+  sh->rows_few = 16;
+  sh->few_limit = s->dtype == SB200_F32 ? -1 : INT32_MAX;
   return SB200_OK;
 }
 
@@ -391,7 +391,9 @@ extern "C" int sb200_paged_attention(void* out, int64_t ldo, float* lse, const v
   a.zero_behind = zero_rows_behind;
   const int workers = attn_workers();
   cudaStream_t s = (cudaStream_t)stream;
-  if (int rc = run_attn_simt(sh.dtype, sh.head_dim, a, workers, s)) return rc;
+  if (int rc = sh.dtype == SB200_F32 ? run_attn_simt(sh.head_dim, a, workers, s)
+                                     : run_attn_tc(sh.dtype, sh.head_dim, a, sh, workers, s))
+    return rc;
   // rows of a slot over four warps each
   const dim3 grid((unsigned)workers, (unsigned)(a.slot_rows >= 128 ? 8 : a.slot_rows >= 32 ? 2 : 1));
   SB_DISPATCH_FLOAT(sh.dtype, SB_CUDA(launch_join<scalar_t>(sh.head_dim, a, grid, s)));

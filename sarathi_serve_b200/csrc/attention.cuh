@@ -124,7 +124,7 @@ __device__ __forceinline__ float attn_inverse(float l, int pos) {
   return pos < 0 ? 0.f : __int_as_float(0x7fc00000);
 }
 
-int run_attn_simt(int dtype, int head_dim, const AttnArgs& a, int workers, cudaStream_t s);
+int run_attn_simt(int head_dim, const AttnArgs& a, int workers, cudaStream_t s);
 int run_attn_tc(int dtype, int head_dim, const AttnArgs& a, const AttnShape& sh, int workers, cudaStream_t s);
 
 }  // namespace sb200

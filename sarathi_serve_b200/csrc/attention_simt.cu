@@ -145,11 +145,10 @@ static int launch_simt(const AttnArgs& a, int workers, cudaStream_t s) {
   return SB200_OK;
 }
 
-int run_attn_simt(int dtype, int head_dim, const AttnArgs& a, int workers, cudaStream_t s) {
-  SB_DISPATCH_FLOAT(dtype, return head_dim == 64    ? launch_simt<scalar_t, 64>(a, workers, s)
-                                  : head_dim == 128 ? launch_simt<scalar_t, 128>(a, workers, s)
-                                                    : launch_simt<scalar_t, 256>(a, workers, s));
-  return SB200_OK;
+int run_attn_simt(int head_dim, const AttnArgs& a, int workers, cudaStream_t s) {
+  return head_dim == 64    ? launch_simt<float, 64>(a, workers, s)
+         : head_dim == 128 ? launch_simt<float, 128>(a, workers, s)
+                           : launch_simt<float, 256>(a, workers, s);
 }
 
 }  // namespace sb200
