@@ -56,7 +56,8 @@ __global__ void __launch_bounds__(kPlanThreads)
 attn_plan_kernel(const PlanArgs a) {
   grid_dependency_begin();
   extern __shared__ int smem_i[];
-  int* first = smem_i;  // [n + 1] first tile of every request
+  int* first = smem_i;               // [n + 1] first tile of every request that has tiles of many rows (or the only kind),
+  int* few = smem_i + a.n + 1;       // and of those with few: these come behind all others
   __shared__ long long red[33];
   const AttnShape& sh = a.sh;
   const int per = (a.n + kPlanThreads - 1) / kPlanThreads, r0 = min(a.n, (int)threadIdx.x * per), r1 = min(a.n, r0 + per);
@@ -72,21 +73,28 @@ attn_plan_kernel(const PlanArgs a) {
     *rows = sh.rows_many;
     return (int)ATTN_MANY;
   };
-  auto tiles_of = [&](int r) {
+  const bool two = sh.few_limit >= 0 && sh.few_limit < INT32_MAX;
+  auto tiles_of = [&](int r, bool want_few) {
     int q0, rows;
     const int q = span(r, &q0);
-    kind_of(q, &rows);
-    return ((long long)q * sh.group + rows - 1) / rows;
+    const bool is_few = kind_of(q, &rows) == ATTN_FEW && two;
+    return is_few == want_few ? ((long long)q * sh.group + rows - 1) / rows : 0;
   };
-  long long s = 0, total;
-  for (int r = r0; r < r1; ++r) s += tiles_of(r);
-  long long p = scan_block(s, red, &total);
-  for (int r = r0; r < r1; ++r) {
-    first[r] = (int)min(p, (long long)a.plan.tiles_cap);
-    p += tiles_of(r);
+  long long total, many_total = 0;
+  for (int kind = 0; kind < 2; ++kind) {
+    int* at = kind ? few : first;
+    long long s = 0;
+    for (int r = r0; r < r1; ++r) s += tiles_of(r, kind);
+    long long p = scan_block(s, red, &total) + many_total;
+    for (int r = r0; r < r1; ++r) {
+      at[r] = (int)min(p, (long long)a.plan.tiles_cap);
+      p += tiles_of(r, kind);
+    }
+    total += many_total;
+    if (threadIdx.x == 0) at[a.n] = (int)min(total, (long long)a.plan.tiles_cap);
+    if (!kind) many_total = total;
   }
-  const int tiles = (int)min(total, (long long)a.plan.tiles_cap);
-  if (threadIdx.x == 0) first[a.n] = tiles;
+  const int tiles = (int)min(total, (long long)a.plan.tiles_cap), tiles_many = (int)min(many_total, (long long)a.plan.tiles_cap);
   __syncthreads();
 
   long long carry = 0;
@@ -94,17 +102,18 @@ attn_plan_kernel(const PlanArgs a) {
     const int t = base + threadIdx.x;
     long long c = 0;
     if (t < tiles) {
+      const int* begin = t < tiles_many ? first : few;
       int lo = 0, hi = a.n;
       while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
-        if (first[mid] <= t) lo = mid;
+        if (begin[mid] <= t) lo = mid;
         else hi = mid - 1;
       }
       AttnTile d;
       int rows;
       const int q = span(lo, &d.q_row);
       d.kind = kind_of(q, &rows);
-      d.row0 = (t - first[lo]) * rows;
+      d.row0 = (t - begin[lo]) * rows;
       d.nrows = (int)min((long long)rows, (long long)q * sh.group - d.row0);
       // no more tokens than the listed pages have room for, whatever the length says
       const long long at0 = min((long long)max(0, a.kv_indptr[lo]), (long long)a.num_kv_indices);
@@ -133,6 +142,7 @@ attn_plan_kernel(const PlanArgs a) {
     a.plan.cost[tiles] = carry;
     a.plan.header[0] = tiles;
     a.plan.header[1] = a.workers;
+    a.plan.header[3] = two ? tiles_many : 0;
     a.plan.header[2] = a.n ? max(0, min(a.qo_indptr[a.n], a.max_tokens)) : 0;
   }
   __syncthreads();
@@ -265,9 +275,13 @@ static int attn_shape(const sb200_attention_shape* s, AttnShape* sh, const char*
   sh->page_size = s->page_size;
   sh->dtype = s->dtype;
   sh->window = s->window;
-  sh->rows_many = s->dtype == SB200_F32 ? 32 : 16;
+  // Tiles of 256 rows on tcgen05 want a block of 128 keys to be whole boxes of whole swizzle atoms (8 rows); other pages, and
+  // heads of 256, whose two outputs and scores do not fit TMEM together, stay with tiles of 16 rows.
+  const bool boxes = (s->page_size % 8 == 0 && kAttnBlock % s->page_size == 0) || s->page_size % kAttnBlock == 0;
+  const bool many = s->dtype != SB200_F32 && s->head_dim <= 128 && boxes;
+  sh->rows_many = s->dtype == SB200_F32 ? 32 : many ? 256 : 16;
   sh->rows_few = 16;
-  sh->few_limit = s->dtype == SB200_F32 ? -1 : INT32_MAX;
+  sh->few_limit = s->dtype == SB200_F32 ? -1 : many ? 16 : INT32_MAX;
   return SB200_OK;
 }
 
@@ -321,7 +335,7 @@ extern "C" int64_t sb200_attention_plan_bytes(const sb200_attention_shape* shape
 extern "C" int64_t sb200_attention_workspace_bytes(const sb200_attention_shape* shape) {
   AttnShape sh;
   if (attn_shape(shape, &sh, "attention_workspace_bytes")) return -1;
-  return (int64_t)2 * kAttnMaxWorkers * slot_rows(sh) * (sh.head_dim + 1) * sizeof(float);
+  return (int64_t)2 * attn_workers() * slot_rows(sh) * (sh.head_dim + 1) * sizeof(float);
 }
 
 extern "C" int sb200_attention_plan(void* plan, int64_t plan_bytes, const sb200_attention_shape* shape, const int32_t* qo_indptr,
@@ -345,7 +359,8 @@ extern "C" int sb200_attention_plan(void* plan, int64_t plan_bytes, const sb200_
   a.workers = attn_workers();
   a.max_tokens = shape->max_tokens;
   a.sh = sh;
-  const size_t smem = (size_t)(num_requests + 1) * sizeof(int);
+  const size_t smem = 2 * (size_t)(num_requests + 1) * sizeof(int);
+  if (smem > 48 * 1024) SB_CUDA(cudaFuncSetAttribute(attn_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   SB_CUDA(launch_dependent(attn_plan_kernel, dim3(1), dim3(kPlanThreads), smem, (cudaStream_t)stream, a));
   return SB200_OK;
 }
@@ -361,10 +376,10 @@ extern "C" int sb200_paged_attention(void* out, int64_t ldo, float* lse, const v
   if (num_tokens == 0) return SB200_OK;
   const int64_t row = (int64_t)sh.heads * sh.head_dim;
   const int64_t es = (int64_t)dtype_size(sh.dtype);
-  SB_CHECK_ARG(out && q && plan && (cache || num_pages == 0) && (kv_indices || num_kv_indices == 0), "paged_attention: null pointer");
+  SB_CHECK_ARG(out && q && plan && cache && (kv_indices || num_kv_indices == 0), "paged_attention: null pointer");
   SB_CHECK_ARG(ldq >= row && ldo >= row && aligned16(q) && aligned16(out) && aligned16(cache) && (ldq * es) % 16 == 0 && (ldo * es) % 16 == 0,
                "paged_attention: rows of q and out must be 16-byte aligned and at least %lld elements apart", (long long)row);
-  SB_CHECK_ARG(num_pages >= 0 && num_kv_indices >= 0 && num_pages * 2 * sh.page_size <= INT32_MAX, "paged_attention: bad cache of %lld pages",
+  SB_CHECK_ARG(num_pages > 0 && num_kv_indices >= 0 && num_pages * 2 * sh.page_size <= INT32_MAX, "paged_attention: bad cache of %lld pages",
                (long long)num_pages);
   SB_CHECK_ARG(workspace && aligned16(workspace) && workspace_bytes >= sb200_attention_workspace_bytes(shape),
                "paged_attention: the workspace must be 16-byte aligned and hold %lld bytes", (long long)sb200_attention_workspace_bytes(shape));
@@ -385,7 +400,7 @@ extern "C" int sb200_paged_attention(void* out, int64_t ldo, float* lse, const v
   a.window = sh.window;
   a.slot_rows = slot_rows(sh);
   a.part_o = reinterpret_cast<float*>(workspace);
-  a.part_l = a.part_o + (size_t)2 * kAttnMaxWorkers * a.slot_rows * sh.head_dim;
+  a.part_l = a.part_o + (size_t)2 * attn_workers() * a.slot_rows * sh.head_dim;
   a.status = status;
   a.scale_log2 = scale * 1.4426950408889634f;
   a.zero_behind = zero_rows_behind;

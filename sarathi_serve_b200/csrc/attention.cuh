@@ -36,7 +36,7 @@ struct AttnTile {
 };
 
 struct AttnPlanView {
-  int* header;       // number of tiles, workers, rows of q that belong to a request
+  int* header;       // number of tiles, workers, rows of q that belong to a request, tiles of many rows (they come first)
   int4* starts;      // [workers + 1] (tile, head, block): where each worker's share begins
   long long* cost;   // [tiles + 1] start of every tile on the line
   AttnTile* tiles;
@@ -47,7 +47,7 @@ struct AttnShape {
   int heads, kv_heads, group, head_dim, page_size, dtype, window;
   int rows_many;   // rows of a tile, and up to how many rows a request takes the kernel for few rows
   int rows_few;
-  int few_limit;   // -1: every tile is ATTN_SIMT
+  int few_limit;   // -1: every tile is ATTN_SIMT; INT32_MAX: ATTN_FEW
 };
 
 struct AttnArgs {
@@ -80,8 +80,14 @@ struct AttnWalk {
   int4 cur, end;
   int worker;
   __device__ __forceinline__ AttnWalk(const AttnArgs& a, int w) : cur(a.plan.starts[w]), end(a.plan.starts[w + 1]), worker(w) {}
+  // Only the tiles before `tile`, or from it on.
+  __device__ __forceinline__ void until(int tile) { if (end.x >= tile) end = make_int4(tile, 0, 0, 0); }
+  __device__ __forceinline__ void from(int tile) { if (cur.x < tile) cur = make_int4(tile, 0, 0, 0); }
+  __device__ __forceinline__ bool more() const {
+    return cur.x < end.x || (cur.x == end.x && (cur.y < end.y || (cur.y == end.y && cur.z < end.z)));
+  }
   __device__ __forceinline__ bool next(const AttnArgs& a, AttnPiece* p) {
-    if (cur.x > end.x || (cur.x == end.x && (cur.y > end.y || (cur.y == end.y && cur.z >= end.z)))) return false;
+    if (!more()) return false;
     const int4* src = reinterpret_cast<const int4*>(a.plan.tiles + cur.x);
     const int4 u = src[0], v = src[1];
     p->t = AttnTile{u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};

@@ -182,6 +182,67 @@ __device__ __forceinline__ void tmem_ld_32x32(uint32_t taddr, uint32_t* r) {
       : "memory");
 }
 
+// 64 columns with two loads in flight.
+__device__ __forceinline__ void tmem_ld_32x64(uint32_t taddr, uint32_t* r) {
+  __syncwarp();
+#define SB_LD32(O, A) "tcgen05.ld.sync.aligned.32x32b.x32.b32 {" O "}, [" A "];\n\t"
+  asm volatile(
+      SB_LD32("%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+              "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31", "%64")
+      SB_LD32("%32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, "
+              "%48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63", "%65")
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]),
+        "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]),
+        "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]),
+        "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]),
+        "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
+      : "r"(taddr), "r"(taddr + 32)
+      : "memory");
+#undef SB_LD32
+}
+// The opposite direction: thread i writes 32 columns of lane (base_lane + i).  Visible to others after tmem_wait_st.
+__device__ __forceinline__ void tmem_st_32x32(uint32_t taddr, const uint32_t* r) {
+  __syncwarp();
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};"
+      ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+        "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
+        "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
+        "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]),
+        "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() {
+  __syncwarp();
+  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+// D[tmem] (+)= A[tmem] * B[smem]: A has 128 lanes (rows) and two 16-bit elements per column, K = 16 in 8 columns.
+__device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// Registers of a warpgroup (all four of its warps call this).  What the groups that grow take has to be given up by the
+// others: the sum must stay within threads x registers of the launch, or the call waits for good.
+template <int N> __device__ __forceinline__ void registers_grow() {
+  __syncwarp();
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N> __device__ __forceinline__ void registers_shrink() {
+  __syncwarp();
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+
 // ------------------------------------------------- CTA pairs (cta_group::2)
 // Two CTAs of a cluster cooperate on one 256-row tile: each holds 128 rows of A, half of the
 // B tile and its 128 accumulator rows; the MMA is issued by the even ("leader") CTA only.
@@ -284,6 +345,17 @@ __device__ __forceinline__ uint64_t make_smem_desc_sw128(uint32_t smem_addr) {
          | (1ull << 46)                           // descriptor version (Blackwell)
          | (2ull << 61);                          // layout: SWIZZLE_128B
 }
+
+// B operand whose rows are the K side ([K rows][64 columns] boxes with 128-byte swizzle): N runs along a row, 64 columns per
+// box, boxes `box_bytes` apart; K runs over the rows, 8 of them per 1024 bytes.  Goes with kIdescBRows in the descriptor.
+__device__ __forceinline__ uint64_t make_smem_desc_rows_sw128(uint32_t smem_addr, uint32_t box_bytes) {
+  return (uint64_t)((smem_addr & 0x3FFFFu) >> 4)
+         | ((uint64_t)(box_bytes >> 4) << 16)     // leading byte offset: to the next 64 columns
+         | (64ull << 32)                          // stride byte offset: to the next 8 rows
+         | (1ull << 46)
+         | (2ull << 61);
+}
+constexpr uint32_t kIdescBRows = 1u << 16;  // B is not K-major
 
 }  // namespace ptx
 }  // namespace sb200
