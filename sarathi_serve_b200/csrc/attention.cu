@@ -275,9 +275,9 @@ static int attn_shape(const sb200_attention_shape* s, AttnShape* sh, const char*
   sh->page_size = s->page_size;
   sh->dtype = s->dtype;
   sh->window = s->window;
-  // Tiles of 256 rows on tcgen05 want a block of 128 keys to be whole boxes of whole swizzle atoms (8 rows); other pages, and
+  // Tiles of 256 rows on tcgen05 want a step of 64 keys to be whole boxes of whole swizzle atoms (8 rows); other pages, and
   // heads of 256, whose two outputs and scores do not fit TMEM together, stay with tiles of 16 rows.
-  const bool boxes = (s->page_size % 8 == 0 && kAttnBlock % s->page_size == 0) || s->page_size % kAttnBlock == 0;
+  const bool boxes = (s->page_size % 8 == 0 && 64 % s->page_size == 0) || s->page_size % 64 == 0;
   const bool many = s->dtype != SB200_F32 && s->head_dim <= 128 && boxes;
   sh->rows_many = s->dtype == SB200_F32 ? 32 : many ? 256 : 16;
   sh->rows_few = 16;
@@ -394,9 +394,8 @@ extern "C" int sb200_paged_attention(void* out, int64_t ldo, float* lse, const v
   a.kv_heads = sh.kv_heads;
   a.group = sh.group;
   a.page_size = sh.page_size;
-  a.page_shift = -1;
-  for (int b = 0; b < 31; ++b)
-    if ((1 << b) == sh.page_size) a.page_shift = b;
+  a.by_group = FastDiv::of(sh.group);
+  a.by_page = FastDiv::of(sh.page_size);
   a.window = sh.window;
   a.slot_rows = slot_rows(sh);
   a.part_o = reinterpret_cast<float*>(workspace);

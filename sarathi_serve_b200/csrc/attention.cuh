@@ -50,6 +50,19 @@ struct AttnShape {
   int few_limit;   // -1: every tile is ATTN_SIMT; INT32_MAX: ATTN_FEW
 };
 
+// n / d for 0 <= n < 2^31 as a product: with 2^(s - 1) < d <= 2^s and m = floor(2^(31 + s) / d) + 1, m d exceeds 2^(31 + s) by at
+// most d <= 2^s, so n m / 2^(31 + s) exceeds n / d by less than 1 / d.  A division takes some 40 instructions instead, and the
+// kernels make one for every row and every page they address.
+struct FastDiv {
+  uint32_t mul, shift, d;
+  __host__ static FastDiv of(int d) {
+    uint32_t s = 0;
+    while ((1ll << s) < d) ++s;
+    return FastDiv{(uint32_t)((1ull << (31 + s)) / (uint32_t)d + 1), 31 + s, (uint32_t)d};
+  }
+  __device__ __forceinline__ int div(int n) const { return (int)(((uint64_t)(uint32_t)n * mul) >> shift); }
+};
+
 struct AttnArgs {
   AttnPlanView plan;
   const void* q; int64_t ldq;
@@ -63,7 +76,7 @@ struct AttnArgs {
   int64_t num_kv_indices;
   int num_pages, num_tokens;
   int kv_heads, group, page_size, window, slot_rows;
-  int page_shift;      // log2(page_size), or -1
+  FastDiv by_group, by_page;
   float scale_log2;    // scale * log2(e): scores in powers of two
   int zero_behind;
 };
@@ -97,8 +110,9 @@ struct AttnWalk {
     const bool head_cut = p->b0 > 0, tail_cut = p->b1 < p->t.nblk;
     p->slot = head_cut ? 2 * worker : tail_cut ? 2 * worker + 1 : -1;
     // q may have fewer rows than the plan was made for
-    p->t.nrows = min((long long)p->t.nrows, max(0ll, ((long long)a.num_tokens - p->t.q_row) * a.group - p->t.row0));
-    const int first = p->t.row0 / a.group, last = (p->t.row0 + max(p->t.nrows, 1) - 1) / a.group;
+    // (tokens x group stays below 2^30)
+    p->t.nrows = min(p->t.nrows, max(0, (a.num_tokens - p->t.q_row) * a.group - p->t.row0));
+    const int first = a.by_group.div(p->t.row0), last = a.by_group.div(p->t.row0 + max(p->t.nrows, 1) - 1);
     p->hi = max(0, p->t.pos0 + last + 1);
     p->lo = a.window > 0 ? max(0, p->t.pos0 + first + 1 - a.window) : 0;
     if (cur.y + 1 < a.kv_heads) cur = make_int4(cur.x, cur.y + 1, 0, 0);
@@ -110,7 +124,7 @@ struct AttnWalk {
 // Cache row (of kv_heads * head_dim elements) of a key, or -1 where its page is not one of the cache's: such a page reads
 // as zeros, so that a bad table cannot reach outside.  The value is page_size rows further.
 __device__ __forceinline__ int attn_key_row(const AttnArgs& a, int page_at, int key) {
-  const int p = a.page_shift >= 0 ? key >> a.page_shift : key / a.page_size;
+  const int p = a.by_page.div(key);
   const long long at = (long long)page_at + p;
   const int page = at >= 0 && at < a.num_kv_indices ? a.kv_indices[at] : -1;
   return (unsigned)page < (unsigned)a.num_pages ? page * 2 * a.page_size + (key - p * a.page_size) : -1;
@@ -118,7 +132,7 @@ __device__ __forceinline__ int attn_key_row(const AttnArgs& a, int page_at, int 
 
 // Where row r of a piece's tile goes: (token row, q head).
 __device__ __forceinline__ void attn_row(const AttnArgs& a, const AttnPiece& p, int r, int* token, int* head, int* pos) {
-  const int row = p.t.row0 + r, tok = row / a.group;
+  const int row = p.t.row0 + r, tok = a.by_group.div(row);
   *token = p.t.q_row + tok;
   *head = p.head * a.group + (row - tok * a.group);
   *pos = p.t.pos0 + tok;

@@ -41,6 +41,49 @@ __device__ __forceinline__ float pow2(float x) {
   return y;
 }
 
+// Two fp32 numbers that one instruction works on.
+using f32x2 = uint64_t;
+__device__ __forceinline__ f32x2 pair(uint32_t lo, uint32_t hi) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
+  return r;
+}
+__device__ __forceinline__ f32x2 pair(float lo, float hi) { return pair(__float_as_uint(lo), __float_as_uint(hi)); }
+__device__ __forceinline__ float low(f32x2 x) { return __uint_as_float((uint32_t)x); }
+__device__ __forceinline__ float high(f32x2 x) { return __uint_as_float((uint32_t)(x >> 32)); }
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+// 2^x for x <= 2^8 on the FMA pipes: x = n + f with n the nearest integer (adding 1.5 * 2^23 leaves it in the low bits), 2^f by a
+// polynomial, n added to the exponent.  The coefficients are fitted to 2^f on [-1/2, 1/2] for the least largest relative error:
+// degree 3, 7.5e-5, where the result is rounded to bf16 (2^-9), degree 4, 2.6e-6, for fp16 (2^-12).  Below -126 the
+// result stays 2^-126.
+template <typename T> __device__ __forceinline__ f32x2 pow2_pair(f32x2 x) {
+  auto both = [](float c) { return pair(c, c); };
+  x = pair(fmaxf(low(x), -126.f), fmaxf(high(x), -126.f));
+  const f32x2 t = add2(x, both(12582912.f)), n = add2(t, both(-12582912.f)), f = fma2(n, both(-1.f), x);
+  f32x2 y;
+  if constexpr (DT<T>::id == SB200_BF16) {
+    y = fma2(f, both(0.0551716685295105f), both(0.2426111251115799f));
+    y = fma2(y, f, both(0.6932609677314758f));
+    y = fma2(y, f, both(0.9999280571937561f));
+  } else {
+    y = fma2(f, both(0.009570102207362652f), both(0.05591785907745361f));
+    y = fma2(y, f, both(0.240247443318367f));
+    y = fma2(y, f, both(0.6931217908859253f));
+    y = fma2(y, f, both(0.9999992847442627f));
+  }
+  return pair((uint32_t)y + ((uint32_t)t << 23), (uint32_t)(y >> 32) + ((uint32_t)(t >> 32) << 23));
+}
+constexpr int kPoly = 3;
+
 template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   uint32_t r;
   if constexpr (DT<T>::id == SB200_BF16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
@@ -90,6 +133,22 @@ __device__ __forceinline__ void few_barrier(int threads) {
 // A maximum is replaced only when the new one is this much larger (in powers of two): until then probabilities grow to at most
 // 2^8, which 16 bits hold as well as numbers below 1, and the output need not be rescaled.
 constexpr float kLazy = 8.f;
+
+// Lane i of a quad has row i's four pieces; afterwards v[j] is piece i of row j.
+__device__ __forceinline__ void turn_quad(uint4 (&v)[4], int lane4) {
+  auto swap = [&](uint4& x, uint4& y, int mask, bool upper) {  // the upper lane gives x and takes y's place
+    uint4 s = upper ? x : y;
+    s.x = __shfl_xor_sync(0xffffffffu, s.x, mask); s.y = __shfl_xor_sync(0xffffffffu, s.y, mask);
+    s.z = __shfl_xor_sync(0xffffffffu, s.z, mask); s.w = __shfl_xor_sync(0xffffffffu, s.w, mask);
+    if (upper) x = s;
+    else y = s;
+  };
+  const bool up1 = lane4 & 1, up2 = lane4 & 2;
+  swap(v[0], v[1], 1, up1);
+  swap(v[2], v[3], 1, up1);
+  swap(v[0], v[2], 2, up2);
+  swap(v[1], v[3], 2, up2);
+}
 
 // One row's output recomputed key by key: what a product with P = 0 cannot do is to leave out a value that is not finite.
 // Called by a warp for a row whose output came out not finite; m is the maximum that the row's sum l was made with.
@@ -206,7 +265,7 @@ __device__ void few_share(const AttnArgs& a, uint8_t* smem, int worker) {
             qf[k][half + 2 * c] = r < p.t.nrows ? *reinterpret_cast<const uint32_t*>(src + k * 16 + c * 8) : 0u;
       }
     }
-    const int pos_first = p.t.pos0 + p.t.row0 / a.group, pos_last = p.hi - 1;
+    const int pos_first = p.t.pos0 + a.by_group.div(p.t.row0), pos_last = p.hi - 1;
     float o[NT][4];
 #pragma unroll
     for (int i = 0; i < NT; ++i) { o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f; }
@@ -324,7 +383,10 @@ __device__ void few_share(const AttnArgs& a, uint8_t* smem, int worker) {
         bool fine = true;
 #pragma unroll
         for (int j = 0; j < N; ++j) fine = fine && fabsf(acc[j]) < INFINITY;
-        if (!__all_sync(0xffffffffu, fine)) attn_repair_row<T, HD>(a, p, r, base, acc);
+        if (!__all_sync(0xffffffffu, fine)) {
+          const AttnPiece copy = p;  // (p itself stays in registers)
+          attn_repair_row<T, HD>(a, copy, r, base, acc);
+        }
         int token, head, pos;
         attn_row(a, p, r, &token, &head, &pos);
         if (p.slot < 0) {
@@ -349,74 +411,93 @@ __device__ void few_share(const AttnArgs& a, uint8_t* smem, int worker) {
 }
 
 // ------------------------------------------------------------------ many rows
-// A tile of 256 query rows in two halves A and B of 128, keys in blocks of 128, both products on tcgen05:
+// A tile of 256 query rows in two halves A and B of 128, keys in steps of 64, both products on tcgen05:
 //   S = Q K^T     both operands in shared memory, K-major
 //   O += P V      P (16 bits) in TMEM where S was, V in shared memory as it lies in the cache (its rows are the K side)
-// TMEM holds S / P of both halves (2 x 128 columns) and O of both (2 x HD).  Warps 0-3 make the probabilities of half A,
-// warps 4-7 those of B, a row per thread; warp 8 issues the products, warp 9 the loads.  While the tensor pipe works for one
-// half, the other half's warps turn S into P; products of one half are issued back to back (P V of a block, then S of the
-// next), so that S needs no second buffer.  The maximum moves only when it has grown by 2^8 (kLazy), so O is hardly ever rescaled,
-// and then by the warps that found out: S of a block is complete after O of the one before it.
-// Bound: 4 HD FLOP and one exponential a (row, key): 1024 + 1024 clocks of the tensor pipe a block of both halves with
-// HD = 128, and 2048 of the exponential unit (16 a clock and SM), side by side.
+// TMEM holds two S / P buffers of 64 columns per half and O of both halves (2 x HD columns): with HD = 128 all of it.  Warps
+// 0-3 make the probabilities of half A, warps 4-7 those of B, a row per thread; warp 8 issues the products, warp 9 loads keys
+// and values, warps 10 and 11 the query rows of the next piece.  The scores of step j + 2 are issued behind P V of step j, so
+// those of j + 1 are there when a warp comes back from step j: it waits for the tensor pipe only when that is the bound.  (With
+// one buffer of 128 columns per half, scores of the next block behind P V of this one, each half waited 1300 of 4000 clocks a
+// block.)  The maximum moves only when it has grown by 2^8 (kLazy), so O is hardly ever rescaled, and then by the warps that found out.
 // Keys and values come a page per box (128-byte swizzle), whatever the page: 8 rows and up.  Pages outside the cache
 // are fetched from behind its end, which fills zeros.  Values of keys that no row of the tile sees (behind the last, before the
 // window) are cleared in shared memory, as 0 x NaN is not 0; rows that meet one all the same are recomputed (attn_repair_row).
+constexpr int kManyKeys = 64;
+
 template <int HD> struct Many {
   static constexpr int HALVES = HD / 64;
-  static constexpr int BOX = 128 * 128;             // bytes of 128 rows x 64 columns
-  static constexpr int TILE = HALVES * BOX;         // 128 rows
-  static constexpr int STAGES = HD == 128 ? 5 : 8;  // blocks of keys or values
-  static constexpr int SMEM = (2 + STAGES) * TILE;
+  static constexpr int QBOX = 128 * 128;                // bytes of 128 rows x 64 columns
+  static constexpr int QTILE = HALVES * QBOX;
+  static constexpr int BOX = kManyKeys * 128;           // bytes of a step's rows x 64 columns
+  static constexpr int TILE = HALVES * BOX;             // a step's keys, or its values
+  static constexpr int STAGES = HD == 128 ? 10 : 16;
+  static constexpr int SMEM = 2 * QTILE + STAGES * TILE;
 };
 
 struct ManySync {
-  uint64_t full[8], empty[8], q_full[2], s_full[2], p_full[2], o_full[2], drain;
+  uint64_t full[16], empty[16], q_full[2], q_empty[2], s_full[2][2], p_full[2], o_full[2], drain;
   uint32_t tmem;
   int abort_word;
 };
+
+// First key and number of steps of a piece.
+__device__ __forceinline__ int many_steps(const AttnPiece& p, int* key) {
+  *key = max(p.lo & ~(kManyKeys - 1), (p.t.blk_lo + p.b0) * kAttnBlock);
+  return max(0, (min(p.hi, (p.t.blk_lo + p.b1) * kAttnBlock) - *key + kManyKeys - 1) / kManyKeys);
+}
 
 template <int HD>
 __device__ __forceinline__ void many_load(const AttnArgs& a, const CUtensorMap* map, uint8_t* smem, ManySync& sy, AttnWalk walk) {
   using M = Many<HD>;
   const int lane = threadIdx.x & 31;
   volatile int* abort_flag = &sy.abort_word;
-  const int box = min(a.page_size, kAttnBlock), boxes = kAttnBlock / box;
+  const int box = min(a.page_size, kManyKeys), boxes = kManyKeys / box;
   const int none = a.num_pages * 2 * a.page_size;  // the first row behind the cache
   int stage = 0, filled = 0;
   uint32_t phase = 0;
   bool ok = true;
   AttnPiece p;
   while (ok && walk.next(a, &p)) {
-    for (int b = p.b0; ok && b < p.b1; ++b) {
-      const int key0 = (p.t.blk_lo + b) * kAttnBlock;
-      const int key = key0 + lane * box;   // lane i: box i of the block
-      const bool want = lane < boxes && key < p.hi && key + box > p.lo;
-      int row = -1;
-      if (want) row = attn_key_row(a, p.t.page_at, key);
-      const uint32_t mask = __ballot_sync(0xffffffffu, want);
-#pragma unroll 1
-      for (int v = 0; ok && v < 2; ++v) {
-        ok = ptx::mbar_wait_warp(&sy.empty[stage], phase ^ 1u, abort_flag);
-        if (!ok) break;
-        uint8_t* dst = smem + (2 + stage) * M::TILE;
-        const int at = row < 0 ? none : row + v * a.page_size;
-        if (ptx::elect_one()) ptx::mbar_expect_tx(&sy.full[stage], (uint32_t)(__popc(mask) * box * HD * 2));
-        __syncwarp();
-        for (int i = 0; i < boxes; ++i) {
-          const int r = __shfl_sync(0xffffffffu, at, i);
-          if ((mask >> i) & 1u) {
-            if (ptx::elect_one()) {
+    int key0;
+    const int n = many_steps(p, &key0);
+    // lane i holds the row of box i: of the step whose keys are fetched now, and of the two before, whose values follow them
+    auto look_up = [&](int j) {
+      const int key = key0 + j * kManyKeys + lane * box;
+      const bool want = j < n && lane < boxes && key < p.hi && key + box > p.lo;
+      return !want ? -2 : attn_key_row(a, p.t.page_at, key);  // -2: not fetched, -1: zeros
+    };
+    auto fetch = [&](int rows, int to_value) {
+      ok = ok && ptx::mbar_wait_warp(&sy.empty[stage], phase ^ 1u, abort_flag);
+      if (!ok) return;
+      uint8_t* dst = smem + 2 * M::QTILE + stage * M::TILE;
+      const uint32_t mask = __ballot_sync(0xffffffffu, rows != -2);
+      const int at = rows < 0 ? none : rows + to_value;
+      if (ptx::elect_one()) ptx::mbar_expect_tx(&sy.full[stage], (uint32_t)(__popc(mask) * box * HD * 2));
+      __syncwarp();
+      for (int i = 0; i < boxes; ++i) {
+        const int r = __shfl_sync(0xffffffffu, at, i);
+        if ((mask >> i) & 1u) {
+          if (ptx::elect_one()) {
 #pragma unroll
-              for (int h = 0; h < M::HALVES; ++h)
-                ptx::tma_load_2d(dst + h * M::BOX + i * box * 128, map, &sy.full[stage], p.head * HD + h * 64, r);
-            }
-            __syncwarp();
+            for (int h = 0; h < M::HALVES; ++h)
+              ptx::tma_load_2d(dst + h * M::BOX + i * box * 128, map, &sy.full[stage], p.head * HD + h * 64, r);
           }
+          __syncwarp();
         }
-        ++filled;
-        if (++stage == M::STAGES) { stage = 0; phase ^= 1u; }
       }
+      ++filled;
+      if (++stage == M::STAGES) { stage = 0; phase ^= 1u; }
+    };
+    if (n == 0) continue;
+    int r0 = look_up(0), r1 = look_up(1), r2 = look_up(2);
+    fetch(r0, 0);
+    if (n > 1) fetch(r1, 0);
+    for (int j = 0; ok && j < n; ++j) {
+      const int r3 = look_up(j + 3);
+      fetch(r0, a.page_size);
+      if (j + 2 < n) fetch(r2, 0);
+      r0 = r1; r1 = r2; r2 = r3;
     }
   }
   if (!ok) {
@@ -428,32 +509,65 @@ __device__ __forceinline__ void many_load(const AttnArgs& a, const CUtensorMap* 
   }
 }
 
+// The query rows of one half, a piece ahead of the warps that will use them.
+template <typename T, int HD>
+__device__ __forceinline__ void many_queries(const AttnArgs& a, uint8_t* smem, ManySync& sy, AttnWalk walk, int sub) {
+  using M = Many<HD>;
+  constexpr int CPR = HD / 8, RPI = 32 / CPR;  // 16-byte pieces of a row, rows per copy instruction of the warp
+  const int lane = threadIdx.x & 31, chunk = lane % CPR, c = chunk & 7, first = lane / CPR;
+  volatile int* abort_flag = &sy.abort_word;
+  const uint32_t dst = ptx::smem_u32(smem) + sub * M::QTILE + (chunk >> 3) * M::QBOX;
+  const T* q = reinterpret_cast<const T*>(a.q) + chunk * 8;
+  uint32_t pieces = 0;
+  AttnPiece p;
+  while (walk.next(a, &p)) {
+    int key0;
+    if (many_steps(p, &key0) == 0 || (sub == 1 && p.t.nrows <= 128)) continue;
+    if (!ptx::mbar_wait_warp(&sy.q_empty[sub], (pieces++ & 1u) ^ 1u, abort_flag)) break;
+#pragma unroll 8
+    for (int i = 0; i < 128; i += RPI) {
+      const int rr = i + first, row = sub * 128 + rr;
+      int token, head, pos;
+      attn_row(a, p, row, &token, &head, &pos);
+      const bool real = row < p.t.nrows;
+      cp_async16(dst + rr * 128 + ((c ^ (rr & 7)) << 4), real ? q + token * a.ldq + head * HD : q, real);
+    }
+    cp_async_commit();
+    cp_async_wait<0>();
+    ptx::fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) ptx::mbar_arrive(&sy.q_full[sub]);
+  }
+}
+
 template <typename T, int HD>
 __device__ __forceinline__ void many_multiply(const AttnArgs& a, uint8_t* smem, ManySync& sy, AttnWalk walk) {
   using M = Many<HD>;
   const int lane = threadIdx.x & 31;
   volatile int* abort_flag = &sy.abort_word;
   constexpr int fmt = DT<T>::id == SB200_BF16 ? 1 : 0;
-  const uint32_t id_s = ptx::make_idesc(fmt, 128), id_o = ptx::make_idesc(fmt, HD) | ptx::kIdescBRows;
-  const uint32_t tmem = sy.tmem, sq = ptx::smem_u32(smem), kv = sq + 2 * M::TILE;
-  auto scores = [&](int sub, int stage) {  // S of half `sub` with the keys in `stage`
+  const uint32_t id_s = ptx::make_idesc(fmt, kManyKeys), id_o = ptx::make_idesc(fmt, HD) | ptx::kIdescBRows;
+  const uint32_t tmem = sy.tmem, sq = ptx::smem_u32(smem), kv = sq + 2 * M::QTILE;
+  auto scores = [&](int sub, int buf, int stage, bool last) {  // S of half `sub` with the keys in `stage`; the piece's last: q is free
     if (ptx::elect_one()) {
-      const uint64_t dq = ptx::make_smem_desc_sw128(sq + sub * M::TILE), dk = ptx::make_smem_desc_sw128(kv + stage * M::TILE);
+      const uint64_t dq = ptx::make_smem_desc_sw128(sq + sub * M::QTILE), dk = ptx::make_smem_desc_sw128(kv + stage * M::TILE);
 #pragma unroll
-      for (int k = 0; k < HD / 16; ++k) {
-        const uint64_t off = (uint64_t)((k >> 2) * (M::BOX >> 4) + (k & 3) * 2);
-        ptx::umma_f16(tmem + sub * 128, dq + off, dk + off, id_s, k > 0 ? 1u : 0u);
-      }
-      ptx::umma_commit(&sy.s_full[sub]);
+      for (int k = 0; k < HD / 16; ++k)
+        ptx::umma_f16(tmem + sub * 128 + buf * 64, dq + (uint64_t)((k >> 2) * (M::QBOX >> 4) + (k & 3) * 2),
+                      dk + (uint64_t)((k >> 2) * (M::BOX >> 4) + (k & 3) * 2), id_s, k > 0 ? 1u : 0u);
+      ptx::umma_commit(&sy.s_full[sub][buf]);
+      if (last) ptx::umma_commit(&sy.q_empty[sub]);
     }
     __syncwarp();
   };
-  auto output = [&](int sub, int stage, bool first) {
+  auto output = [&](int sub, int buf, int stage, bool first) {
     if (ptx::elect_one()) {
       const uint64_t dv = ptx::make_smem_desc_rows_sw128(kv + stage * M::TILE, M::BOX);
 #pragma unroll
-      for (int k = 0; k < kAttnBlock / 16; ++k)
-        ptx::umma_f16_ts(tmem + 256 + sub * HD, tmem + sub * 128 + k * 8, dv + (uint64_t)(k * (16 * 128 >> 4)), id_o, !first || k > 0 ? 1u : 0u);
+      for (int k = 0; k < kManyKeys / 16; ++k)
+        ptx::umma_f16_ts(tmem + 256 + sub * HD, tmem + sub * 128 + buf * 64 + k * 8, dv + (uint64_t)(k * (16 * 128 >> 4)), id_o,
+                         !first || k > 0 ? 1u : 0u);
+      ptx::umma_commit(&sy.o_full[sub]);
     }
     __syncwarp();
   };
@@ -462,69 +576,63 @@ __device__ __forceinline__ void many_multiply(const AttnArgs& a, uint8_t* smem, 
     __syncwarp();
   };
   int stage = 0;
-  uint32_t phase = 0, pieces[2] = {0, 0}, blocks[2] = {0, 0};
-  auto wait_full = [&]() {
-    const bool ok = ptx::mbar_wait_warp(&sy.full[stage], phase, abort_flag);
-    ptx::tc_fence_after();
-    return ok;
-  };
-  auto advance = [&]() { if (++stage == M::STAGES) { stage = 0; phase ^= 1u; } };
+  uint32_t phase = 0, pieces[2] = {0, 0}, steps[2] = {0, 0};
   bool ok = true;
+  auto next_full = [&]() {  // the next stage, once it has been filled
+    const int s = stage;
+    ok = ok && ptx::mbar_wait_warp(&sy.full[s], phase, abort_flag);
+    ptx::tc_fence_after();
+    if (++stage == M::STAGES) { stage = 0; phase ^= 1u; }
+    return s;
+  };
   AttnPiece p;
   while (ok && walk.next(a, &p)) {
-    if (p.b0 >= p.b1) continue;
+    int key0;
+    const int n = many_steps(p, &key0);
+    if (n == 0) continue;
     const int subs = p.t.nrows > 128 ? 2 : 1;
-    ok = wait_full();
-    for (int s = 0; ok && s < subs; ++s) {
-      ok = ptx::mbar_wait_warp(&sy.q_full[s], pieces[s]++ & 1u, abort_flag);
-      ptx::tc_fence_after();
-      if (ok) scores(s, stage);
-    }
-    if (!ok) break;
-    release(stage);
-    advance();
-    for (int b = p.b0; ok && b < p.b1; ++b) {
-      const int vs = stage;
-      int ks = vs;
+    for (int j = 0; j < 2 && j < n; ++j) {
+      const int ks = next_full();
       for (int s = 0; ok && s < subs; ++s) {
-        if (s == 0) {
-          ok = wait_full();
-          if (!ok) break;
-          // values that no row sees
-          const int key0 = (p.t.blk_lo + b) * kAttnBlock, lo = max(0, min(128, p.lo - key0)), hi = max(0, min(128, p.hi - key0));
-          if (lo > 0 || hi < 128) {
-            uint8_t* v = smem + (2 + vs) * M::TILE;
-            for (int i = lane; i < 128 * 8; i += 32) {
-              const int r = i >> 3;
-              if (r < lo || r >= hi)
-#pragma unroll
-                for (int h = 0; h < M::HALVES; ++h) *reinterpret_cast<uint4*>(v + h * M::BOX + i * 16) = make_uint4(0, 0, 0, 0);
-            }
-            ptx::fence_proxy_async_smem();
-            __syncwarp();
-          }
-          advance();
+        if (j == 0) {
+          ok = ptx::mbar_wait_warp(&sy.q_full[s], pieces[s]++ & 1u, abort_flag);
+          ptx::tc_fence_after();
         }
-        ok = ptx::mbar_wait_warp(&sy.p_full[s], blocks[s]++ & 1u, abort_flag);
+        if (ok) scores(s, j, ks, j + 1 == n);
+      }
+      if (!ok) break;
+      release(ks);
+    }
+    for (int j = 0; ok && j < n; ++j) {
+      const int vs = next_full();
+      if (!ok) break;
+      // values that no row sees
+      const int at = key0 + j * kManyKeys, lo = max(0, min(kManyKeys, p.lo - at)), hi = max(0, min(kManyKeys, p.hi - at));
+      if (lo > 0 || hi < kManyKeys) {
+        uint8_t* v = smem + 2 * M::QTILE + vs * M::TILE;
+        for (int i = lane; i < kManyKeys * 8; i += 32) {
+          const int r = i >> 3;
+          if (r < lo || r >= hi)
+#pragma unroll
+            for (int h = 0; h < M::HALVES; ++h) *reinterpret_cast<uint4*>(v + h * M::BOX + i * 16) = make_uint4(0, 0, 0, 0);
+        }
+        ptx::fence_proxy_async_smem();
+        __syncwarp();
+      }
+      int ks = 0;
+      for (int s = 0; ok && s < subs; ++s) {
+        ok = ptx::mbar_wait_warp(&sy.p_full[s], steps[s]++ & 1u, abort_flag);
         if (!ok) break;
         ptx::tc_fence_after();
-        output(s, vs, b == p.b0);
-        if (b + 1 < p.b1) {
-          if (s == 0) {
-            ok = wait_full();
-            if (!ok) break;
-            ks = stage;
-            advance();
-          }
-          scores(s, ks);
-        } else {
-          if (ptx::elect_one()) ptx::umma_commit(&sy.o_full[s]);
-          __syncwarp();
+        output(s, j & 1, vs, j == 0);
+        if (j + 2 < n) {
+          if (s == 0) ks = next_full();
+          if (ok) scores(s, j & 1, ks, j + 3 == n);
         }
       }
       if (!ok) break;
       release(vs);
-      if (b + 1 < p.b1) release(ks);
+      if (j + 2 < n) release(ks);
     }
   }
   if (!ok) {  // given up: what has been issued may still read shared memory and write TMEM
@@ -544,100 +652,108 @@ __device__ __forceinline__ void many_softmax(const AttnArgs& a, uint8_t* smem, M
   volatile int* abort_flag = &sy.abort_word;
   const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
   const uint32_t t_s = sy.tmem + sub * 128 + lanes, t_o = sy.tmem + 256 + sub * HD + lanes;
-  // the maximum is taken before the scaling and masked scores are -inf, so the sign of the scale (or its being 0) goes into q
+  // the maximum is taken before the scaling and masked scores are -inf, so the sign of the scale (or its being 0) goes first
   const float scale = a.scale_log2 == 0.f ? 1.f : fabsf(a.scale_log2);
-  const uint32_t flip = a.scale_log2 < 0.f ? 0x80008000u : 0u, keep = a.scale_log2 == 0.f ? 0u : ~0u;
-  uint32_t pieces = 0, blocks = 0;
+  uint32_t steps = 0, uses[2] = {0, 0};
   AttnPiece p;
   while (walk.next(a, &p)) {
     if (sub == 1 && p.t.nrows <= 128) continue;
-    int token, head, pos;
+    int token, head, pos, key0;
     attn_row(a, p, min(r, max(p.t.nrows - 1, 0)), &token, &head, &pos);
+    const int n = many_steps(p, &key0);
     float m = -INFINITY, l = 0.f;
-    const bool any = p.b0 < p.b1;
-    if (any) {
-      // ---- the warp's 32 query rows to shared memory
-      constexpr int CPR = HD / 8, RPI = 32 / CPR;
-      const int chunk = lane % CPR, c = chunk & 7;
-      uint8_t* dst = smem + sub * M::TILE + (chunk >> 3) * M::BOX;
-#pragma unroll
-      for (int i0 = 0; i0 < 32 / RPI; i0 += 8) {
-        uint4 x[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int rr = quarter * 32 + (i0 + i) * RPI + lane / CPR, row = sub * 128 + rr;
-          x[i] = make_uint4(0, 0, 0, 0);
-          if (row < p.t.nrows) {
-            int tk, hd, ps;
-            attn_row(a, p, row, &tk, &hd, &ps);
-            x[i] = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.q) + tk * a.ldq + hd * HD + chunk * 8);
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int rr = quarter * 32 + (i0 + i) * RPI + lane / CPR;
-          x[i] = make_uint4((x[i].x ^ flip) & keep, (x[i].y ^ flip) & keep, (x[i].z ^ flip) & keep, (x[i].w ^ flip) & keep);
-          *reinterpret_cast<uint4*>(dst + rr * 128 + ((c ^ (rr & 7)) << 4)) = x[i];
-        }
-      }
-      ptx::fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) ptx::mbar_arrive(&sy.q_full[sub]);
-    }
     // keys that all rows of this half see need no mask
-    const int pos_first = p.t.pos0 + (p.t.row0 + sub * 128) / a.group, pos_last = p.hi - 1;
-    for (int b = p.b0; b < p.b1; ++b) {
-      if (!ptx::mbar_wait_warp(&sy.s_full[sub], blocks++ & 1u, abort_flag)) return;
+    const int pos_first = p.t.pos0 + a.by_group.div(p.t.row0 + sub * 128), pos_last = p.hi - 1;
+    auto one_step = [&](int j, int buf) {
+      if (!ptx::mbar_wait_warp(&sy.s_full[sub][buf], uses[buf]++ & 1u, abort_flag)) return false;
       ptx::tc_fence_after();
-      uint32_t raw[128];
-      ptx::tmem_ld_32x64(t_s, raw);
-      ptx::tmem_ld_32x64(t_s + 64, raw + 64);
-      const int key0 = (p.t.blk_lo + b) * kAttnBlock;
-      if (!(key0 + kAttnBlock - 1 <= pos_first && (a.window == 0 || key0 > pos_last - a.window))) {
-        const int hi = pos - key0, lo = a.window > 0 ? hi - a.window : -1;
+      uint32_t raw[64];
+      ptx::tmem_ld_32x64(t_s + buf * 64, raw);
+      if (a.scale_log2 <= 0.f) {
 #pragma unroll
-        for (int i = 0; i < 128; ++i)
-          if (i > hi || (a.window > 0 && i <= lo)) raw[i] = 0xff800000u;
+        for (int i = 0; i < 64; ++i) raw[i] = __float_as_uint(__uint_as_float(raw[i]) * (a.scale_log2 < 0.f ? -1.f : 0.f));
       }
-      float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+      const int key = key0 + j * kManyKeys;
+      const bool masked = !(key + kManyKeys - 1 <= pos_first && (a.window == 0 || key > pos_last - a.window));
+      if (masked) {  // of the step's keys the row sees [lo, hi]
+        const int hi = pos - key, lo = a.window > 0 ? max(0, hi - a.window + 1) : 0;
+        const uint32_t count = (uint32_t)max(0, hi - lo + 1);
 #pragma unroll
-      for (int i = 0; i < 128; ++i) top[i & 3] = fmaxf(top[i & 3], __uint_as_float(raw[i]));
-      const float now = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+        for (int i = 0; i < 64; ++i)
+          if ((uint32_t)(i - lo) >= count) raw[i] = 0xff800000u;
+      }
+      float top0 = -INFINITY, top1 = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < 32; i += 2) {
+        top0 = fmaxf(fmaxf(top0, __uint_as_float(raw[2 * i])), __uint_as_float(raw[2 * i + 1]));
+        top1 = fmaxf(fmaxf(top1, __uint_as_float(raw[2 * i + 2])), __uint_as_float(raw[2 * i + 3]));
+      }
+      const float now = fmaxf(top0, top1);
       const bool grow = (now - m) * scale > kLazy || (m == -INFINITY && now > m);
-      if (__any_sync(0xffffffffu, grow)) {
-        const float next = fmaxf(m, now), f = m == -INFINITY ? 0.f : pow2((m - next) * scale);
+      const bool rescale = __any_sync(0xffffffffu, grow);
+      float f = 1.f;
+      if (rescale) {
+        const float next = fmaxf(m, now);
+        f = m == -INFINITY ? 0.f : pow2((m - next) * scale);
         m = next;
         l *= f;
-        if (b > p.b0) {
+      }
+      const float base = m == -INFINITY ? 0.f : -m * scale;
+      // kPoly of every eight pairs go to the FMA pipes (pow2_pair), the others to the exponential unit.  Where something is
+      // masked, or a row has seen nothing but -inf, all go to the unit, which makes exact zeros.
+      const bool exact = __any_sync(0xffffffffu, m == -INFINITY) || masked;
+      const f32x2 sc = pair(scale, scale), bs = pair(base, base);
+      f32x2 sum0 = pair(0.f, 0.f), sum1 = pair(0.f, 0.f);
+      if (exact) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          const f32x2 x = fma2(pair(raw[2 * i], raw[2 * i + 1]), sc, bs);
+          const float u = pow2(low(x)), v = pow2(high(x));
+          if (i & 1) sum1 = add2(sum1, pair(u, v));
+          else sum0 = add2(sum0, pair(u, v));
+          raw[i] = pack2<T>(u, v);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          const f32x2 x = fma2(pair(raw[2 * i], raw[2 * i + 1]), sc, bs);
+          const f32x2 y = i % 8 < kPoly ? pow2_pair<T>(x) : pair(pow2(low(x)), pow2(high(x)));
+          if (i & 1) sum1 = add2(sum1, y);
+          else sum0 = add2(sum0, y);
+          raw[i] = pack2<T>(low(y), high(y));
+        }
+      }
+      sum0 = add2(sum0, sum1);
+      l += low(sum0) + high(sum0);
+      ptx::tmem_st_32x32(t_s + buf * 64, raw);
+      // P V of the step before is complete (every one of these is waited for, so that the phases stay in step)
+      if (j > 0) {
+        if (!ptx::mbar_wait_warp(&sy.o_full[sub], steps++ & 1u, abort_flag)) return false;
+        if (rescale) {
+          ptx::tc_fence_after();
 #pragma unroll
           for (int i = 0; i < HD / 32; ++i) {
             uint32_t o[32];
             ptx::tmem_ld_32x32(t_o + i * 32, o);
 #pragma unroll
-            for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
             ptx::tmem_st_32x32(t_o + i * 32, o);
           }
         }
       }
-      const float base = m == -INFINITY ? 0.f : -m * scale;
-      float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int i = 0; i < 64; ++i) {
-        const float x = pow2(fmaf(__uint_as_float(raw[2 * i]), scale, base)), y = pow2(fmaf(__uint_as_float(raw[2 * i + 1]), scale, base));
-        sum[i & 1] += x;
-        sum[2 + (i & 1)] += y;
-        raw[i] = pack2<T>(x, y);
-      }
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-      ptx::tmem_st_32x32(t_s, raw);
-      ptx::tmem_st_32x32(t_s + 32, raw + 32);
       ptx::tmem_wait_st();
       ptx::tc_fence_before();
       __syncwarp();
       if (lane == 0) ptx::mbar_arrive(&sy.p_full[sub]);
+      return true;
+    };
+    for (int j = 0; j < n; j += 2) {
+      if (!one_step(j, 0)) return;
+      if (j + 1 < n && !one_step(j + 1, 1)) return;
     }
+    const bool any = n > 0;
     if (any) {
-      if (!ptx::mbar_wait_warp(&sy.o_full[sub], pieces++ & 1u, abort_flag)) return;
+      if (!ptx::mbar_wait_warp(&sy.o_full[sub], steps++ & 1u, abort_flag)) return;
       ptx::tc_fence_after();
     }
     // ---- a row per thread
@@ -647,6 +763,10 @@ __device__ __forceinline__ void many_softmax(const AttnArgs& a, uint8_t* smem, M
     const int64_t at = (int64_t)p.slot * a.slot_rows + r;
     const float base2 = m == -INFINITY ? 0.f : m * scale;
     bool fine = true;
+    const long long mine = !real ? -1 : p.slot < 0 ? token * a.ldo + head * HD : at * HD;  // where this thread's row goes
+    long long quad_off[4];                                                                  // and those of its four lanes
+#pragma unroll
+    for (int j = 0; j < 4; ++j) quad_off[j] = __shfl_sync(0xffffffffu, mine, (lane & ~3) + j);
 #pragma unroll
     for (int i = 0; i < HD / 32; ++i) {
       uint32_t o[32];
@@ -654,31 +774,37 @@ __device__ __forceinline__ void many_softmax(const AttnArgs& a, uint8_t* smem, M
       else
 #pragma unroll
         for (int j = 0; j < 32; ++j) o[j] = 0u;
-      float big = 0.f;
+      float none = 0.f;  // 0 x v is 0 unless v is not finite
 #pragma unroll
       for (int j = 0; j < 32; ++j) {
-        const float v = __uint_as_float(o[j]);
-        big = fmaxf(big, fabsf(v));
-        fine = fine && v == v;
-        o[j] = __float_as_uint(v * inv);
+        none = fmaf(__uint_as_float(o[j]), 0.f, none);
+        o[j] = __float_as_uint(__uint_as_float(o[j]) * inv);
       }
-      fine = fine && big < INFINITY;
-      if (real) {
-        if (p.slot < 0) {
-          T* dst = reinterpret_cast<T*>(a.out) + token * a.ldo + head * HD + i * 32;
+      fine = fine && none == 0.f;
+      // four lanes turn their rows' 4 x 16 bytes around, so that a store has 64 bytes of a row side by side
+      const int lane4 = lane & 3;
+      if (p.slot < 0) {
+        uint4 v[4];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            uint4 v;
-            v.x = pack2<T>(__uint_as_float(o[8 * j]), __uint_as_float(o[8 * j + 1]));
-            v.y = pack2<T>(__uint_as_float(o[8 * j + 2]), __uint_as_float(o[8 * j + 3]));
-            v.z = pack2<T>(__uint_as_float(o[8 * j + 4]), __uint_as_float(o[8 * j + 5]));
-            v.w = pack2<T>(__uint_as_float(o[8 * j + 6]), __uint_as_float(o[8 * j + 7]));
-            reinterpret_cast<uint4*>(dst)[j] = v;
-          }
-        } else {
-          uint4* dst = reinterpret_cast<uint4*>(a.part_o + at * HD + i * 32);
+        for (int j = 0; j < 4; ++j)
+          v[j] = make_uint4(pack2<T>(__uint_as_float(o[8 * j]), __uint_as_float(o[8 * j + 1])),
+                            pack2<T>(__uint_as_float(o[8 * j + 2]), __uint_as_float(o[8 * j + 3])),
+                            pack2<T>(__uint_as_float(o[8 * j + 4]), __uint_as_float(o[8 * j + 5])),
+                            pack2<T>(__uint_as_float(o[8 * j + 6]), __uint_as_float(o[8 * j + 7])));
+        turn_quad(v, lane4);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) dst[j] = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+        for (int j = 0; j < 4; ++j)
+          if (quad_off[j] >= 0) *reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.out) + quad_off[j] + i * 32 + lane4 * 8) = v[j];
+      } else {
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+          uint4 v[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) v[j] = make_uint4(o[16 * hf + 4 * j], o[16 * hf + 4 * j + 1], o[16 * hf + 4 * j + 2], o[16 * hf + 4 * j + 3]);
+          turn_quad(v, lane4);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (quad_off[j] >= 0) *reinterpret_cast<uint4*>(a.part_o + quad_off[j] + i * 32 + hf * 16 + lane4 * 4) = v[j];
         }
       }
     }
@@ -691,10 +817,11 @@ __device__ __forceinline__ void many_softmax(const AttnArgs& a, uint8_t* smem, M
       const int who = __ffs(bad) - 1;
       bad &= bad - 1;
       constexpr int N = HD / 32;
+      const AttnPiece copy = p;  // (p itself stays in registers)
       float o[N];
       const int row = sub * 128 + quarter * 32 + who;
       const float f = __shfl_sync(0xffffffffu, inv, who);
-      attn_repair_row<T, HD>(a, p, row, __shfl_sync(0xffffffffu, base2, who), o);
+      attn_repair_row<T, HD>(a, copy, row, __shfl_sync(0xffffffffu, base2, who), o);
       int tk, hd, ps;
       attn_row(a, p, row, &tk, &hd, &ps);
 #pragma unroll
@@ -715,7 +842,7 @@ template <int HD> constexpr int tc_smem() {
 }
 
 // One CTA per SM: its share's tiles of many rows first, then those of few.
-// 384 threads x 168 registers, dealt out again: 8 warps that compute x 216, and 72 for the four of which two issue products
+// 384 threads x 168 registers, dealt out again: 8 warps that compute x 216, and 72 for the four that issue products
 // and loads.  (256 x 216 + 128 x 72 = 384 x 168.)
 template <typename T, int HD>
 __global__ void __launch_bounds__(tc_threads<HD>(), 1)
@@ -737,7 +864,7 @@ attn_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUten
       if (threadIdx.x == 0) {
         for (int i = 0; i < Many<HD>::STAGES; ++i) { ptx::mbar_init(&sy.full[i], 1); ptx::mbar_init(&sy.empty[i], 1); }
         for (int i = 0; i < 2; ++i) {
-          ptx::mbar_init(&sy.q_full[i], 4); ptx::mbar_init(&sy.s_full[i], 1);
+          ptx::mbar_init(&sy.q_full[i], 1); ptx::mbar_init(&sy.q_empty[i], 1); ptx::mbar_init(&sy.s_full[i][0], 1); ptx::mbar_init(&sy.s_full[i][1], 1);
           ptx::mbar_init(&sy.p_full[i], 4); ptx::mbar_init(&sy.o_full[i], 1);
         }
         ptx::mbar_init(&sy.drain, 1);
@@ -756,6 +883,7 @@ attn_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUten
       ptx::registers_shrink<72>();
       if (!many) return;
       if (warp == 9) many_load<HD>(a, &map, smem, sy, walk);
+      else if (warp >= 10) many_queries<T, HD>(a, smem, sy, walk, warp - 10);
       else if (warp == 8) many_multiply<T, HD>(a, smem, sy, walk);
       __syncwarp();
       ptx::tc_fence_before();
@@ -784,7 +912,7 @@ static int launch_tc(const AttnArgs& a, bool many, int workers, cudaStream_t s) 
   CUtensorMap map = {};
   if (many) {
     const int rc = make_tmap_2d(&map, DT<T>::id, a.cache, (int64_t)a.num_pages * 2 * a.page_size, (int64_t)a.kv_heads * HD,
-                                (int64_t)a.kv_heads * HD, a.page_size < kAttnBlock ? a.page_size : kAttnBlock, 64);
+                                (int64_t)a.kv_heads * HD, a.page_size < kManyKeys ? a.page_size : kManyKeys, 64);
     if (rc) return rc;
   }
   SB_CUDA(cudaFuncSetAttribute(attn_tc_kernel<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
