@@ -62,27 +62,34 @@ __device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
   return r;
 }
 // 2^x for x <= 2^8 on the FMA pipes: x = n + f with n the nearest integer (adding 1.5 * 2^23 leaves it in the low bits), 2^f by a
-// polynomial, n added to the exponent.  The coefficients are fitted to 2^f on [-1/2, 1/2] for the least largest relative error:
-// degree 3, 7.5e-5, where the result is rounded to bf16 (2^-9), degree 4, 2.6e-6, for fp16 (2^-12).  Below -126 the
-// result stays 2^-126.
+// polynomial, n added to the exponent.  The coefficients are fitted to 2^f on [-1/2, 1/2] for the least largest relative error
+// of a polynomial that is 1 at 0: degree 3, 1.02e-4, where the result is rounded to bf16 (2^-9), degree 4, 2.9e-6, for fp16
+// (2^-12).  From -127 down the result is exactly 0 (there f = 0, and the exponent of 1 less 127 is that of 0), between -126 and -127
+// less than 2^-126.
 template <typename T> __device__ __forceinline__ f32x2 pow2_pair(f32x2 x) {
   auto both = [](float c) { return pair(c, c); };
-  x = pair(fmaxf(low(x), -126.f), fmaxf(high(x), -126.f));
+  x = pair(fmaxf(low(x), -127.f), fmaxf(high(x), -127.f));
   const f32x2 t = add2(x, both(12582912.f)), n = add2(t, both(-12582912.f)), f = fma2(n, both(-1.f), x);
   f32x2 y;
   if constexpr (DT<T>::id == SB200_BF16) {
-    y = fma2(f, both(0.0551716685295105f), both(0.2426111251115799f));
-    y = fma2(y, f, both(0.6932609677314758f));
-    y = fma2(y, f, both(0.9999280571937561f));
+    y = fma2(f, both(0.05500893294811249f), both(0.24221095442771912f));
+    y = fma2(y, f, both(0.6932829022407532f));
   } else {
-    y = fma2(f, both(0.009570102207362652f), both(0.05591785907745361f));
-    y = fma2(y, f, both(0.240247443318367f));
-    y = fma2(y, f, both(0.6931217908859253f));
-    y = fma2(y, f, both(0.9999992847442627f));
+    y = fma2(f, both(0.009582852944731712f), both(0.055906426161527634f));
+    y = fma2(y, f, both(0.24024099111557007f));
+    y = fma2(y, f, both(0.6931241750717163f));
   }
+  y = fma2(y, f, both(1.f));
   return pair((uint32_t)y + ((uint32_t)t << 23), (uint32_t)(y >> 32) + ((uint32_t)(t >> 32) << 23));
 }
 constexpr int kPoly = 3;
+
+// The largest of three, or NaN if one of them is.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
 
 template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   uint32_t r;
@@ -654,7 +661,7 @@ __device__ __forceinline__ void many_softmax(const AttnArgs& a, uint8_t* smem, M
   const uint32_t t_s = sy.tmem + sub * 128 + lanes, t_o = sy.tmem + 256 + sub * HD + lanes;
   // the maximum is taken before the scaling and masked scores are -inf, so the sign of the scale (or its being 0) goes first
   const float scale = a.scale_log2 == 0.f ? 1.f : fabsf(a.scale_log2);
-  uint32_t steps = 0, uses[2] = {0, 0};
+  uint32_t steps = 0, uses = 0;  // (uses: the phase bit of either score buffer)
   AttnPiece p;
   while (walk.next(a, &p)) {
     if (sub == 1 && p.t.nrows <= 128) continue;
@@ -664,8 +671,10 @@ __device__ __forceinline__ void many_softmax(const AttnArgs& a, uint8_t* smem, M
     float m = -INFINITY, l = 0.f;
     // keys that all rows of this half see need no mask
     const int pos_first = p.t.pos0 + a.by_group.div(p.t.row0 + sub * 128), pos_last = p.hi - 1;
-    auto one_step = [&](int j, int buf) {
-      if (!ptx::mbar_wait_warp(&sy.s_full[sub][buf], uses[buf]++ & 1u, abort_flag)) return false;
+    for (int j = 0; j < n; ++j) {
+      const int buf = j & 1;
+      if (!ptx::mbar_wait_warp(&sy.s_full[sub][buf], (uses >> buf) & 1u, abort_flag)) return;
+      uses ^= 1u << buf;
       ptx::tc_fence_after();
       uint32_t raw[64];
       ptx::tmem_ld_32x64(t_s + buf * 64, raw);
@@ -674,61 +683,52 @@ __device__ __forceinline__ void many_softmax(const AttnArgs& a, uint8_t* smem, M
         for (int i = 0; i < 64; ++i) raw[i] = __float_as_uint(__uint_as_float(raw[i]) * (a.scale_log2 < 0.f ? -1.f : 0.f));
       }
       const int key = key0 + j * kManyKeys;
-      const bool masked = !(key + kManyKeys - 1 <= pos_first && (a.window == 0 || key > pos_last - a.window));
-      if (masked) {  // of the step's keys the row sees [lo, hi]
-        const int hi = pos - key, lo = a.window > 0 ? max(0, hi - a.window + 1) : 0;
-        const uint32_t count = (uint32_t)max(0, hi - lo + 1);
+      if (!(key + kManyKeys - 1 <= pos_first && (a.window == 0 || key > pos_last - a.window))) {
+        const int hi = pos - key;
 #pragma unroll
         for (int i = 0; i < 64; ++i)
-          if ((uint32_t)(i - lo) >= count) raw[i] = 0xff800000u;
+          if (i > hi) raw[i] = 0xff800000u;
+        if (a.window > 0) {
+          const int lo = hi - a.window;
+#pragma unroll
+          for (int i = 0; i < 64; ++i)
+            if (i <= lo) raw[i] = 0xff800000u;
+        }
       }
       float top0 = -INFINITY, top1 = -INFINITY;
 #pragma unroll
       for (int i = 0; i < 32; i += 2) {
-        top0 = fmaxf(fmaxf(top0, __uint_as_float(raw[2 * i])), __uint_as_float(raw[2 * i + 1]));
-        top1 = fmaxf(fmaxf(top1, __uint_as_float(raw[2 * i + 2])), __uint_as_float(raw[2 * i + 3]));
+        top0 = max3(top0, __uint_as_float(raw[2 * i]), __uint_as_float(raw[2 * i + 1]));
+        top1 = max3(top1, __uint_as_float(raw[2 * i + 2]), __uint_as_float(raw[2 * i + 3]));
       }
-      const float now = fmaxf(top0, top1);
-      const bool grow = (now - m) * scale > kLazy || (m == -INFINITY && now > m);
+      const float now = max3(top0, top1, -INFINITY);
+      const bool grow = now != -INFINITY && !((now - m) * scale <= kLazy);  // (also the first score, and one that is no number)
       const bool rescale = __any_sync(0xffffffffu, grow);
       float f = 1.f;
       if (rescale) {
-        const float next = fmaxf(m, now);
+        const float next = max3(m, now, -INFINITY);
         f = m == -INFINITY ? 0.f : pow2((m - next) * scale);
         m = next;
         l *= f;
       }
       const float base = m == -INFINITY ? 0.f : -m * scale;
-      // kPoly of every eight pairs go to the FMA pipes (pow2_pair), the others to the exponential unit.  Where something is
-      // masked, or a row has seen nothing but -inf, all go to the unit, which makes exact zeros.
-      const bool exact = __any_sync(0xffffffffu, m == -INFINITY) || masked;
+      // kPoly of every eight pairs go to the FMA pipes (pow2_pair), the others to the exponential unit; both make a masked score 0
       const f32x2 sc = pair(scale, scale), bs = pair(base, base);
       f32x2 sum0 = pair(0.f, 0.f), sum1 = pair(0.f, 0.f);
-      if (exact) {
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          const f32x2 x = fma2(pair(raw[2 * i], raw[2 * i + 1]), sc, bs);
-          const float u = pow2(low(x)), v = pow2(high(x));
-          if (i & 1) sum1 = add2(sum1, pair(u, v));
-          else sum0 = add2(sum0, pair(u, v));
-          raw[i] = pack2<T>(u, v);
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          const f32x2 x = fma2(pair(raw[2 * i], raw[2 * i + 1]), sc, bs);
-          const f32x2 y = i % 8 < kPoly ? pow2_pair<T>(x) : pair(pow2(low(x)), pow2(high(x)));
-          if (i & 1) sum1 = add2(sum1, y);
-          else sum0 = add2(sum0, y);
-          raw[i] = pack2<T>(low(y), high(y));
-        }
+      for (int i = 0; i < 32; ++i) {
+        const f32x2 x = fma2(pair(raw[2 * i], raw[2 * i + 1]), sc, bs);
+        const f32x2 y = i % 8 < kPoly ? pow2_pair<T>(x) : pair(pow2(low(x)), pow2(high(x)));
+        if (i & 1) sum1 = add2(sum1, y);
+        else sum0 = add2(sum0, y);
+        raw[i] = pack2<T>(low(y), high(y));
       }
       sum0 = add2(sum0, sum1);
       l += low(sum0) + high(sum0);
       ptx::tmem_st_32x32(t_s + buf * 64, raw);
       // P V of the step before is complete (every one of these is waited for, so that the phases stay in step)
       if (j > 0) {
-        if (!ptx::mbar_wait_warp(&sy.o_full[sub], steps++ & 1u, abort_flag)) return false;
+        if (!ptx::mbar_wait_warp(&sy.o_full[sub], steps++ & 1u, abort_flag)) return;
         if (rescale) {
           ptx::tc_fence_after();
 #pragma unroll
@@ -745,11 +745,6 @@ __device__ __forceinline__ void many_softmax(const AttnArgs& a, uint8_t* smem, M
       ptx::tc_fence_before();
       __syncwarp();
       if (lane == 0) ptx::mbar_arrive(&sy.p_full[sub]);
-      return true;
-    };
-    for (int j = 0; j < n; j += 2) {
-      if (!one_step(j, 0)) return;
-      if (j + 1 < n && !one_step(j + 1, 1)) return;
     }
     const bool any = n > 0;
     if (any) {

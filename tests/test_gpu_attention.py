@@ -5,7 +5,7 @@ Tolerances (u(t) = eps(t) / 2, the most that one rounding is off, relative to th
   * fp16 / bf16 round the probabilities once:          u(dtype) W,  W = sum_j p_j |v_j|
   * a score is off by at most (hd + 16) 2^-24 A, A = scale max_j sum_i |q_i k_ji| (fp32 products summed in any order, scaling,
     the subtraction of the maximum), the power of two by E relative: fp32 2^-21 (two units of exp2f), fp16 2^-18 (a polynomial
-    that is off by 2.6e-6 at most, and its rounding), bf16 2^-13.5 (one that is off by 7.5e-5); that moves numerator and
+    that is off by 2.9e-6 at most, and its rounding), bf16 2^-13 (one that is off by 1.02e-4); that moves numerator and
     denominator alike:                                 2 ((hd + 16) 2^-24 A + E) W
   * fp32 sums over n keys, twice (numerator, denominator), and a join:  2 (n + 16) 2^-24 W
   * fp16 probabilities below its smallest step:        n 2^-25 max|v|   (the sum they are divided by is at least 1)
@@ -95,7 +95,7 @@ def reference(c, scale, window=0):
                     va = torch.where(bad, 0, vz).abs()
                     W = p @ va
                     A = (q[:, h].abs() @ torch.where(torch.isfinite(kh), kh, 0).abs().T * abs(scale)).amax(1)
-                    delta = (hd + 16) * 2.0 ** -24 * A + 2.0 ** {torch.float32: -21, torch.float16: -18, torch.bfloat16: -13.5}[c["dtype"]]
+                    delta = (hd + 16) * 2.0 ** -24 * A + 2.0 ** {torch.float32: -21, torch.float16: -18, torch.bfloat16: -13}[c["dtype"]]
                     t = u * res.abs() + (2 * delta[:, None] + 2 * (n + 16) * 2.0 ** -24) * W
                     if c["dtype"] != torch.float32:
                         t = t + u * W
@@ -187,6 +187,26 @@ def test_values_that_a_row_does_not_see(dtype, hd, bad):
             clean, _, tol = reference(c2, hd ** -0.5, window)
             d = (got.view(c["total"], -1) - clean).abs() - tol
             assert d[fine.view(c["total"], -1)].max() <= 0, (window, new, before, at)
+
+
+@pytest.mark.parametrize("dtype,hd", [(torch.bfloat16, 128), (torch.float16, 64), (torch.float32, 128)])
+def test_keys_that_are_not_numbers(dtype, hd):
+    """A NaN in a key makes the rows that see it NaN, wherever it lies in a block, and leaves the others alone."""
+    from sarathi_serve_b200 import attention_ops
+    for window in (0, 40):
+        for new, before, at in [(200, 100, 131 + 7 * i) for i in range(9)] + [(3, 200, 201), (1, 60, 59), (260, 20, 100)]:
+            c = make(11, dtype, 4, 2, hd, 16, [(new, before), (1, 77)], cache_fill=0.0)
+            clean, _, tol = reference(c, hd ** -0.5, window)
+            c["cache"][c["table"][0, at // 16], 0, at % 16, 1, 3] = float("nan")
+            plan, _ = plan_of(c, window)
+            lse = torch.zeros(c["T"], 4, device="cuda")
+            out = attention_ops.paged_attention(c["q"], c["cache"], plan, hd ** -0.5, lse=lse)
+            pos = before + torch.arange(new, device="cuda")
+            sees = (pos >= at) & ((pos < at + window) if window else (pos >= 0))
+            got = out[:c["total"]].double().view(-1, 4, hd)
+            assert torch.isnan(got[:new][sees][:, 2:]).all() and torch.isnan(lse[:new][sees][:, 2:]).all()
+            got[:new, 2:][sees] = clean.view(-1, 4, hd)[:new, 2:][sees]
+            assert ((got.view(c["total"], -1) - clean).abs() <= tol).all(), (window, new, before, at)
 
 
 @pytest.mark.parametrize("dtype,hd", [(torch.bfloat16, 128), (torch.float16, 64), (torch.float32, 64)])
