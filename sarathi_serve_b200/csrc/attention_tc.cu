@@ -82,7 +82,7 @@ template <typename T> __device__ __forceinline__ f32x2 pow2_pair(f32x2 x) {
   y = fma2(y, f, both(1.f));
   return pair((uint32_t)y + ((uint32_t)t << 23), (uint32_t)(y >> 32) + ((uint32_t)(t >> 32) << 23));
 }
-constexpr int kPoly = 3;
+constexpr int kPoly = 2;
 
 // The largest of three, or NaN if one of them is.
 __device__ __forceinline__ float max3(float a, float b, float c) {
@@ -443,7 +443,7 @@ template <int HD> struct Many {
 };
 
 struct ManySync {
-  uint64_t full[16], empty[16], q_full[2], q_empty[2], s_full[2][2], p_full[2], o_full[2], drain;
+  uint64_t full[16], empty[16], q_full[2], q_empty[2], turn[2][2], p_full[2][2], drain;
   uint32_t tmem;
   int abort_word;
 };
@@ -562,7 +562,6 @@ __device__ __forceinline__ void many_multiply(const AttnArgs& a, uint8_t* smem, 
       for (int k = 0; k < HD / 16; ++k)
         ptx::umma_f16(tmem + sub * 128 + buf * 64, dq + (uint64_t)((k >> 2) * (M::QBOX >> 4) + (k & 3) * 2),
                       dk + (uint64_t)((k >> 2) * (M::BOX >> 4) + (k & 3) * 2), id_s, k > 0 ? 1u : 0u);
-      ptx::umma_commit(&sy.s_full[sub][buf]);
       if (last) ptx::umma_commit(&sy.q_empty[sub]);
     }
     __syncwarp();
@@ -574,8 +573,11 @@ __device__ __forceinline__ void many_multiply(const AttnArgs& a, uint8_t* smem, 
       for (int k = 0; k < kManyKeys / 16; ++k)
         ptx::umma_f16_ts(tmem + 256 + sub * HD, tmem + sub * 128 + buf * 64 + k * 8, dv + (uint64_t)(k * (16 * 128 >> 4)), id_o,
                          !first || k > 0 ? 1u : 0u);
-      ptx::umma_commit(&sy.o_full[sub]);
     }
+    __syncwarp();
+  };
+  auto turn = [&](int sub, int buf) {  // all that has been issued for this buffer's turn
+    if (ptx::elect_one()) ptx::umma_commit(&sy.turn[sub][buf]);
     __syncwarp();
   };
   auto release = [&](int stage) {
@@ -583,7 +585,7 @@ __device__ __forceinline__ void many_multiply(const AttnArgs& a, uint8_t* smem, 
     __syncwarp();
   };
   int stage = 0;
-  uint32_t phase = 0, pieces[2] = {0, 0}, steps[2] = {0, 0};
+  uint32_t phase = 0, pieces[2] = {0, 0}, given[2] = {0, 0};  // given: phase bits of a half's p_full, one per buffer
   bool ok = true;
   auto next_full = [&]() {  // the next stage, once it has been filled
     const int s = stage;
@@ -591,6 +593,11 @@ __device__ __forceinline__ void many_multiply(const AttnArgs& a, uint8_t* smem, 
     ptx::tc_fence_after();
     if (++stage == M::STAGES) { stage = 0; phase ^= 1u; }
     return s;
+  };
+  auto wait_p = [&](int sub, int buf) {
+    const uint32_t bit = (given[sub] >> buf) & 1u;
+    given[sub] ^= 1u << buf;
+    return ptx::mbar_wait_warp(&sy.p_full[sub][buf], bit, abort_flag);
   };
   AttnPiece p;
   while (ok && walk.next(a, &p)) {
@@ -605,11 +612,16 @@ __device__ __forceinline__ void many_multiply(const AttnArgs& a, uint8_t* smem, 
           ok = ptx::mbar_wait_warp(&sy.q_full[s], pieces[s]++ & 1u, abort_flag);
           ptx::tc_fence_after();
         }
-        if (ok) scores(s, j, ks, j + 1 == n);
+        if (ok) {
+          scores(s, j, ks, j + 1 == n);
+          turn(s, j);
+        }
       }
       if (!ok) break;
       release(ks);
     }
+    if (n == 1)  // (every buffer has the same number of turns, whatever the number of steps: see many_softmax)
+      for (int s = 0; ok && s < subs; ++s) turn(s, 1);
     for (int j = 0; ok && j < n; ++j) {
       const int vs = next_full();
       if (!ok) break;
@@ -628,7 +640,7 @@ __device__ __forceinline__ void many_multiply(const AttnArgs& a, uint8_t* smem, 
       }
       int ks = 0;
       for (int s = 0; ok && s < subs; ++s) {
-        ok = ptx::mbar_wait_warp(&sy.p_full[s], steps[s]++ & 1u, abort_flag);
+        ok = wait_p(s, j & 1);
         if (!ok) break;
         ptx::tc_fence_after();
         output(s, j & 1, vs, j == 0);
@@ -636,11 +648,14 @@ __device__ __forceinline__ void many_multiply(const AttnArgs& a, uint8_t* smem, 
           if (s == 0) ks = next_full();
           if (ok) scores(s, j & 1, ks, j + 3 == n);
         }
+        if (ok) turn(s, j & 1);
       }
       if (!ok) break;
       release(vs);
       if (j + 2 < n) release(ks);
     }
+    // the next piece's first turns come only after this one's last have been seen: a barrier is never two turns ahead of its reader
+    for (int s = 0; ok && s < subs; ++s) ok = wait_p(s, n & 1);
   }
   if (!ok) {  // given up: what has been issued may still read shared memory and write TMEM
     __shared__ int never;
@@ -661,7 +676,9 @@ __device__ __forceinline__ void many_softmax(const AttnArgs& a, uint8_t* smem, M
   const uint32_t t_s = sy.tmem + sub * 128 + lanes, t_o = sy.tmem + 256 + sub * HD + lanes;
   // the maximum is taken before the scaling and masked scores are -inf, so the sign of the scale (or its being 0) goes first
   const float scale = a.scale_log2 == 0.f ? 1.f : fabsf(a.scale_log2);
-  uint32_t steps = 0, uses = 0;  // (uses: the phase bit of either score buffer)
+  // Turn j of a piece (buffer j & 1) is complete when the scores of step j are there and P V of step j - 2 is done; with n steps
+  // there are n + 2 turns, so that the last two stand for the end of O.
+  uint32_t phases = 0;  // phase bit of either buffer
   AttnPiece p;
   while (walk.next(a, &p)) {
     if (sub == 1 && p.t.nrows <= 128) continue;
@@ -673,8 +690,8 @@ __device__ __forceinline__ void many_softmax(const AttnArgs& a, uint8_t* smem, M
     const int pos_first = p.t.pos0 + a.by_group.div(p.t.row0 + sub * 128), pos_last = p.hi - 1;
     for (int j = 0; j < n; ++j) {
       const int buf = j & 1;
-      if (!ptx::mbar_wait_warp(&sy.s_full[sub][buf], (uses >> buf) & 1u, abort_flag)) return;
-      uses ^= 1u << buf;
+      ptx::mbar_wait_converged(&sy.turn[sub][buf], (phases >> buf) & 1u, abort_flag);
+      phases ^= 1u << buf;
       ptx::tc_fence_after();
       uint32_t raw[64];
       ptx::tmem_ld_32x64(t_s + buf * 64, raw);
@@ -726,30 +743,32 @@ __device__ __forceinline__ void many_softmax(const AttnArgs& a, uint8_t* smem, M
       sum0 = add2(sum0, sum1);
       l += low(sum0) + high(sum0);
       ptx::tmem_st_32x32(t_s + buf * 64, raw);
-      // P V of the step before is complete (every one of these is waited for, so that the phases stay in step)
-      if (j > 0) {
-        if (!ptx::mbar_wait_warp(&sy.o_full[sub], steps++ & 1u, abort_flag)) return;
-        if (rescale) {
-          ptx::tc_fence_after();
+      if (rescale && j > 0) {  // P V of the step before has to be done: turn j + 1
+        ptx::mbar_wait_converged(&sy.turn[sub][buf ^ 1], (phases >> (buf ^ 1)) & 1u, abort_flag);
+        ptx::tc_fence_after();
 #pragma unroll
-          for (int i = 0; i < HD / 32; ++i) {
-            uint32_t o[32];
-            ptx::tmem_ld_32x32(t_o + i * 32, o);
+        for (int i = 0; i < HD / 32; ++i) {
+          uint32_t o[32];
+          ptx::tmem_ld_32x32(t_o + i * 32, o);
 #pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-            ptx::tmem_st_32x32(t_o + i * 32, o);
-          }
+          for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+          ptx::tmem_st_32x32(t_o + i * 32, o);
         }
       }
       ptx::tmem_wait_st();
       ptx::tc_fence_before();
       __syncwarp();
-      if (lane == 0) ptx::mbar_arrive(&sy.p_full[sub]);
+      if (lane == 0) ptx::mbar_arrive(&sy.p_full[sub][buf]);
     }
     const bool any = n > 0;
     if (any) {
-      if (!ptx::mbar_wait_warp(&sy.o_full[sub], steps++ & 1u, abort_flag)) return;
+      for (int j = n; j < n + 2; ++j) {
+        ptx::mbar_wait_converged(&sy.turn[sub][j & 1], (phases >> (j & 1)) & 1u, abort_flag);
+        phases ^= 1u << (j & 1);
+      }
       ptx::tc_fence_after();
+      if (__any_sync(0xffffffffu, *abort_flag != 0)) return;
+      if (lane == 0) ptx::mbar_arrive(&sy.p_full[sub][n & 1]);  // the next piece's scores may begin
     }
     // ---- a row per thread
     const bool real = r < p.t.nrows;
@@ -762,13 +781,16 @@ __device__ __forceinline__ void many_softmax(const AttnArgs& a, uint8_t* smem, M
     long long quad_off[4];                                                                  // and those of its four lanes
 #pragma unroll
     for (int j = 0; j < 4; ++j) quad_off[j] = __shfl_sync(0xffffffffu, mine, (lane & ~3) + j);
+    uint32_t both[64];
 #pragma unroll
     for (int i = 0; i < HD / 32; ++i) {
-      uint32_t o[32];
-      if (any) ptx::tmem_ld_32x32(t_o + i * 32, o);
-      else
+      uint32_t* o = both + (i & 1) * 32;
+      if (i % 2 == 0) {
+        if (any) ptx::tmem_ld_32x64(t_o + i * 32, both);
+        else
 #pragma unroll
-        for (int j = 0; j < 32; ++j) o[j] = 0u;
+          for (int j = 0; j < 64; ++j) both[j] = 0u;
+      }
       float none = 0.f;  // 0 x v is 0 unless v is not finite
 #pragma unroll
       for (int j = 0; j < 32; ++j) {
@@ -859,8 +881,8 @@ attn_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUten
       if (threadIdx.x == 0) {
         for (int i = 0; i < Many<HD>::STAGES; ++i) { ptx::mbar_init(&sy.full[i], 1); ptx::mbar_init(&sy.empty[i], 1); }
         for (int i = 0; i < 2; ++i) {
-          ptx::mbar_init(&sy.q_full[i], 1); ptx::mbar_init(&sy.q_empty[i], 1); ptx::mbar_init(&sy.s_full[i][0], 1); ptx::mbar_init(&sy.s_full[i][1], 1);
-          ptx::mbar_init(&sy.p_full[i], 4); ptx::mbar_init(&sy.o_full[i], 1);
+          ptx::mbar_init(&sy.q_full[i], 1); ptx::mbar_init(&sy.q_empty[i], 1); ptx::mbar_init(&sy.turn[i][0], 1); ptx::mbar_init(&sy.turn[i][1], 1);
+          ptx::mbar_init(&sy.p_full[i][0], 4); ptx::mbar_init(&sy.p_full[i][1], 4);
         }
         ptx::mbar_init(&sy.drain, 1);
         sy.abort_word = 0;

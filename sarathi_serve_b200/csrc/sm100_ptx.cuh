@@ -84,6 +84,13 @@ __device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, v
   return ok;
 }
 
+// The wait of a loop that cannot afford a vote in every turn: all lanes of a warp come out together, with nothing said about
+// whether the wait ran out.  The caller looks at the abort flag every so often (after it is set, a wait takes 256 looks at most).
+__device__ __forceinline__ void mbar_wait_converged(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  if (!mbar_try_wait(bar, parity)) mbar_wait(bar, parity, abort_flag);
+  __syncwarp();
+}
+
 // ----------------------------------------------------------------------- TMA
 __device__ __forceinline__ void prefetch_tensormap(const CUtensorMap* m) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(m)) : "memory");
