@@ -275,10 +275,9 @@ static int attn_shape(const sb200_attention_shape* s, AttnShape* sh, const char*
   sh->page_size = s->page_size;
   sh->dtype = s->dtype;
   sh->window = s->window;
-  // Tiles of 256 rows on tcgen05 want a step of 64 keys to be whole boxes of whole swizzle atoms (8 rows); other pages, and
+  // Tiles of 256 rows on tcgen05 fetch keys in boxes of whole swizzle atoms (8 rows); pages that are no multiple of 8, and
   // heads of 256, whose two outputs and scores do not fit TMEM together, stay with tiles of 16 rows.
-  const bool boxes = (s->page_size % 8 == 0 && 64 % s->page_size == 0) || s->page_size % 64 == 0;
-  const bool many = s->dtype != SB200_F32 && s->head_dim <= 128 && boxes;
+  const bool many = s->dtype != SB200_F32 && s->head_dim <= 128 && s->page_size % 8 == 0;
   sh->rows_many = s->dtype == SB200_F32 ? 32 : many ? 256 : 16;
   sh->rows_few = 16;
   sh->few_limit = s->dtype == SB200_F32 ? -1 : many ? 16 : INT32_MAX;

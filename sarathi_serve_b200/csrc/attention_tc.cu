@@ -418,93 +418,78 @@ __device__ void few_share(const AttnArgs& a, uint8_t* smem, int worker) {
 }
 
 // ------------------------------------------------------------------ many rows
-// A tile of 256 query rows in two halves A and B of 128, keys in steps of 64, both products on tcgen05:
+// A tile of 256 query rows in two halves A and B of 128, keys in blocks of 128, both products on tcgen05:
 //   S = Q K^T     both operands in shared memory, K-major
 //   O += P V      P (16 bits) in TMEM where S was, V in shared memory as it lies in the cache (its rows are the K side)
-// TMEM holds two S / P buffers of 64 columns per half and O of both halves (2 x HD columns): with HD = 128 all of it.  Warps
-// 0-3 make the probabilities of half A, warps 4-7 those of B, a row per thread; warp 8 issues the products, warp 9 loads keys
-// and values, warps 10 and 11 the query rows of the next piece.  The scores of step j + 2 are issued behind P V of step j, so
-// those of j + 1 are there when a warp comes back from step j: it waits for the tensor pipe only when that is the bound.  (With
-// one buffer of 128 columns per half, scores of the next block behind P V of this one, each half waited 1300 of 4000 clocks a
-// block.)  The maximum moves only when it has grown by 2^8 (kLazy), so O is hardly ever rescaled, and then by the warps that found out.
-// Keys and values come a page per box (128-byte swizzle), whatever the page: 8 rows and up.  Pages outside the cache
-// are fetched from behind its end, which fills zeros.  Values of keys that no row of the tile sees (behind the last, before the
-// window) are cleared in shared memory, as 0 x NaN is not 0; rows that meet one all the same are recomputed (attn_repair_row).
-constexpr int kManyKeys = 64;
-
+// TMEM holds S / P of both halves (2 x 128 columns) and O of both (2 x HD): with HD = 128 all of it.  Warps 0-3 make the
+// probabilities of half A, warps 4-7 those of B, a row per thread; warp 8 issues the products, warp 9 loads keys and values,
+// warps 10 and 11 the query rows of the next piece.  While the tensor pipe works for one half, the other half's warps turn S into P.
+// P is handed over in two parts of 64 keys, so that P V of the first runs under the exponentials of the second; the next
+// block's S follows P V at once.  (Steps of 64 keys with two score buffers per half take the tensor pipe 56 clocks per
+// instruction of 64 columns, as long as one of 128: 4300 clocks a block.)  The maximum moves only when it has grown by 2^8 (kLazy), so
+// O is hardly ever rescaled, and then by the warps that found out: S of a block is complete after O of the one before it.
+// Keys and values come in boxes (128-byte swizzle) of as many rows, up to 128, as the page size has powers of two.  Pages
+// outside the cache are fetched from behind its end, which fills zeros.  Values of keys that no row of the tile sees (behind
+// the last, before the window) are cleared in shared memory, as 0 x NaN is not 0; rows that meet one all the same are recomputed
+// (attn_repair_row).
 template <int HD> struct Many {
   static constexpr int HALVES = HD / 64;
-  static constexpr int QBOX = 128 * 128;                // bytes of 128 rows x 64 columns
-  static constexpr int QTILE = HALVES * QBOX;
-  static constexpr int BOX = kManyKeys * 128;           // bytes of a step's rows x 64 columns
-  static constexpr int TILE = HALVES * BOX;             // a step's keys, or its values
-  static constexpr int STAGES = HD == 128 ? 10 : 16;
-  static constexpr int SMEM = 2 * QTILE + STAGES * TILE;
+  static constexpr int BOX = 128 * 128;             // bytes of 128 rows x 64 columns
+  static constexpr int TILE = HALVES * BOX;         // 128 rows
+  static constexpr int STAGES = HD == 128 ? 5 : 8;  // blocks of keys or values
+  static constexpr int SMEM = (2 + STAGES) * TILE;
 };
 
 struct ManySync {
-  uint64_t full[16], empty[16], q_full[2], q_empty[2], turn[2][2], p_full[2][2], drain;
+  uint64_t full[8], empty[8], q_full[2], q_empty[2], turn[2], p_full[2][2], drain;
   uint32_t tmem;
   int abort_word;
 };
-
-// First key and number of steps of a piece.
-__device__ __forceinline__ int many_steps(const AttnPiece& p, int* key) {
-  *key = max(p.lo & ~(kManyKeys - 1), (p.t.blk_lo + p.b0) * kAttnBlock);
-  return max(0, (min(p.hi, (p.t.blk_lo + p.b1) * kAttnBlock) - *key + kManyKeys - 1) / kManyKeys);
-}
 
 template <int HD>
 __device__ __forceinline__ void many_load(const AttnArgs& a, const CUtensorMap* map, uint8_t* smem, ManySync& sy, AttnWalk walk) {
   using M = Many<HD>;
   const int lane = threadIdx.x & 31;
   volatile int* abort_flag = &sy.abort_word;
-  const int box = min(a.page_size, kManyKeys), boxes = kManyKeys / box;
+  const int box = min(a.page_size & -a.page_size, kAttnBlock), boxes = kAttnBlock / box;
   const int none = a.num_pages * 2 * a.page_size;  // the first row behind the cache
   int stage = 0, filled = 0;
   uint32_t phase = 0;
   bool ok = true;
   AttnPiece p;
   while (ok && walk.next(a, &p)) {
-    int key0;
-    const int n = many_steps(p, &key0);
-    // lane i holds the row of box i: of the step whose keys are fetched now, and of the two before, whose values follow them
-    auto look_up = [&](int j) {
-      const int key = key0 + j * kManyKeys + lane * box;
-      const bool want = j < n && lane < boxes && key < p.hi && key + box > p.lo;
-      return !want ? -2 : attn_key_row(a, p.t.page_at, key);  // -2: not fetched, -1: zeros
+    auto look_up = [&](int b) {  // lane i: the row of box i (-2: not fetched, -1: zeros)
+      const int key = (p.t.blk_lo + b) * kAttnBlock + lane * box;
+      const bool want = b < p.b1 && lane < boxes && key < p.hi && key + box > p.lo;
+      return !want ? -2 : attn_key_row(a, p.t.page_at, key);
     };
-    auto fetch = [&](int rows, int to_value) {
-      ok = ok && ptx::mbar_wait_warp(&sy.empty[stage], phase ^ 1u, abort_flag);
-      if (!ok) return;
-      uint8_t* dst = smem + 2 * M::QTILE + stage * M::TILE;
+    int next = look_up(p.b0);
+    for (int b = p.b0; ok && b < p.b1; ++b) {
+      const int rows = next;
+      next = look_up(b + 1);
       const uint32_t mask = __ballot_sync(0xffffffffu, rows != -2);
-      const int at = rows < 0 ? none : rows + to_value;
-      if (ptx::elect_one()) ptx::mbar_expect_tx(&sy.full[stage], (uint32_t)(__popc(mask) * box * HD * 2));
-      __syncwarp();
-      for (int i = 0; i < boxes; ++i) {
-        const int r = __shfl_sync(0xffffffffu, at, i);
-        if ((mask >> i) & 1u) {
-          if (ptx::elect_one()) {
+#pragma unroll 1
+      for (int v = 0; ok && v < 2; ++v) {
+        ok = ptx::mbar_wait_warp(&sy.empty[stage], phase ^ 1u, abort_flag);
+        if (!ok) break;
+        uint8_t* dst = smem + (2 + stage) * M::TILE;
+        const int at = rows < 0 ? none : rows + v * a.page_size;
+        if (ptx::elect_one()) ptx::mbar_expect_tx(&sy.full[stage], (uint32_t)(__popc(mask) * box * HD * 2));
+        __syncwarp();
+        for (int i = 0; i < boxes; ++i) {
+          const int r = __shfl_sync(0xffffffffu, at, i);
+          if ((mask >> i) & 1u) {
+            if (ptx::elect_one()) {
 #pragma unroll
-            for (int h = 0; h < M::HALVES; ++h)
-              ptx::tma_load_2d(dst + h * M::BOX + i * box * 128, map, &sy.full[stage], p.head * HD + h * 64, r);
+              for (int h = 0; h < M::HALVES; ++h)
+                ptx::tma_load_2d(dst + h * M::BOX + i * box * 128, map, &sy.full[stage], p.head * HD + h * 64, r);
+            }
+            __syncwarp();
           }
-          __syncwarp();
         }
+        ++filled;
+        if (++stage == M::STAGES) { stage = 0; phase ^= 1u; }
       }
-      ++filled;
-      if (++stage == M::STAGES) { stage = 0; phase ^= 1u; }
-    };
-    if (n == 0) continue;
-    int r0 = look_up(0), r1 = look_up(1), r2 = look_up(2);
-    fetch(r0, 0);
-    if (n > 1) fetch(r1, 0);
-    for (int j = 0; ok && j < n; ++j) {
-      const int r3 = look_up(j + 3);
-      fetch(r0, a.page_size);
-      if (j + 2 < n) fetch(r2, 0);
-      r0 = r1; r1 = r2; r2 = r3;
     }
   }
   if (!ok) {
@@ -523,15 +508,14 @@ __device__ __forceinline__ void many_queries(const AttnArgs& a, uint8_t* smem, M
   constexpr int CPR = HD / 8, RPI = 32 / CPR;  // 16-byte pieces of a row, rows per copy instruction of the warp
   const int lane = threadIdx.x & 31, chunk = lane % CPR, c = chunk & 7, first = lane / CPR;
   volatile int* abort_flag = &sy.abort_word;
-  const uint32_t dst = ptx::smem_u32(smem) + sub * M::QTILE + (chunk >> 3) * M::QBOX;
+  const uint32_t dst = ptx::smem_u32(smem) + sub * M::TILE + (chunk >> 3) * M::BOX;
   const T* q = reinterpret_cast<const T*>(a.q) + chunk * 8;
   uint32_t pieces = 0;
   AttnPiece p;
   while (walk.next(a, &p)) {
-    int key0;
-    if (many_steps(p, &key0) == 0 || (sub == 1 && p.t.nrows <= 128)) continue;
+    if (p.b0 >= p.b1 || (sub == 1 && p.t.nrows <= 128)) continue;
     if (!ptx::mbar_wait_warp(&sy.q_empty[sub], (pieces++ & 1u) ^ 1u, abort_flag)) break;
-#pragma unroll 8
+#pragma unroll 4
     for (int i = 0; i < 128; i += RPI) {
       const int rr = i + first, row = sub * 128 + rr;
       int token, head, pos;
@@ -547,89 +531,82 @@ __device__ __forceinline__ void many_queries(const AttnArgs& a, uint8_t* smem, M
   }
 }
 
+// Every half has one barrier for "your turn": turn j of a piece is complete when S of block j is there and P V of block j - 1 is
+// done; turn n, after the last block, stands for the end of O.  p_full[0 | 1]: the first | second part of P.  A barrier is
+// never two phases ahead of its reader: turn j + 1 follows p_full of block j, which follows turn j, and the next piece's turn 0
+// waits for an extra p_full[1], given when turn n has been seen.
 template <typename T, int HD>
 __device__ __forceinline__ void many_multiply(const AttnArgs& a, uint8_t* smem, ManySync& sy, AttnWalk walk) {
   using M = Many<HD>;
   const int lane = threadIdx.x & 31;
   volatile int* abort_flag = &sy.abort_word;
   constexpr int fmt = DT<T>::id == SB200_BF16 ? 1 : 0;
-  const uint32_t id_s = ptx::make_idesc(fmt, kManyKeys), id_o = ptx::make_idesc(fmt, HD) | ptx::kIdescBRows;
-  const uint32_t tmem = sy.tmem, sq = ptx::smem_u32(smem), kv = sq + 2 * M::QTILE;
-  auto scores = [&](int sub, int buf, int stage, bool last) {  // S of half `sub` with the keys in `stage`; the piece's last: q is free
+  const uint32_t id_s = ptx::make_idesc(fmt, 128), id_o = ptx::make_idesc(fmt, HD) | ptx::kIdescBRows;
+  const uint32_t tmem = sy.tmem, sq = ptx::smem_u32(smem);
+  // descriptors differ in the address field only, which counts 16 bytes
+  const uint64_t d_rows = ptx::make_smem_desc_sw128(sq), d_value = ptx::make_smem_desc_rows_sw128(sq, M::BOX);
+  auto scores = [&](int sub, int stage, bool last) {  // S of half `sub` with the keys in `stage`; the piece's last: q is free
     if (ptx::elect_one()) {
-      const uint64_t dq = ptx::make_smem_desc_sw128(sq + sub * M::QTILE), dk = ptx::make_smem_desc_sw128(kv + stage * M::TILE);
+      const uint64_t dq = d_rows + (uint64_t)(sub * (M::TILE >> 4)), dk = d_rows + (uint64_t)((2 + stage) * (M::TILE >> 4));
 #pragma unroll
-      for (int k = 0; k < HD / 16; ++k)
-        ptx::umma_f16(tmem + sub * 128 + buf * 64, dq + (uint64_t)((k >> 2) * (M::QBOX >> 4) + (k & 3) * 2),
-                      dk + (uint64_t)((k >> 2) * (M::BOX >> 4) + (k & 3) * 2), id_s, k > 0 ? 1u : 0u);
+      for (int k = 0; k < HD / 16; ++k) {
+        const uint64_t off = (uint64_t)((k >> 2) * (M::BOX >> 4) + (k & 3) * 2);
+        ptx::umma_f16(tmem + sub * 128, dq + off, dk + off, id_s, k > 0 ? 1u : 0u);
+      }
+      ptx::umma_commit(&sy.turn[sub]);
       if (last) ptx::umma_commit(&sy.q_empty[sub]);
     }
     __syncwarp();
   };
-  auto output = [&](int sub, int buf, int stage, bool first) {
+  auto output = [&](int sub, int part, int stage, bool first) {
     if (ptx::elect_one()) {
-      const uint64_t dv = ptx::make_smem_desc_rows_sw128(kv + stage * M::TILE, M::BOX);
+      const uint64_t dv = d_value + (uint64_t)((2 + stage) * (M::TILE >> 4) + part * (64 * 128 >> 4));
 #pragma unroll
-      for (int k = 0; k < kManyKeys / 16; ++k)
-        ptx::umma_f16_ts(tmem + 256 + sub * HD, tmem + sub * 128 + buf * 64 + k * 8, dv + (uint64_t)(k * (16 * 128 >> 4)), id_o,
-                         !first || k > 0 ? 1u : 0u);
+      for (int k = 0; k < 4; ++k)
+        ptx::umma_f16_ts(tmem + 256 + sub * HD, tmem + sub * 128 + part * 32 + k * 8, dv + (uint64_t)(k * (16 * 128 >> 4)), id_o,
+                         !first || part > 0 || k > 0 ? 1u : 0u);
     }
     __syncwarp();
   };
-  auto turn = [&](int sub, int buf) {  // all that has been issued for this buffer's turn
-    if (ptx::elect_one()) ptx::umma_commit(&sy.turn[sub][buf]);
-    __syncwarp();
-  };
-  auto release = [&](int stage) {
-    if (ptx::elect_one()) ptx::umma_commit(&sy.empty[stage]);
+  auto commit = [&](uint64_t* bar) {
+    if (ptx::elect_one()) ptx::umma_commit(bar);
     __syncwarp();
   };
   int stage = 0;
-  uint32_t phase = 0, pieces[2] = {0, 0}, given[2] = {0, 0};  // given: phase bits of a half's p_full, one per buffer
+  uint32_t phase = 0, p_phase[2][2] = {{0, 0}, {0, 0}}, q_phase[2] = {0, 0};
   bool ok = true;
   auto next_full = [&]() {  // the next stage, once it has been filled
     const int s = stage;
-    ok = ok && ptx::mbar_wait_warp(&sy.full[s], phase, abort_flag);
-    ptx::tc_fence_after();
+    ptx::mbar_wait_converged(&sy.full[s], phase, abort_flag);
     if (++stage == M::STAGES) { stage = 0; phase ^= 1u; }
     return s;
   };
-  auto wait_p = [&](int sub, int buf) {
-    const uint32_t bit = (given[sub] >> buf) & 1u;
-    given[sub] ^= 1u << buf;
-    return ptx::mbar_wait_warp(&sy.p_full[sub][buf], bit, abort_flag);
+  auto wait_p = [&](int sub, int part) {
+    ptx::mbar_wait_converged(&sy.p_full[sub][part], p_phase[sub][part], abort_flag);
+    p_phase[sub][part] ^= 1u;
   };
   AttnPiece p;
   while (ok && walk.next(a, &p)) {
-    int key0;
-    const int n = many_steps(p, &key0);
-    if (n == 0) continue;
-    const int subs = p.t.nrows > 128 ? 2 : 1;
-    for (int j = 0; j < 2 && j < n; ++j) {
-      const int ks = next_full();
-      for (int s = 0; ok && s < subs; ++s) {
-        if (j == 0) {
-          ok = ptx::mbar_wait_warp(&sy.q_full[s], pieces[s]++ & 1u, abort_flag);
-          ptx::tc_fence_after();
-        }
-        if (ok) {
-          scores(s, j, ks, j + 1 == n);
-          turn(s, j);
-        }
+    if (p.b0 >= p.b1) continue;
+    const bool both = p.t.nrows > 128;
+    const int ks0 = next_full();
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+      if (s == 0 || both) {
+        ptx::mbar_wait_converged(&sy.q_full[s], q_phase[s], abort_flag);
+        q_phase[s] ^= 1u;
+        ptx::tc_fence_after();
+        scores(s, ks0, p.b0 + 1 == p.b1);
       }
-      if (!ok) break;
-      release(ks);
-    }
-    if (n == 1)  // (every buffer has the same number of turns, whatever the number of steps: see many_softmax)
-      for (int s = 0; ok && s < subs; ++s) turn(s, 1);
-    for (int j = 0; ok && j < n; ++j) {
-      const int vs = next_full();
-      if (!ok) break;
-      // values that no row sees
-      const int at = key0 + j * kManyKeys, lo = max(0, min(kManyKeys, p.lo - at)), hi = max(0, min(kManyKeys, p.hi - at));
-      if (lo > 0 || hi < kManyKeys) {
-        uint8_t* v = smem + 2 * M::QTILE + vs * M::TILE;
-        for (int i = lane; i < kManyKeys * 8; i += 32) {
+    commit(&sy.empty[ks0]);
+    for (int b = p.b0; ok && b < p.b1; ++b) {
+      const int vs = next_full(), key0 = (p.t.blk_lo + b) * kAttnBlock;
+      const bool more = b + 1 < p.b1;
+      if (key0 < p.lo || key0 + kAttnBlock > p.hi) {  // values that no row sees
+        const int lo = p.lo - key0, hi = p.hi - key0;
+        uint8_t* v = smem + (2 + vs) * M::TILE;
+#pragma unroll 1
+        for (int i = lane; i < 128 * 8; i += 32) {
           const int r = i >> 3;
           if (r < lo || r >= hi)
 #pragma unroll
@@ -639,29 +616,37 @@ __device__ __forceinline__ void many_multiply(const AttnArgs& a, uint8_t* smem, 
         __syncwarp();
       }
       int ks = 0;
-      for (int s = 0; ok && s < subs; ++s) {
-        ok = wait_p(s, j & 1);
-        if (!ok) break;
-        ptx::tc_fence_after();
-        output(s, j & 1, vs, j == 0);
-        if (j + 2 < n) {
-          if (s == 0) ks = next_full();
-          if (ok) scores(s, j & 1, ks, j + 3 == n);
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+        if (s == 0 || both) {
+#pragma unroll
+          for (int part = 0; part < 2; ++part) {
+            wait_p(s, part);
+            ptx::tc_fence_after();
+            output(s, part, vs, b == p.b0);
+          }
+          if (more) {
+            if (s == 0) ks = next_full();
+            scores(s, ks, b + 2 == p.b1);
+          } else {
+            commit(&sy.turn[s]);
+          }
         }
-        if (ok) turn(s, j & 1);
-      }
-      if (!ok) break;
-      release(vs);
-      if (j + 2 < n) release(ks);
+      commit(&sy.empty[vs]);
+      if (more) commit(&sy.empty[ks]);
+      ok = __all_sync(0xffffffffu, *abort_flag == 0);  // a wait may have run out
     }
-    // the next piece's first turns come only after this one's last have been seen: a barrier is never two turns ahead of its reader
-    for (int s = 0; ok && s < subs; ++s) ok = wait_p(s, n & 1);
+    if (ok)
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+        if (s == 0 || both) wait_p(s, 1);
   }
+  ok = __all_sync(0xffffffffu, *abort_flag == 0);
   if (!ok) {  // given up: what has been issued may still read shared memory and write TMEM
     __shared__ int never;
     if (lane == 0) never = 0;
     __syncwarp();
-    if (ptx::elect_one()) ptx::umma_commit(&sy.drain);
+    commit(&sy.drain);
     ptx::mbar_wait_warp(&sy.drain, 0u, &never);
   }
 }
@@ -676,99 +661,90 @@ __device__ __forceinline__ void many_softmax(const AttnArgs& a, uint8_t* smem, M
   const uint32_t t_s = sy.tmem + sub * 128 + lanes, t_o = sy.tmem + 256 + sub * HD + lanes;
   // the maximum is taken before the scaling and masked scores are -inf, so the sign of the scale (or its being 0) goes first
   const float scale = a.scale_log2 == 0.f ? 1.f : fabsf(a.scale_log2);
-  // Turn j of a piece (buffer j & 1) is complete when the scores of step j are there and P V of step j - 2 is done; with n steps
-  // there are n + 2 turns, so that the last two stand for the end of O.
-  uint32_t phases = 0;  // phase bit of either buffer
+  uint32_t phase = 0;  // of this half's turns
   AttnPiece p;
   while (walk.next(a, &p)) {
     if (sub == 1 && p.t.nrows <= 128) continue;
-    int token, head, pos, key0;
+    int token, head, pos;
     attn_row(a, p, min(r, max(p.t.nrows - 1, 0)), &token, &head, &pos);
-    const int n = many_steps(p, &key0);
     float m = -INFINITY, l = 0.f;
     // keys that all rows of this half see need no mask
     const int pos_first = p.t.pos0 + a.by_group.div(p.t.row0 + sub * 128), pos_last = p.hi - 1;
-    for (int j = 0; j < n; ++j) {
-      const int buf = j & 1;
-      ptx::mbar_wait_converged(&sy.turn[sub][buf], (phases >> buf) & 1u, abort_flag);
-      phases ^= 1u << buf;
+    for (int b = p.b0; b < p.b1; ++b) {
+      ptx::mbar_wait_converged(&sy.turn[sub], phase, abort_flag);
+      phase ^= 1u;
       ptx::tc_fence_after();
-      uint32_t raw[64];
-      ptx::tmem_ld_32x64(t_s + buf * 64, raw);
+      uint32_t raw[128];
+      ptx::tmem_ld_32x64(t_s, raw);
+      ptx::tmem_ld_32x64(t_s + 64, raw + 64);
       if (a.scale_log2 <= 0.f) {
 #pragma unroll
-        for (int i = 0; i < 64; ++i) raw[i] = __float_as_uint(__uint_as_float(raw[i]) * (a.scale_log2 < 0.f ? -1.f : 0.f));
+        for (int i = 0; i < 128; ++i) raw[i] = __float_as_uint(__uint_as_float(raw[i]) * (a.scale_log2 < 0.f ? -1.f : 0.f));
       }
-      const int key = key0 + j * kManyKeys;
-      if (!(key + kManyKeys - 1 <= pos_first && (a.window == 0 || key > pos_last - a.window))) {
+      const int key = (p.t.blk_lo + b) * kAttnBlock;
+      if (!(key + kAttnBlock - 1 <= pos_first && (a.window == 0 || key > pos_last - a.window))) {
         const int hi = pos - key;
 #pragma unroll
-        for (int i = 0; i < 64; ++i)
+        for (int i = 0; i < 128; ++i)
           if (i > hi) raw[i] = 0xff800000u;
         if (a.window > 0) {
           const int lo = hi - a.window;
 #pragma unroll
-          for (int i = 0; i < 64; ++i)
+          for (int i = 0; i < 128; ++i)
             if (i <= lo) raw[i] = 0xff800000u;
         }
       }
-      float top0 = -INFINITY, top1 = -INFINITY;
+      float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-      for (int i = 0; i < 32; i += 2) {
-        top0 = max3(top0, __uint_as_float(raw[2 * i]), __uint_as_float(raw[2 * i + 1]));
-        top1 = max3(top1, __uint_as_float(raw[2 * i + 2]), __uint_as_float(raw[2 * i + 3]));
-      }
-      const float now = max3(top0, top1, -INFINITY);
+      for (int i = 0; i < 64; ++i) top[i & 3] = max3(top[i & 3], __uint_as_float(raw[2 * i]), __uint_as_float(raw[2 * i + 1]));
+      const float now = max3(max3(top[0], top[1], top[2]), top[3], -INFINITY);
       const bool grow = now != -INFINITY && !((now - m) * scale <= kLazy);  // (also the first score, and one that is no number)
-      const bool rescale = __any_sync(0xffffffffu, grow);
-      float f = 1.f;
-      if (rescale) {
-        const float next = max3(m, now, -INFINITY);
-        f = m == -INFINITY ? 0.f : pow2((m - next) * scale);
+      if (__any_sync(0xffffffffu, grow)) {
+        const float next = max3(m, now, -INFINITY), f = m == -INFINITY ? 0.f : pow2((m - next) * scale);
         m = next;
         l *= f;
+        if (b > p.b0) {  // P V of the block before is done
+#pragma unroll 1
+          for (int i = 0; i < HD / 32; ++i) {
+            uint32_t o[32];
+            ptx::tmem_ld_32x32(t_o + i * 32, o);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+            ptx::tmem_st_32x32(t_o + i * 32, o);
+          }
+        }
       }
       const float base = m == -INFINITY ? 0.f : -m * scale;
       // kPoly of every eight pairs go to the FMA pipes (pow2_pair), the others to the exponential unit; both make a masked score 0
       const f32x2 sc = pair(scale, scale), bs = pair(base, base);
       f32x2 sum0 = pair(0.f, 0.f), sum1 = pair(0.f, 0.f);
 #pragma unroll
-      for (int i = 0; i < 32; ++i) {
-        const f32x2 x = fma2(pair(raw[2 * i], raw[2 * i + 1]), sc, bs);
-        const f32x2 y = i % 8 < kPoly ? pow2_pair<T>(x) : pair(pow2(low(x)), pow2(high(x)));
-        if (i & 1) sum1 = add2(sum1, y);
-        else sum0 = add2(sum0, y);
-        raw[i] = pack2<T>(low(y), high(y));
+      for (int part = 0; part < 2; ++part) {
+        uint32_t prob[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          const f32x2 x = fma2(pair(raw[part * 64 + 2 * i], raw[part * 64 + 2 * i + 1]), sc, bs);
+          const f32x2 y = i % 8 < kPoly ? pow2_pair<T>(x) : pair(pow2(low(x)), pow2(high(x)));
+          if (i & 1) sum1 = add2(sum1, y);
+          else sum0 = add2(sum0, y);
+          prob[i] = pack2<T>(low(y), high(y));
+        }
+        ptx::tmem_st_32x32(t_s + part * 32, prob);
+        ptx::tmem_wait_st();
+        ptx::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(&sy.p_full[sub][part]);
       }
       sum0 = add2(sum0, sum1);
       l += low(sum0) + high(sum0);
-      ptx::tmem_st_32x32(t_s + buf * 64, raw);
-      if (rescale && j > 0) {  // P V of the step before has to be done: turn j + 1
-        ptx::mbar_wait_converged(&sy.turn[sub][buf ^ 1], (phases >> (buf ^ 1)) & 1u, abort_flag);
-        ptx::tc_fence_after();
-#pragma unroll
-        for (int i = 0; i < HD / 32; ++i) {
-          uint32_t o[32];
-          ptx::tmem_ld_32x32(t_o + i * 32, o);
-#pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-          ptx::tmem_st_32x32(t_o + i * 32, o);
-        }
-      }
-      ptx::tmem_wait_st();
-      ptx::tc_fence_before();
-      __syncwarp();
-      if (lane == 0) ptx::mbar_arrive(&sy.p_full[sub][buf]);
     }
-    const bool any = n > 0;
+    const bool any = p.b0 < p.b1;
     if (any) {
-      for (int j = n; j < n + 2; ++j) {
-        ptx::mbar_wait_converged(&sy.turn[sub][j & 1], (phases >> (j & 1)) & 1u, abort_flag);
-        phases ^= 1u << (j & 1);
-      }
+      ptx::mbar_wait_converged(&sy.turn[sub], phase, abort_flag);
+      phase ^= 1u;
       ptx::tc_fence_after();
       if (__any_sync(0xffffffffu, *abort_flag != 0)) return;
-      if (lane == 0) ptx::mbar_arrive(&sy.p_full[sub][n & 1]);  // the next piece's scores may begin
+      if (lane == 0) ptx::mbar_arrive(&sy.p_full[sub][1]);  // the next piece's scores may begin
     }
     // ---- a row per thread
     const bool real = r < p.t.nrows;
@@ -781,47 +757,47 @@ __device__ __forceinline__ void many_softmax(const AttnArgs& a, uint8_t* smem, M
     long long quad_off[4];                                                                  // and those of its four lanes
 #pragma unroll
     for (int j = 0; j < 4; ++j) quad_off[j] = __shfl_sync(0xffffffffu, mine, (lane & ~3) + j);
-    uint32_t both[64];
+    const int lane4 = lane & 3;
+#pragma unroll 1
+    for (int i0 = 0; i0 < HD; i0 += 64) {  // (rolled: this code runs once a piece, and what it costs is fetching it)
+      uint32_t o[64];
+      if (any) ptx::tmem_ld_32x64(t_o + i0, o);
+      else
 #pragma unroll
-    for (int i = 0; i < HD / 32; ++i) {
-      uint32_t* o = both + (i & 1) * 32;
-      if (i % 2 == 0) {
-        if (any) ptx::tmem_ld_32x64(t_o + i * 32, both);
-        else
-#pragma unroll
-          for (int j = 0; j < 64; ++j) both[j] = 0u;
-      }
+        for (int j = 0; j < 64; ++j) o[j] = 0u;
       float none = 0.f;  // 0 x v is 0 unless v is not finite
 #pragma unroll
-      for (int j = 0; j < 32; ++j) {
+      for (int j = 0; j < 64; ++j) {
         none = fmaf(__uint_as_float(o[j]), 0.f, none);
         o[j] = __float_as_uint(__uint_as_float(o[j]) * inv);
       }
       fine = fine && none == 0.f;
       // four lanes turn their rows' 4 x 16 bytes around, so that a store has 64 bytes of a row side by side
-      const int lane4 = lane & 3;
       if (p.slot < 0) {
-        uint4 v[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          v[j] = make_uint4(pack2<T>(__uint_as_float(o[8 * j]), __uint_as_float(o[8 * j + 1])),
-                            pack2<T>(__uint_as_float(o[8 * j + 2]), __uint_as_float(o[8 * j + 3])),
-                            pack2<T>(__uint_as_float(o[8 * j + 4]), __uint_as_float(o[8 * j + 5])),
-                            pack2<T>(__uint_as_float(o[8 * j + 6]), __uint_as_float(o[8 * j + 7])));
-        turn_quad(v, lane4);
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (quad_off[j] >= 0) *reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.out) + quad_off[j] + i * 32 + lane4 * 8) = v[j];
-      } else {
-#pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
+        for (int h = 0; h < 2; ++h) {
           uint4 v[4];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) v[j] = make_uint4(o[16 * hf + 4 * j], o[16 * hf + 4 * j + 1], o[16 * hf + 4 * j + 2], o[16 * hf + 4 * j + 3]);
+          for (int j = 0; j < 4; ++j) {
+            const uint32_t* x = o + 32 * h + 8 * j;
+            auto two = [&](int e) { return pack2<T>(__uint_as_float(x[e]), __uint_as_float(x[e + 1])); };
+            v[j] = make_uint4(two(0), two(2), two(4), two(6));
+          }
           turn_quad(v, lane4);
 #pragma unroll
           for (int j = 0; j < 4; ++j)
-            if (quad_off[j] >= 0) *reinterpret_cast<uint4*>(a.part_o + quad_off[j] + i * 32 + hf * 16 + lane4 * 4) = v[j];
+            if (quad_off[j] >= 0) *reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.out) + quad_off[j] + i0 + h * 32 + lane4 * 8) = v[j];
+        }
+      } else {
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {
+          uint4 v[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) v[j] = make_uint4(o[16 * h + 4 * j], o[16 * h + 4 * j + 1], o[16 * h + 4 * j + 2], o[16 * h + 4 * j + 3]);
+          turn_quad(v, lane4);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (quad_off[j] >= 0) *reinterpret_cast<uint4*>(a.part_o + quad_off[j] + i0 + h * 16 + lane4 * 4) = v[j];
         }
       }
     }
@@ -881,7 +857,7 @@ attn_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUten
       if (threadIdx.x == 0) {
         for (int i = 0; i < Many<HD>::STAGES; ++i) { ptx::mbar_init(&sy.full[i], 1); ptx::mbar_init(&sy.empty[i], 1); }
         for (int i = 0; i < 2; ++i) {
-          ptx::mbar_init(&sy.q_full[i], 1); ptx::mbar_init(&sy.q_empty[i], 1); ptx::mbar_init(&sy.turn[i][0], 1); ptx::mbar_init(&sy.turn[i][1], 1);
+          ptx::mbar_init(&sy.q_full[i], 1); ptx::mbar_init(&sy.q_empty[i], 1); ptx::mbar_init(&sy.turn[i], 1);
           ptx::mbar_init(&sy.p_full[i][0], 4); ptx::mbar_init(&sy.p_full[i][1], 4);
         }
         ptx::mbar_init(&sy.drain, 1);
@@ -929,7 +905,7 @@ static int launch_tc(const AttnArgs& a, bool many, int workers, cudaStream_t s) 
   CUtensorMap map = {};
   if (many) {
     const int rc = make_tmap_2d(&map, DT<T>::id, a.cache, (int64_t)a.num_pages * 2 * a.page_size, (int64_t)a.kv_heads * HD,
-                                (int64_t)a.kv_heads * HD, a.page_size < kManyKeys ? a.page_size : kManyKeys, 64);
+                                (int64_t)a.kv_heads * HD, min(a.page_size & -a.page_size, kAttnBlock), 64);
     if (rc) return rc;
   }
   SB_CUDA(cudaFuncSetAttribute(attn_tc_kernel<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
