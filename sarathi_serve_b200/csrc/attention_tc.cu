@@ -82,7 +82,7 @@ template <typename T> __device__ __forceinline__ f32x2 pow2_pair(f32x2 x) {
   y = fma2(y, f, both(1.f));
   return pair((uint32_t)y + ((uint32_t)t << 23), (uint32_t)(y >> 32) + ((uint32_t)(t >> 32) << 23));
 }
-constexpr int kPoly = 2;
+constexpr int kPoly = 3;
 
 // The largest of three, or NaN if one of them is.
 __device__ __forceinline__ float max3(float a, float b, float c) {
@@ -434,8 +434,9 @@ __device__ void few_share(const AttnArgs& a, uint8_t* smem, int worker) {
 // (attn_repair_row).
 template <int HD> struct Many {
   static constexpr int HALVES = HD / 64;
-  static constexpr int BOX = 128 * 128;             // bytes of 128 rows x 64 columns
-  static constexpr int TILE = HALVES * BOX;         // 128 rows
+  static constexpr int TILE = HALVES * 128 * 128;   // 128 rows
+  static constexpr int QHALF = 128 * 128;           // query rows: [64 columns][128 rows]
+  static constexpr int GROUP = HALVES * 1024;       // keys, values: [8 rows][64 columns][8 x 128 bytes]
   static constexpr int STAGES = HD == 128 ? 5 : 8;  // blocks of keys or values
   static constexpr int SMEM = (2 + STAGES) * TILE;
 };
@@ -451,41 +452,39 @@ __device__ __forceinline__ void many_load(const AttnArgs& a, const CUtensorMap* 
   using M = Many<HD>;
   const int lane = threadIdx.x & 31;
   volatile int* abort_flag = &sy.abort_word;
-  const int box = min(a.page_size & -a.page_size, kAttnBlock), boxes = kAttnBlock / box;
-  const int none = a.num_pages * 2 * a.page_size;  // the first row behind the cache
+  const int box = min(a.page_size & -a.page_size, kAttnBlock), boxes = kAttnBlock / box, groups = box / 8;
+  const int none = a.num_pages * 2 * (a.page_size / 8);  // the first group of 8 rows behind the cache
   int stage = 0, filled = 0;
   uint32_t phase = 0;
   bool ok = true;
   AttnPiece p;
   while (ok && walk.next(a, &p)) {
-    auto look_up = [&](int b) {  // lane i: the row of box i (-2: not fetched, -1: zeros)
-      const int key = (p.t.blk_lo + b) * kAttnBlock + lane * box;
-      const bool want = b < p.b1 && lane < boxes && key < p.hi && key + box > p.lo;
-      return !want ? -2 : attn_key_row(a, p.t.page_at, key);
+    // lane i: the page of box i, asked for a block ahead and looked at when its turn comes
+    auto key_of = [&](int b) { return (p.t.blk_lo + b) * kAttnBlock + lane * box; };
+    auto page_of = [&](int b) {
+      const int key = key_of(b);
+      const long long at = (long long)p.t.page_at + a.by_page.div(key);
+      return b < p.b1 && lane < boxes && key < p.hi && at < a.num_kv_indices ? a.kv_indices[at] : -1;
     };
-    int next = look_up(p.b0);
+    int next = page_of(p.b0);
     for (int b = p.b0; ok && b < p.b1; ++b) {
-      const int rows = next;
-      next = look_up(b + 1);
-      const uint32_t mask = __ballot_sync(0xffffffffu, rows != -2);
+      const int page = next, key = key_of(b);
+      next = page_of(b + 1);
+      const bool want = lane < boxes && key < p.hi && key + box > p.lo;
+      const uint32_t mask = __ballot_sync(0xffffffffu, want);
+      const int slot = key - a.by_page.div(key) * a.page_size;
+      const bool real = (unsigned)page < (unsigned)a.num_pages;
 #pragma unroll 1
       for (int v = 0; ok && v < 2; ++v) {
         ok = ptx::mbar_wait_warp(&sy.empty[stage], phase ^ 1u, abort_flag);
         if (!ok) break;
         uint8_t* dst = smem + (2 + stage) * M::TILE;
-        const int at = rows < 0 ? none : rows + v * a.page_size;
+        const int at = real ? (page * 2 + v) * (a.page_size / 8) + slot / 8 : none;
         if (ptx::elect_one()) ptx::mbar_expect_tx(&sy.full[stage], (uint32_t)(__popc(mask) * box * HD * 2));
-        __syncwarp();
         for (int i = 0; i < boxes; ++i) {
-          const int r = __shfl_sync(0xffffffffu, at, i);
-          if ((mask >> i) & 1u) {
-            if (ptx::elect_one()) {
-#pragma unroll
-              for (int h = 0; h < M::HALVES; ++h)
-                ptx::tma_load_2d(dst + h * M::BOX + i * box * 128, map, &sy.full[stage], p.head * HD + h * 64, r);
-            }
-            __syncwarp();
-          }
+          const int g = __shfl_sync(0xffffffffu, at, i);
+          if ((mask >> i) & 1u)
+            if (ptx::elect_one()) ptx::tma_load_4d(dst + i * groups * M::GROUP, map, &sy.full[stage], 0, 0, p.head * M::HALVES, g);
         }
         ++filled;
         if (++stage == M::STAGES) { stage = 0; phase ^= 1u; }
@@ -508,7 +507,7 @@ __device__ __forceinline__ void many_queries(const AttnArgs& a, uint8_t* smem, M
   constexpr int CPR = HD / 8, RPI = 32 / CPR;  // 16-byte pieces of a row, rows per copy instruction of the warp
   const int lane = threadIdx.x & 31, chunk = lane % CPR, c = chunk & 7, first = lane / CPR;
   volatile int* abort_flag = &sy.abort_word;
-  const uint32_t dst = ptx::smem_u32(smem) + sub * M::TILE + (chunk >> 3) * M::BOX;
+  const uint32_t dst = ptx::smem_u32(smem) + sub * M::TILE + (chunk >> 3) * M::QHALF;
   const T* q = reinterpret_cast<const T*>(a.q) + chunk * 8;
   uint32_t pieces = 0;
   AttnPiece p;
@@ -544,46 +543,37 @@ __device__ __forceinline__ void many_multiply(const AttnArgs& a, uint8_t* smem, 
   const uint32_t id_s = ptx::make_idesc(fmt, 128), id_o = ptx::make_idesc(fmt, HD) | ptx::kIdescBRows;
   const uint32_t tmem = sy.tmem, sq = ptx::smem_u32(smem);
   // descriptors differ in the address field only, which counts 16 bytes
-  const uint64_t d_rows = ptx::make_smem_desc_sw128(sq), d_value = ptx::make_smem_desc_rows_sw128(sq, M::BOX);
-  auto scores = [&](int sub, int stage, bool last) {  // S of half `sub` with the keys in `stage`; the piece's last: q is free
-    if (ptx::elect_one()) {
-      const uint64_t dq = d_rows + (uint64_t)(sub * (M::TILE >> 4)), dk = d_rows + (uint64_t)((2 + stage) * (M::TILE >> 4));
+  const uint64_t d_query = ptx::make_smem_desc_sw128(sq), d_key = ptx::make_smem_desc_groups_sw128(sq, M::GROUP);
+  const uint64_t d_value = ptx::make_smem_desc_rows_sw128(sq, 1024, M::GROUP);
+  // The issuing lane's part.  S of half `sub` with the keys in `stage`:
+  auto scores = [&](int sub, int stage) {
+    const uint64_t dq = d_query + (uint64_t)(sub * (M::TILE >> 4)), dk = d_key + (uint64_t)((2 + stage) * (M::TILE >> 4));
 #pragma unroll
-      for (int k = 0; k < HD / 16; ++k) {
-        const uint64_t off = (uint64_t)((k >> 2) * (M::BOX >> 4) + (k & 3) * 2);
-        ptx::umma_f16(tmem + sub * 128, dq + off, dk + off, id_s, k > 0 ? 1u : 0u);
-      }
-      ptx::umma_commit(&sy.turn[sub]);
-      if (last) ptx::umma_commit(&sy.q_empty[sub]);
-    }
-    __syncwarp();
+    for (int k = 0; k < HD / 16; ++k)
+      ptx::umma_f16(tmem + sub * 128, dq + (uint64_t)((k >> 2) * (M::QHALF >> 4) + (k & 3) * 2),
+                    dk + (uint64_t)((k >> 2) * (1024 >> 4) + (k & 3) * 2), id_s, k > 0 ? 1u : 0u);
   };
+  // O of half `sub` with the values in `stage` that go with a part of P.
   auto output = [&](int sub, int part, int stage, bool first) {
-    if (ptx::elect_one()) {
-      const uint64_t dv = d_value + (uint64_t)((2 + stage) * (M::TILE >> 4) + part * (64 * 128 >> 4));
+    const uint64_t dv = d_value + (uint64_t)((2 + stage) * (M::TILE >> 4) + part * (8 * M::GROUP >> 4));
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
-        ptx::umma_f16_ts(tmem + 256 + sub * HD, tmem + sub * 128 + part * 32 + k * 8, dv + (uint64_t)(k * (16 * 128 >> 4)), id_o,
-                         !first || part > 0 || k > 0 ? 1u : 0u);
-    }
-    __syncwarp();
-  };
-  auto commit = [&](uint64_t* bar) {
-    if (ptx::elect_one()) ptx::umma_commit(bar);
-    __syncwarp();
+    for (int k = 0; k < 4; ++k)
+      ptx::umma_f16_ts(tmem + 256 + sub * HD, tmem + sub * 128 + part * 32 + k * 8, dv + (uint64_t)(k * (2 * M::GROUP >> 4)), id_o,
+                       !first || part > 0 || k > 0 ? 1u : 0u);
   };
   int stage = 0;
   uint32_t phase = 0, p_phase[2][2] = {{0, 0}, {0, 0}}, q_phase[2] = {0, 0};
   bool ok = true;
   auto next_full = [&]() {  // the next stage, once it has been filled
     const int s = stage;
-    ptx::mbar_wait_converged(&sy.full[s], phase, abort_flag);
+    ptx::mbar_wait_lanes(&sy.full[s], phase, abort_flag);
     if (++stage == M::STAGES) { stage = 0; phase ^= 1u; }
     return s;
   };
   auto wait_p = [&](int sub, int part) {
-    ptx::mbar_wait_converged(&sy.p_full[sub][part], p_phase[sub][part], abort_flag);
+    ptx::mbar_wait_lanes(&sy.p_full[sub][part], p_phase[sub][part], abort_flag);
     p_phase[sub][part] ^= 1u;
+    ptx::tc_fence_after();
   };
   AttnPiece p;
   while (ok && walk.next(a, &p)) {
@@ -593,12 +583,16 @@ __device__ __forceinline__ void many_multiply(const AttnArgs& a, uint8_t* smem, 
 #pragma unroll
     for (int s = 0; s < 2; ++s)
       if (s == 0 || both) {
-        ptx::mbar_wait_converged(&sy.q_full[s], q_phase[s], abort_flag);
+        ptx::mbar_wait_lanes(&sy.q_full[s], q_phase[s], abort_flag);
         q_phase[s] ^= 1u;
         ptx::tc_fence_after();
-        scores(s, ks0, p.b0 + 1 == p.b1);
+        if (ptx::elect_one()) {
+          scores(s, ks0);
+          ptx::umma_commit(&sy.turn[s]);
+          if (p.b0 + 1 == p.b1) ptx::umma_commit(&sy.q_empty[s]);
+          if ((s == 1) == both) ptx::umma_commit(&sy.empty[ks0]);
+        }
       }
-    commit(&sy.empty[ks0]);
     for (int b = p.b0; ok && b < p.b1; ++b) {
       const int vs = next_full(), key0 = (p.t.blk_lo + b) * kAttnBlock;
       const bool more = b + 1 < p.b1;
@@ -610,7 +604,8 @@ __device__ __forceinline__ void many_multiply(const AttnArgs& a, uint8_t* smem, 
           const int r = i >> 3;
           if (r < lo || r >= hi)
 #pragma unroll
-            for (int h = 0; h < M::HALVES; ++h) *reinterpret_cast<uint4*>(v + h * M::BOX + i * 16) = make_uint4(0, 0, 0, 0);
+            for (int h = 0; h < M::HALVES; ++h)
+              *reinterpret_cast<uint4*>(v + (r >> 3) * M::GROUP + h * 1024 + (r & 7) * 128 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
         }
         ptx::fence_proxy_async_smem();
         __syncwarp();
@@ -619,21 +614,21 @@ __device__ __forceinline__ void many_multiply(const AttnArgs& a, uint8_t* smem, 
 #pragma unroll
       for (int s = 0; s < 2; ++s)
         if (s == 0 || both) {
-#pragma unroll
-          for (int part = 0; part < 2; ++part) {
-            wait_p(s, part);
-            ptx::tc_fence_after();
-            output(s, part, vs, b == p.b0);
-          }
-          if (more) {
-            if (s == 0) ks = next_full();
-            scores(s, ks, b + 2 == p.b1);
-          } else {
-            commit(&sy.turn[s]);
+          wait_p(s, 0);
+          if (ptx::elect_one()) output(s, 0, vs, b == p.b0);
+          if (s == 0 && more) ks = next_full();
+          wait_p(s, 1);
+          if (ptx::elect_one()) {
+            output(s, 1, vs, b == p.b0);
+            if (more) scores(s, ks);
+            ptx::umma_commit(&sy.turn[s]);
+            if (b + 2 == p.b1) ptx::umma_commit(&sy.q_empty[s]);  // that was the last use of the queries
+            if ((s == 1) == both) {
+              ptx::umma_commit(&sy.empty[vs]);
+              if (more) ptx::umma_commit(&sy.empty[ks]);
+            }
           }
         }
-      commit(&sy.empty[vs]);
-      if (more) commit(&sy.empty[ks]);
       ok = __all_sync(0xffffffffu, *abort_flag == 0);  // a wait may have run out
     }
     if (ok)
@@ -646,7 +641,7 @@ __device__ __forceinline__ void many_multiply(const AttnArgs& a, uint8_t* smem, 
     __shared__ int never;
     if (lane == 0) never = 0;
     __syncwarp();
-    commit(&sy.drain);
+    if (ptx::elect_one()) ptx::umma_commit(&sy.drain);
     ptx::mbar_wait_warp(&sy.drain, 0u, &never);
   }
 }
@@ -671,12 +666,11 @@ __device__ __forceinline__ void many_softmax(const AttnArgs& a, uint8_t* smem, M
     // keys that all rows of this half see need no mask
     const int pos_first = p.t.pos0 + a.by_group.div(p.t.row0 + sub * 128), pos_last = p.hi - 1;
     for (int b = p.b0; b < p.b1; ++b) {
-      ptx::mbar_wait_converged(&sy.turn[sub], phase, abort_flag);
+      ptx::mbar_wait_lanes(&sy.turn[sub], phase, abort_flag);
       phase ^= 1u;
       ptx::tc_fence_after();
       uint32_t raw[128];
-      ptx::tmem_ld_32x64(t_s, raw);
-      ptx::tmem_ld_32x64(t_s + 64, raw + 64);
+      ptx::tmem_ld_32x128(t_s, raw);
       if (a.scale_log2 <= 0.f) {
 #pragma unroll
         for (int i = 0; i < 128; ++i) raw[i] = __float_as_uint(__uint_as_float(raw[i]) * (a.scale_log2 < 0.f ? -1.f : 0.f));
@@ -740,7 +734,7 @@ __device__ __forceinline__ void many_softmax(const AttnArgs& a, uint8_t* smem, M
     }
     const bool any = p.b0 < p.b1;
     if (any) {
-      ptx::mbar_wait_converged(&sy.turn[sub], phase, abort_flag);
+      ptx::mbar_wait_lanes(&sy.turn[sub], phase, abort_flag);
       phase ^= 1u;
       ptx::tc_fence_after();
       if (__any_sync(0xffffffffu, *abort_flag != 0)) return;
@@ -904,8 +898,12 @@ static int launch_tc(const AttnArgs& a, bool many, int workers, cudaStream_t s) 
   constexpr int smem = tc_smem<HD>();
   CUtensorMap map = {};
   if (many) {
-    const int rc = make_tmap_2d(&map, DT<T>::id, a.cache, (int64_t)a.num_pages * 2 * a.page_size, (int64_t)a.kv_heads * HD,
-                                (int64_t)a.kv_heads * HD, min(a.page_size & -a.page_size, kAttnBlock), 64);
+    // [64 columns][8 rows][kv heads x halves][groups of 8 rows]: a box is 64 columns x 8 rows x the halves of a head x its groups
+    const uint64_t row = (uint64_t)a.kv_heads * HD * 2;
+    const uint64_t dims[4] = {64, 8, (uint64_t)a.kv_heads * (HD / 64), (uint64_t)a.num_pages * 2 * (a.page_size / 8)};
+    const uint64_t strides[3] = {row, 128, 8 * row};
+    const uint32_t box[4] = {64, 8, HD / 64, (uint32_t)min(a.page_size & -a.page_size, kAttnBlock) / 8};
+    const int rc = make_tmap_4d(&map, DT<T>::id, a.cache, dims, strides, box);
     if (rc) return rc;
   }
   SB_CUDA(cudaFuncSetAttribute(attn_tc_kernel<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));

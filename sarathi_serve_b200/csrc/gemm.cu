@@ -56,6 +56,25 @@ int make_tmap_2d(CUtensorMap* map, int dtype, const void* ptr, int64_t rows, int
   return SB200_OK;
 }
 
+int make_tmap_4d(CUtensorMap* map, int dtype, const void* ptr, const uint64_t* dims, const uint64_t* strides, const uint32_t* box) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) {
+    set_error("cuTensorMapEncodeTiled is not available from the CUDA driver");
+    return SB200_ERR_CUDA;
+  }
+  const CUtensorMapDataType dt = dtype == SB200_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  cuuint64_t d[4], s[3];
+  cuuint32_t b[4], estr[4] = {1, 1, 1, 1};
+  for (int i = 0; i < 4; ++i) { d[i] = dims[i]; b[i] = box[i]; if (i < 3) s[i] = strides[i]; }
+  const CUresult r = fn(map, dt, 4, const_cast<void*>(ptr), d, s, b, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    set_error("cuTensorMapEncodeTiled failed with CUresult %d (4-D box of %u x %u x %u x %u)", (int)r, b[0], b[1], b[2], b[3]);
+    return SB200_ERR_CUDA;
+  }
+  return SB200_OK;
+}
+
 // Clusters of `cluster_ctas` GEMM CTAs (one CTA per SM) that can be resident at the same time.  A cluster must
 // sit inside one GPC, so this is less than #SMs / cluster_ctas when the GPCs' SM counts are not multiples of the
 // cluster size.  It matters for the row-parallel kernel: its CTAs wait, after their tiles, for flags that depend

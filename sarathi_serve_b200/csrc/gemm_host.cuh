@@ -8,6 +8,8 @@ namespace sb200 {
 
 int make_tmap_2d(CUtensorMap* map, int dtype, const void* ptr, int64_t rows, int64_t cols, int64_t ld_elems,
                  int box_rows, int box_cols);
+// 16-bit elements, strides in bytes (from the second dimension on), 128-byte swizzle.
+int make_tmap_4d(CUtensorMap* map, int dtype, const void* ptr, const uint64_t* dims, const uint64_t* strides, const uint32_t* box);
 // First bytes of a split-K workspace hold the per-(tile, slot) arrival counters (zero between launches).
 constexpr size_t kWsCounterBytes = 64 * 1024;
 

@@ -84,11 +84,10 @@ __device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, v
   return ok;
 }
 
-// The wait of a loop that cannot afford a vote in every turn: all lanes of a warp come out together, with nothing said about
-// whether the wait ran out.  The caller looks at the abort flag every so often (after it is set, a wait takes 256 looks at most).
-__device__ __forceinline__ void mbar_wait_converged(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+// The wait of a loop that cannot afford a vote in every turn: nothing is said about whether the wait ran out, and the lanes need
+// not come out together.  The caller looks at the abort flag every so often (once it is set, a wait takes 256 looks at most).
+__device__ __forceinline__ void mbar_wait_lanes(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
   if (!mbar_try_wait(bar, parity)) mbar_wait(bar, parity, abort_flag);
-  __syncwarp();
 }
 
 // ----------------------------------------------------------------------- TMA
@@ -120,6 +119,14 @@ __device__ __forceinline__ void tma_load_2d_once(void* smem_dst, const CUtensorM
 __device__ __forceinline__ void tma_prefetch_l2_2d(const CUtensorMap* m, int c0, int c1) {
   asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];"
                ::"l"(reinterpret_cast<uint64_t>(m)), "r"(c0), "r"(c1) : "memory");
+}
+
+// 4-D variant (pages of a KV cache).
+__device__ __forceinline__ void tma_load_4d(void* smem_dst, const CUtensorMap* m, uint64_t* bar, int c0, int c1, int c2, int c3) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
+      ::"r"(smem_u32(smem_dst)), "l"(reinterpret_cast<uint64_t>(m)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+      : "memory");
 }
 
 // 3-D variant (expert-stacked weights).
@@ -189,15 +196,13 @@ __device__ __forceinline__ void tmem_ld_32x32(uint32_t taddr, uint32_t* r) {
       : "memory");
 }
 
-// 64 columns with two loads in flight.
+// 64 and 128 columns, their loads in flight together.
 __device__ __forceinline__ void tmem_ld_32x64(uint32_t taddr, uint32_t* r) {
   __syncwarp();
 #define SB_LD32(O, A) "tcgen05.ld.sync.aligned.32x32b.x32.b32 {" O "}, [" A "];\n\t"
   asm volatile(
-      SB_LD32("%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-              "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31", "%64")
-      SB_LD32("%32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, "
-              "%48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63", "%65")
+      SB_LD32("%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31", "%64")
+      SB_LD32("%32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, %48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63", "%65")
       "tcgen05.wait::ld.sync.aligned;"
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
         "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
@@ -208,6 +213,35 @@ __device__ __forceinline__ void tmem_ld_32x64(uint32_t taddr, uint32_t* r) {
         "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]),
         "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
       : "r"(taddr), "r"(taddr + 32)
+      : "memory");
+#undef SB_LD32
+}
+__device__ __forceinline__ void tmem_ld_32x128(uint32_t taddr, uint32_t* r) {
+  __syncwarp();
+#define SB_LD32(O, A) "tcgen05.ld.sync.aligned.32x32b.x32.b32 {" O "}, [" A "];\n\t"
+  asm volatile(
+      SB_LD32("%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31", "%128")
+      SB_LD32("%32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, %48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63", "%129")
+      SB_LD32("%64, %65, %66, %67, %68, %69, %70, %71, %72, %73, %74, %75, %76, %77, %78, %79, %80, %81, %82, %83, %84, %85, %86, %87, %88, %89, %90, %91, %92, %93, %94, %95", "%130")
+      SB_LD32("%96, %97, %98, %99, %100, %101, %102, %103, %104, %105, %106, %107, %108, %109, %110, %111, %112, %113, %114, %115, %116, %117, %118, %119, %120, %121, %122, %123, %124, %125, %126, %127", "%131")
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]),
+        "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]),
+        "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]),
+        "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]),
+        "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63]),
+        "=r"(r[64]), "=r"(r[65]), "=r"(r[66]), "=r"(r[67]), "=r"(r[68]), "=r"(r[69]), "=r"(r[70]), "=r"(r[71]),
+        "=r"(r[72]), "=r"(r[73]), "=r"(r[74]), "=r"(r[75]), "=r"(r[76]), "=r"(r[77]), "=r"(r[78]), "=r"(r[79]),
+        "=r"(r[80]), "=r"(r[81]), "=r"(r[82]), "=r"(r[83]), "=r"(r[84]), "=r"(r[85]), "=r"(r[86]), "=r"(r[87]),
+        "=r"(r[88]), "=r"(r[89]), "=r"(r[90]), "=r"(r[91]), "=r"(r[92]), "=r"(r[93]), "=r"(r[94]), "=r"(r[95]),
+        "=r"(r[96]), "=r"(r[97]), "=r"(r[98]), "=r"(r[99]), "=r"(r[100]), "=r"(r[101]), "=r"(r[102]), "=r"(r[103]),
+        "=r"(r[104]), "=r"(r[105]), "=r"(r[106]), "=r"(r[107]), "=r"(r[108]), "=r"(r[109]), "=r"(r[110]), "=r"(r[111]),
+        "=r"(r[112]), "=r"(r[113]), "=r"(r[114]), "=r"(r[115]), "=r"(r[116]), "=r"(r[117]), "=r"(r[118]), "=r"(r[119]),
+        "=r"(r[120]), "=r"(r[121]), "=r"(r[122]), "=r"(r[123]), "=r"(r[124]), "=r"(r[125]), "=r"(r[126]), "=r"(r[127])
+      : "r"(taddr), "r"(taddr + 32), "r"(taddr + 64), "r"(taddr + 96)
       : "memory");
 #undef SB_LD32
 }
@@ -353,12 +387,16 @@ __device__ __forceinline__ uint64_t make_smem_desc_sw128(uint32_t smem_addr) {
          | (2ull << 61);                          // layout: SWIZZLE_128B
 }
 
-// B operand whose rows are the K side ([K rows][64 columns] boxes with 128-byte swizzle): N runs along a row, 64 columns per
-// box, boxes `box_bytes` apart; K runs over the rows, 8 of them per 1024 bytes.  Goes with kIdescBRows in the descriptor.
-__device__ __forceinline__ uint64_t make_smem_desc_rows_sw128(uint32_t smem_addr, uint32_t box_bytes) {
+// The same for rows that lie in groups of 8 x 128 bytes, `group_bytes` apart.
+__device__ __forceinline__ uint64_t make_smem_desc_groups_sw128(uint32_t smem_addr, uint32_t group_bytes) {
+  return (uint64_t)((smem_addr & 0x3FFFFu) >> 4) | (1ull << 16) | ((uint64_t)(group_bytes >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+// B operand whose rows are the K side (groups of 8 rows x 64 columns with 128-byte swizzle): N runs along a row, the next 64
+// columns `column_bytes` further; K runs over the rows, the next 8 of them `group_bytes` further.  Goes with kIdescBRows.
+__device__ __forceinline__ uint64_t make_smem_desc_rows_sw128(uint32_t smem_addr, uint32_t column_bytes, uint32_t group_bytes) {
   return (uint64_t)((smem_addr & 0x3FFFFu) >> 4)
-         | ((uint64_t)(box_bytes >> 4) << 16)     // leading byte offset: to the next 64 columns
-         | (64ull << 32)                          // stride byte offset: to the next 8 rows
+         | ((uint64_t)(column_bytes >> 4) << 16)  // leading byte offset
+         | ((uint64_t)(group_bytes >> 4) << 32)   // stride byte offset
          | (1ull << 46)
          | (2ull << 61);
 }
