@@ -61,29 +61,6 @@ __device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
-// 2^x for x <= 2^8 on the FMA pipes: x = n + f with n the nearest integer (adding 1.5 * 2^23 leaves it in the low bits), 2^f by a
-// polynomial, n added to the exponent.  The coefficients are fitted to 2^f on [-1/2, 1/2] for the least largest relative error
-// of a polynomial that is 1 at 0: degree 3, 1.02e-4, where the result is rounded to bf16 (2^-9), degree 4, 2.9e-6, for fp16
-// (2^-12).  From -127 down the result is exactly 0 (there f = 0, and the exponent of 1 less 127 is that of 0), between -126 and -127
-// less than 2^-126.
-template <typename T> __device__ __forceinline__ f32x2 pow2_pair(f32x2 x) {
-  auto both = [](float c) { return pair(c, c); };
-  x = pair(fmaxf(low(x), -127.f), fmaxf(high(x), -127.f));
-  const f32x2 t = add2(x, both(12582912.f)), n = add2(t, both(-12582912.f)), f = fma2(n, both(-1.f), x);
-  f32x2 y;
-  if constexpr (DT<T>::id == SB200_BF16) {
-    y = fma2(f, both(0.05500893294811249f), both(0.24221095442771912f));
-    y = fma2(y, f, both(0.6932829022407532f));
-  } else {
-    y = fma2(f, both(0.009582852944731712f), both(0.055906426161527634f));
-    y = fma2(y, f, both(0.24024099111557007f));
-    y = fma2(y, f, both(0.6931241750717163f));
-  }
-  y = fma2(y, f, both(1.f));
-  return pair((uint32_t)y + ((uint32_t)t << 23), (uint32_t)(y >> 32) + ((uint32_t)(t >> 32) << 23));
-}
-constexpr int kPoly = 3;
-
 // The largest of three, or NaN if one of them is.
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
@@ -688,9 +665,35 @@ __device__ __forceinline__ void many_softmax(const AttnArgs& a, uint8_t* smem, M
             if (i <= lo) raw[i] = 0xff800000u;
         }
       }
+      // The probabilities of the first 64 keys are made with the maximum as it stands while the block's own is being found, and made
+      // again in the rare case that it has grown too far.  (The maximum first, then the exponentials: 250 clocks of 2900 a block more.)
+      uint32_t prob[32];
+      f32x2 sum0, sum1;
+      auto exponentials = [&](int part) {
+        const float base = m == -INFINITY ? 0.f : -m * scale;
+        const f32x2 sc = pair(scale, scale), bs = pair(base, base);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          const f32x2 x = fma2(pair(raw[part * 64 + 2 * i], raw[part * 64 + 2 * i + 1]), sc, bs);
+          const f32x2 y = pair(pow2(low(x)), pow2(high(x)));
+          if (i == 0 && part == 0) sum0 = y;
+          else if (i == 1 && part == 0) sum1 = y;
+          else if (i & 1) sum1 = add2(sum1, y);
+          else sum0 = add2(sum0, y);
+          prob[i] = pack2<T>(low(y), high(y));
+        }
+      };
+      auto publish = [&](int part) {
+        ptx::tmem_st_32x32(t_s + part * 32, prob);
+        ptx::tmem_wait_st();
+        ptx::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(&sy.p_full[sub][part]);
+      };
       float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
       for (int i = 0; i < 64; ++i) top[i & 3] = max3(top[i & 3], __uint_as_float(raw[2 * i]), __uint_as_float(raw[2 * i + 1]));
+      exponentials(0);
       const float now = max3(max3(top[0], top[1], top[2]), top[3], -INFINITY);
       const bool grow = now != -INFINITY && !((now - m) * scale <= kLazy);  // (also the first score, and one that is no number)
       if (__any_sync(0xffffffffu, grow)) {
@@ -707,28 +710,11 @@ __device__ __forceinline__ void many_softmax(const AttnArgs& a, uint8_t* smem, M
             ptx::tmem_st_32x32(t_o + i * 32, o);
           }
         }
+        exponentials(0);
       }
-      const float base = m == -INFINITY ? 0.f : -m * scale;
-      // kPoly of every eight pairs go to the FMA pipes (pow2_pair), the others to the exponential unit; both make a masked score 0
-      const f32x2 sc = pair(scale, scale), bs = pair(base, base);
-      f32x2 sum0 = pair(0.f, 0.f), sum1 = pair(0.f, 0.f);
-#pragma unroll
-      for (int part = 0; part < 2; ++part) {
-        uint32_t prob[32];
-#pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          const f32x2 x = fma2(pair(raw[part * 64 + 2 * i], raw[part * 64 + 2 * i + 1]), sc, bs);
-          const f32x2 y = i % 8 < kPoly ? pow2_pair<T>(x) : pair(pow2(low(x)), pow2(high(x)));
-          if (i & 1) sum1 = add2(sum1, y);
-          else sum0 = add2(sum0, y);
-          prob[i] = pack2<T>(low(y), high(y));
-        }
-        ptx::tmem_st_32x32(t_s + part * 32, prob);
-        ptx::tmem_wait_st();
-        ptx::tc_fence_before();
-        __syncwarp();
-        if (lane == 0) ptx::mbar_arrive(&sy.p_full[sub][part]);
-      }
+      publish(0);
+      exponentials(1);
+      publish(1);
       sum0 = add2(sum0, sum1);
       l += low(sum0) + high(sum0);
     }

@@ -4,9 +4,8 @@ Tolerances (u(t) = eps(t) / 2, the most that one rounding is off, relative to th
   * the result is rounded once:                        u(dtype) |o|
   * fp16 / bf16 round the probabilities once:          u(dtype) W,  W = sum_j p_j |v_j|
   * a score is off by at most (hd + 16) 2^-24 A, A = scale max_j sum_i |q_i k_ji| (fp32 products summed in any order, scaling,
-    the subtraction of the maximum), the power of two by E relative: fp32 2^-21 (two units of exp2f), fp16 2^-18 (a polynomial
-    that is off by 2.9e-6 at most, and its rounding), bf16 2^-13 (one that is off by 1.02e-4); that moves numerator and
-    denominator alike:                                 2 ((hd + 16) 2^-24 A + E) W
+    the subtraction of the maximum), the power of two by 2^-21 relative (two units of its approximation); that moves numerator
+    and denominator alike:                             2 ((hd + 16) 2^-24 A + 2^-21) W
   * fp32 sums over n keys, twice (numerator, denominator), and a join:  2 (n + 16) 2^-24 W
   * fp16 probabilities below its smallest step:        n 2^-25 max|v|   (the sum they are divided by is at least 1)
 Nothing is compared where a result is not finite; non-finite results are expected exactly where 64 bits have them."""
@@ -95,7 +94,7 @@ def reference(c, scale, window=0):
                     va = torch.where(bad, 0, vz).abs()
                     W = p @ va
                     A = (q[:, h].abs() @ torch.where(torch.isfinite(kh), kh, 0).abs().T * abs(scale)).amax(1)
-                    delta = (hd + 16) * 2.0 ** -24 * A + 2.0 ** {torch.float32: -21, torch.float16: -18, torch.bfloat16: -13}[c["dtype"]]
+                    delta = (hd + 16) * 2.0 ** -24 * A + 2.0 ** -21
                     t = u * res.abs() + (2 * delta[:, None] + 2 * (n + 16) * 2.0 ** -24) * W
                     if c["dtype"] != torch.float32:
                         t = t + u * W
