@@ -18,11 +18,14 @@ struct PlanArgs {
   AttnShape sh;
 };
 
-// What a block of keys, and a unit apart from its blocks, costs a CTA: see the measurements in attention_tc.cu.
-__device__ __forceinline__ void unit_cost(int kind, int nrows, int* block, int* fixed, int* least) {
-  if (kind == ATTN_MANY) { *block = nrows > 128 ? 8 : 6; *fixed = 12; *least = 2; }
-  else if (kind == ATTN_FEW) { *block = 8; *fixed = 4; *least = 2; }
-  else { *block = 8; *fixed = 2; *least = 1; }
+// What a block of keys, and a unit apart from its blocks, costs a CTA, in tenths of a microsecond, and the least blocks of a
+// piece.  Measured with every SM at the same kind: units of 1 to 64 blocks, and several of them one after the other.  Few rows
+// count at the share of HBM that an SM has when all of them stream.
+__device__ __forceinline__ void unit_cost(const AttnShape& sh, int kind, int nrows, int* block, int* fixed, int* least) {
+  const bool wide = sh.head_dim > 64;
+  if (kind == ATTN_MANY) { *block = nrows > 128 ? (wide ? 17 : 15) : (wide ? 15 : 14); *fixed = 45; *least = 2; }
+  else if (kind == ATTN_FEW) { *block = sh.head_dim == 256 ? 39 : wide ? 15 : 10; *fixed = 22; *least = 2; }
+  else { *block = 20; *fixed = 10; *least = 1; }
 }
 
 __device__ __forceinline__ long long scan_block(long long v, long long* red, long long* total) {
@@ -131,20 +134,15 @@ attn_plan_kernel(const PlanArgs a) {
       dst[0] = make_int4(d.q_row, d.row0, d.nrows, d.kind);
       dst[1] = make_int4(d.pos0, d.page_at, d.blk_lo, d.nblk);
       int block, fixed, least;
-      unit_cost(d.kind, d.nrows, &block, &fixed, &least);
+      unit_cost(sh, d.kind, d.nrows, &block, &fixed, &least);
       c = ((long long)d.nblk * block + fixed) * sh.kv_heads;
     }
     const long long at = carry + scan_block(c, red, &total);
     if (t < tiles) a.plan.cost[t] = at;
     carry += total;
   }
-  if (threadIdx.x == 0) {
-    a.plan.cost[tiles] = carry;
-    a.plan.header[0] = tiles;
-    a.plan.header[1] = a.workers;
-    a.plan.header[3] = two ? tiles_many : 0;
-    a.plan.header[2] = a.n ? max(0, min(a.qo_indptr[a.n], a.max_tokens)) : 0;
-  }
+  __shared__ int4 at[kAttnMaxWorkers + 1];
+  if (threadIdx.x == 0) a.plan.cost[tiles] = carry;
   __syncthreads();
   for (int w = threadIdx.x; w <= a.workers; w += kPlanThreads) {
     int4 out = make_int4(tiles, 0, 0, 0);
@@ -158,7 +156,7 @@ attn_plan_kernel(const PlanArgs a) {
       }
       const AttnTile d = a.plan.tiles[lo];
       int block, fixed, least;
-      unit_cost(d.kind, d.nrows, &block, &fixed, &least);
+      unit_cost(sh, d.kind, d.nrows, &block, &fixed, &least);
       const long long unit = (long long)d.nblk * block + fixed, rem = x - a.plan.cost[lo];
       int head = (int)(rem / unit);
       const long long in = rem - head * unit;
@@ -168,12 +166,30 @@ attn_plan_kernel(const PlanArgs a) {
       else if (d.nblk - blk < least) { blk = 0; ++head; }
       out = head < sh.kv_heads ? make_int4(lo, head, blk, 0) : make_int4(lo + 1, 0, 0, 0);
     }
-    a.plan.starts[w] = out;
+    at[w] = out;
+  }
+  __syncthreads();
+  for (int w = threadIdx.x; w <= a.workers; w += kPlanThreads) {
+    AttnStart s;
+    s.at = at[w];
+    s.tile = s.at.x < tiles ? a.plan.tiles[s.at.x] : AttnTile{};
+    s.many = two ? tiles_many : 0;
+    s.rows = a.n ? max(0, min(a.qo_indptr[a.n], a.max_tokens)) : 0;
+    s.pieces = s.pad = 0;
+    auto same = [&](int v) { return at[v].x == s.at.x && at[v].y == s.at.y; };
+    if (w > 0 && w < a.workers && s.at.z > 0 && !(same(w - 1) && at[w - 1].z > 0)) {
+      int last = w;  // the workers w .. last begin inside this unit
+      while (last + 1 < a.workers && same(last + 1)) ++last;
+      s.pieces = last - w + 2;
+    }
+    const int4* src = reinterpret_cast<const int4*>(&s);
+    int4* dst = reinterpret_cast<int4*>(a.plan.starts + w);
+    for (int i = 0; i < 4; ++i) dst[i] = src[i];
   }
 }
 
 // Joins the pieces of cut units: o = sum_p 2^(l_p - m) o_p / sum_p 2^(l_p - m) with l_p the log2 of piece p's sum, in the
-// order of the keys.  CTA (x, y): the unit that worker x's share begins inside of, if it is the first such worker, rows
+// order of the keys.  CTA (x, y): the unit that the share of worker x + 1 begins inside of, if that is the first such worker, rows
 // y, y + gridDim.y ... of it, a warp per row.  Also clears the rows of q that belong to no request, when asked to.
 template <typename T, int HD>
 __global__ void __launch_bounds__(128)
@@ -181,10 +197,11 @@ attn_join_kernel(const AttnArgs a) {
   grid_dependency_begin();
   constexpr int N = HD / 32;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int workers = a.plan.header[1];
   T* out = reinterpret_cast<T*>(a.out);
+  const int w = min((int)blockIdx.x + 1, a.workers);
+  const AttnStart s = a.plan.starts[w];
   if (a.zero_behind) {
-    const int rows0 = min(a.plan.header[2], a.num_tokens), per_row = a.kv_heads * a.group * HD;
+    const int rows0 = min(s.rows, a.num_tokens), per_row = a.kv_heads * a.group * HD;
     const int ctas = gridDim.x * gridDim.y, cta = blockIdx.y * gridDim.x + blockIdx.x;
     for (int t = rows0 + cta; t < a.num_tokens; t += ctas) {
       for (int i = threadIdx.x; i < per_row; i += blockDim.x) out[t * a.ldo + i] = DT<T>::from_f(0.f);
@@ -193,27 +210,17 @@ attn_join_kernel(const AttnArgs a) {
           a.lse[(int64_t)t * (a.kv_heads * a.group) + i] = -INFINITY;
     }
   }
-  const int w = blockIdx.x + 1;
-  if (w >= workers) return;
-  const int4 at = a.plan.starts[w], before = a.plan.starts[w - 1];
-  if (at.z == 0 || (before.x == at.x && before.y == at.y && before.z > 0)) return;
-  int last = w;  // the workers w .. last begin inside this unit
-  while (last + 1 < workers) {
-    const int4 n = a.plan.starts[last + 1];
-    if (n.x != at.x || n.y != at.y) break;
-    ++last;
-  }
+  if (s.pieces == 0) return;
   AttnPiece p;
-  p.t = a.plan.tiles[at.x];
-  p.head = at.y;
-  const int rows = (int)min((long long)p.t.nrows, max(0ll, ((long long)a.num_tokens - p.t.q_row) * a.group - p.t.row0));
+  p.t = s.tile;
+  p.head = s.at.y;
+  const int rows = min(p.t.nrows, max(0, (a.num_tokens - p.t.q_row) * a.group - p.t.row0)), pieces = s.pieces;
   for (int r = blockIdx.y * 4 + warp; r < rows; r += gridDim.y * 4) {
     // piece 0 is the last of worker w - 1, piece i > 0 the first of worker w + i - 1 (none, if the next one begins there too)
-    const int pieces = last - w + 2;
     auto slot = [&](int i) { return i == 0 ? 2 * (w - 1) + 1 : 2 * (w + i - 1); };
     auto lse_of = [&](int i) {
       if (i > 0 && i + 1 < pieces) {
-        const int4 x = a.plan.starts[w + i - 1], y = a.plan.starts[w + i];
+        const int4 x = a.plan.starts[w + i - 1].at, y = a.plan.starts[w + i].at;
         if (x.x == y.x && x.y == y.y && x.z == y.z) return -INFINITY;
       }
       return a.part_l[(int64_t)slot(i) * a.slot_rows + r];
@@ -294,10 +301,8 @@ static size_t align16(size_t v) { return (v + 15) & ~size_t(15); }
 static size_t plan_view(void* base, int64_t cap, AttnPlanView* v) {
   uint8_t* p = reinterpret_cast<uint8_t*>(base);
   size_t at = 0;
-  v->header = reinterpret_cast<int*>(p + at);
-  at += kAttnHeaderInts * sizeof(int);
-  v->starts = reinterpret_cast<int4*>(p + at);
-  at += (kAttnMaxWorkers + 1) * sizeof(int4);
+  v->starts = reinterpret_cast<AttnStart*>(p + at);
+  at += (kAttnMaxWorkers + 1) * sizeof(AttnStart);
   v->cost = reinterpret_cast<long long*>(p + at);
   at += align16((size_t)(cap + 1) * sizeof(long long));
   v->tiles = reinterpret_cast<AttnTile*>(p + at);
@@ -402,7 +407,7 @@ extern "C" int sb200_paged_attention(void* out, int64_t ldo, float* lse, const v
   a.status = status;
   a.scale_log2 = scale * 1.4426950408889634f;
   a.zero_behind = zero_rows_behind;
-  const int workers = attn_workers();
+  const int workers = a.workers = attn_workers();
   cudaStream_t s = (cudaStream_t)stream;
   if (int rc = sh.dtype == SB200_F32 ? run_attn_simt(sh.head_dim, a, workers, s)
                                      : run_attn_tc(sh.dtype, sh.head_dim, a, sh, workers, s))

@@ -20,7 +20,6 @@ namespace sb200 {
 
 constexpr int kAttnBlock = 128;       // keys of a block
 constexpr int kAttnMaxWorkers = 256;  // (B200: 148 SMs)
-constexpr int kAttnHeaderInts = 16;
 
 // How the rows of a tile are computed.
 enum { ATTN_SIMT = 0, ATTN_FEW = 1, ATTN_MANY = 2 };
@@ -35,9 +34,19 @@ struct AttnTile {
   int blk_lo, nblk;  // blocks of keys that some row sees
 };
 
+// Where a worker's share begins, with the tile it begins in, in one line of memory: what a CTA needs before its first load of
+// keys is one load away.
+struct alignas(16) AttnStart {
+  int4 at;        // (tile, head, block); (tiles, 0, 0) behind the last
+  AttnTile tile;  // of `at`
+  int many;       // tiles of many rows (they come before the others)
+  int pieces;     // > 0: this worker is the first that begins inside the unit `at`, which is cut into so many pieces
+  int rows;       // rows of q that belong to a request
+  int pad;
+};
+
 struct AttnPlanView {
-  int* header;       // number of tiles, workers, rows of q that belong to a request, tiles of many rows (they come first)
-  int4* starts;      // [workers + 1] (tile, head, block): where each worker's share begins
+  AttnStart* starts; // [workers + 1]
   long long* cost;   // [tiles + 1] start of every tile on the line
   AttnTile* tiles;
   int tiles_cap;
@@ -75,6 +84,7 @@ struct AttnArgs {
   uint32_t* status;
   int64_t num_kv_indices;
   int num_pages, num_tokens;
+  int workers;
   int kv_heads, group, page_size, window, slot_rows;
   FastDiv by_group, by_page;
   float scale_log2;    // scale * log2(e): scores in powers of two
@@ -91,32 +101,52 @@ struct AttnPiece {
 // Walks a worker's share of the line.
 struct AttnWalk {
   int4 cur, end;
-  int worker;
-  __device__ __forceinline__ AttnWalk(const AttnArgs& a, int w) : cur(a.plan.starts[w]), end(a.plan.starts[w + 1]), worker(w) {}
-  // Only the tiles before `tile`, or from it on.
-  __device__ __forceinline__ void until(int tile) { if (end.x >= tile) end = make_int4(tile, 0, 0, 0); }
-  __device__ __forceinline__ void from(int tile) { if (cur.x < tile) cur = make_int4(tile, 0, 0, 0); }
+  AttnTile tile;  // of cur
+  int worker, many;
+  __device__ __forceinline__ AttnWalk(const AttnArgs& a, int w) : worker(w) {
+    const int4* s = reinterpret_cast<const int4*>(a.plan.starts + w);
+    const int4 x = s[0], u = s[1], v = s[2], e = s[3];
+    end = reinterpret_cast<const int4*>(a.plan.starts + w + 1)[0];
+    cur = x;
+    tile = AttnTile{u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+    many = e.x;
+  }
+  __device__ __forceinline__ void fetch(const AttnArgs& a) {
+    if (!more()) return;
+    const int4* src = reinterpret_cast<const int4*>(a.plan.tiles + cur.x);
+    const int4 u = src[0], v = src[1];
+    tile = AttnTile{u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+  }
+  // Only the tiles of many rows, or the others.
+  __device__ __forceinline__ void only_many() { if (end.x >= many) end = make_int4(many, 0, 0, 0); }
+  __device__ __forceinline__ void only_few(const AttnArgs& a) {
+    if (cur.x < many) {
+      cur = make_int4(many, 0, 0, 0);
+      fetch(a);
+    }
+  }
   __device__ __forceinline__ bool more() const {
     return cur.x < end.x || (cur.x == end.x && (cur.y < end.y || (cur.y == end.y && cur.z < end.z)));
   }
   __device__ __forceinline__ bool next(const AttnArgs& a, AttnPiece* p) {
     if (!more()) return false;
-    const int4* src = reinterpret_cast<const int4*>(a.plan.tiles + cur.x);
-    const int4 u = src[0], v = src[1];
-    p->t = AttnTile{u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+    p->t = tile;
     p->head = cur.y;
     p->b0 = cur.z;
     p->b1 = cur.x == end.x && cur.y == end.y ? end.z : p->t.nblk;
     const bool head_cut = p->b0 > 0, tail_cut = p->b1 < p->t.nblk;
     p->slot = head_cut ? 2 * worker : tail_cut ? 2 * worker + 1 : -1;
-    // q may have fewer rows than the plan was made for
-    // (tokens x group stays below 2^30)
+    // q may have fewer rows than the plan was made for (tokens x group stays below 2^30)
     p->t.nrows = min(p->t.nrows, max(0, (a.num_tokens - p->t.q_row) * a.group - p->t.row0));
     const int first = a.by_group.div(p->t.row0), last = a.by_group.div(p->t.row0 + max(p->t.nrows, 1) - 1);
     p->hi = max(0, p->t.pos0 + last + 1);
     p->lo = a.window > 0 ? max(0, p->t.pos0 + first + 1 - a.window) : 0;
-    if (cur.y + 1 < a.kv_heads) cur = make_int4(cur.x, cur.y + 1, 0, 0);
-    else cur = make_int4(cur.x + 1, 0, 0, 0);
+    if (cur.y + 1 < a.kv_heads) {
+      cur = make_int4(cur.x, cur.y + 1, 0, 0);
+    } else {
+      cur = make_int4(cur.x + 1, 0, 0, 0);
+      fetch(a);  // (in good time for the next call)
+    }
     return true;
   }
 };

@@ -28,9 +28,8 @@ attn_simt_kernel(const AttnArgs a) {
   const T* q = reinterpret_cast<const T*>(a.q);
   const T* cache = reinterpret_cast<const T*>(a.cache);
   const int64_t ldc = (int64_t)a.kv_heads * HD;
-  const int workers = a.plan.header[1];
 
-  for (int w = blockIdx.x; w < workers; w += gridDim.x) {
+  for (int w = blockIdx.x; w < a.workers; w += gridDim.x) {
     AttnWalk walk(a, w);
     AttnPiece p;
     while (walk.next(a, &p)) {

@@ -167,7 +167,7 @@ template <int HD> struct FewSteps {
   AttnWalk walk;
   AttnPiece p;
   int key, end;   // next step of the current piece, and where it ends
-  __device__ __forceinline__ FewSteps(const AttnArgs& a, int worker) : walk(a, worker), key(0), end(0) { walk.from(a.plan.header[3]); }
+  __device__ __forceinline__ FewSteps(const AttnArgs& a, int worker) : walk(a, worker), key(0), end(0) { walk.only_few(a); }
   __device__ __forceinline__ bool next_piece(const AttnArgs& a, int warp) {
     if (!walk.next(a, &p)) return false;
     key = (max(p.lo, (p.t.blk_lo + p.b0) * kAttnBlock) & ~(kFewKeys - 1)) + warp * kFewKeys;
@@ -823,7 +823,6 @@ attn_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUten
   extern __shared__ uint8_t smem_tc[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_tc) + 1023) & ~uintptr_t(1023));
   ptx::grid_dependency_wait();
-  if ((int)blockIdx.x >= a.plan.header[1]) return;
   if constexpr (HD == 256) {
     ptx::grid_launch_dependents();
     few_share<T, HD>(a, smem, blockIdx.x);
@@ -831,7 +830,7 @@ attn_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUten
     __shared__ __align__(8) ManySync sy;
     const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0);
     AttnWalk walk(a, blockIdx.x);
-    walk.until(a.plan.header[3]);
+    walk.only_many();
     const bool many = walk.more();  // the same for the whole CTA
     if (many) {
       if (threadIdx.x == 0) {
