@@ -186,7 +186,8 @@ __device__ void few_share(const AttnArgs& a, uint8_t* smem, int worker) {
   constexpr int KS = HD / 16, NT = HD / 8;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
   const uint32_t ring = ptx::smem_u32(smem) + warp * (F::STAGES * 2 * F::HALF);
-  float* join = reinterpret_cast<float*>(smem + F::RING);               // [warp][row of a pass][HD]
+  float* join = reinterpret_cast<float*>(smem + F::RING);               // [warp][row of a pass][HD], and the query rows before
+  const uint32_t sq = ptx::smem_u32(join + warp * 8 * HD);
   float* stat_m = reinterpret_cast<float*>(smem + F::RING + F::JOIN);   // [warp][16]
   float* stat_l = stat_m + F::WARPS * kFewRows;
   const T* cache = reinterpret_cast<const T*>(a.cache);
@@ -232,22 +233,33 @@ __device__ void few_share(const AttnArgs& a, uint8_t* smem, int worker) {
   int get = 0;
   while (st.next_piece(a, warp)) {
     const AttnPiece& p = st.p;
-    // query rows as the A operand: rows g and g + 8, columns 2 t and 2 t + 8 of every 16
-    uint32_t qf[KS][4];
-    int pos_lo, pos_hi;
+    // The query rows, 16 x HD, to this warp's part of the join buffer (swizzled like the keys): as the A operand they come from
+    // there in every step, which costs less than the registers they would take.
+    {
+      T* q = reinterpret_cast<T*>(join + warp * 8 * HD);
+      constexpr int RPI = 32 / CPR > 0 ? 32 / CPR : 1;
+      const int sub = lane / CPR, chunk = lane % CPR;
+      uint4 x[16 / RPI];
+#pragma unroll
+      for (int i = 0; i < 16 / RPI; ++i) {
+        const int r = i * RPI + sub;
+        int token, head, pos;
+        attn_row(a, p, r, &token, &head, &pos);
+        x[i] = make_uint4(0, 0, 0, 0);
+        if (r < p.t.nrows) x[i] = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.q) + token * a.ldq + head * HD + chunk * 8);
+      }
+#pragma unroll
+      for (int i = 0; i < 16 / RPI; ++i) {
+        const int r = i * RPI + sub;
+        *reinterpret_cast<uint4*>(q + r * HD + ((chunk ^ (r & 7)) << 3)) = x[i];
+      }
+      __syncwarp();
+    }
+    int pos_lo, pos_hi;  // of rows g and g + 8
     {
       int token, head;
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const int r = g + 8 * half;
-        attn_row(a, p, min(r, max(p.t.nrows - 1, 0)), &token, &head, half ? &pos_hi : &pos_lo);
-        const T* src = reinterpret_cast<const T*>(a.q) + token * a.ldq + head * HD + 2 * t4;
-#pragma unroll
-        for (int k = 0; k < KS; ++k)
-#pragma unroll
-          for (int c = 0; c < 2; ++c)
-            qf[k][half + 2 * c] = r < p.t.nrows ? *reinterpret_cast<const uint32_t*>(src + k * 16 + c * 8) : 0u;
-      }
+      attn_row(a, p, min(g, max(p.t.nrows - 1, 0)), &token, &head, &pos_lo);
+      attn_row(a, p, min(g + 8, max(p.t.nrows - 1, 0)), &token, &head, &pos_hi);
     }
     const int pos_first = p.t.pos0 + a.by_group.div(p.t.row0), pos_last = p.hi - 1;
     float o[NT][4];
@@ -262,14 +274,15 @@ __device__ void few_share(const AttnArgs& a, uint8_t* smem, int worker) {
       if (++get == F::STAGES) get = 0;
       float s[2][4] = {};
       {
-        const int r = ((lane >> 4) << 3) + (lane & 7), c = (lane >> 3) & 1;
+        const int r = ((lane >> 4) << 3) + (lane & 7), c = (lane >> 3) & 1, rq = lane & 15, cq = lane >> 4;
 #pragma unroll
         for (int k0 = 0; k0 < KS; k0 += 4) {
           constexpr int KB = 4;
-          uint32_t kf[KB][4];
+          uint32_t kf[KB][4], qf[KB][4];
           load_matrices<KB, false>(kf, [&](int k) { return sk + r * F::ROW + ((((k0 + k) * 2 + c) ^ (r & 7)) << 4); });
+          load_matrices<KB, false>(qf, [&](int k) { return sq + rq * F::ROW + ((((k0 + k) * 2 + cq) ^ (rq & 7)) << 4); });
           multiply<T, 2 * KB>([&](int i, float** cc, const uint32_t** aa, const uint32_t** bb) {
-            *cc = s[i & 1]; *aa = qf[k0 + (i >> 1)]; *bb = &kf[i >> 1][2 * (i & 1)];
+            *cc = s[i & 1]; *aa = qf[i >> 1]; *bb = &kf[i >> 1][2 * (i & 1)];
           });
         }
       }
