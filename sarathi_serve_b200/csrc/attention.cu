@@ -178,9 +178,12 @@ attn_plan_kernel(const PlanArgs a) {
     s.pieces = s.pad = 0;
     auto same = [&](int v) { return at[v].x == s.at.x && at[v].y == s.at.y; };
     if (w > 0 && w < a.workers && s.at.z > 0 && !(same(w - 1) && at[w - 1].z > 0)) {
-      int last = w;  // the workers w .. last begin inside this unit
-      while (last + 1 < a.workers && same(last + 1)) ++last;
-      s.pieces = last - w + 2;
+      // The last piece of worker w - 1, then the first of every worker that begins inside the unit, unless the next one begins
+      // at the same place.  (Entries of one unit stay below those of the next: it has at most twice as many as workers.)
+      int* slots = a.plan.slots + 2 * (w - 1);
+      slots[s.pieces++] = 2 * (w - 1) + 1;
+      for (int v = w; v < a.workers && same(v); ++v)
+        if (v + 1 == a.workers || !same(v + 1) || at[v + 1].z > at[v].z) slots[s.pieces++] = 2 * v;
     }
     const int4* src = reinterpret_cast<const int4*>(&s);
     int4* dst = reinterpret_cast<int4*>(a.plan.starts + w);
@@ -190,9 +193,12 @@ attn_plan_kernel(const PlanArgs a) {
 
 // Joins the pieces of cut units: o = sum_p 2^(l_p - m) o_p / sum_p 2^(l_p - m) with l_p the log2 of piece p's sum, in the
 // order of the keys.  CTA (x, y): the unit that the share of worker x + 1 begins inside of, if that is the first such worker, rows
-// y, y + gridDim.y ... of it, a warp per row.  Also clears the rows of q that belong to no request, when asked to.
+// from 8 y on, a warp per row.  Also clears the rows of q that belong to no request, when asked to.  Latency is all: the sums of
+// all pieces are one load (a lane each), the outputs are loaded four at a time.
+constexpr int kJoinWarps = 8;
+
 template <typename T, int HD>
-__global__ void __launch_bounds__(128)
+__global__ void __launch_bounds__(kJoinWarps * 32)
 attn_join_kernel(const AttnArgs a) {
   grid_dependency_begin();
   constexpr int N = HD / 32;
@@ -214,34 +220,40 @@ attn_join_kernel(const AttnArgs a) {
   AttnPiece p;
   p.t = s.tile;
   p.head = s.at.y;
-  const int rows = min(p.t.nrows, max(0, (a.num_tokens - p.t.q_row) * a.group - p.t.row0)), pieces = s.pieces;
-  for (int r = blockIdx.y * 4 + warp; r < rows; r += gridDim.y * 4) {
-    // piece 0 is the last of worker w - 1, piece i > 0 the first of worker w + i - 1 (none, if the next one begins there too)
-    auto slot = [&](int i) { return i == 0 ? 2 * (w - 1) + 1 : 2 * (w + i - 1); };
-    auto lse_of = [&](int i) {
-      if (i > 0 && i + 1 < pieces) {
-        const int4 x = a.plan.starts[w + i - 1].at, y = a.plan.starts[w + i].at;
-        if (x.x == y.x && x.y == y.y && x.z == y.z) return -INFINITY;
-      }
-      return a.part_l[(int64_t)slot(i) * a.slot_rows + r];
-    };
-    float m = -INFINITY;
-    for (int i = lane; i < pieces; i += 32) m = fmaxf(m, lse_of(i));
+  const int rows = min(p.t.nrows, max(0, (a.num_tokens - p.t.q_row) * a.group - p.t.row0));
+  const int* slots = a.plan.slots + 2 * (w - 1);
+  for (int r = blockIdx.y * kJoinWarps + warp; r < rows; r += gridDim.y * kJoinWarps) {
+    float m = -INFINITY, acc[N] = {}, sum = 0.f;
+    for (int i0 = 0; i0 < s.pieces; i0 += 32) {  // (more than 32: the sums so far are brought to the new maximum)
+      const int n = min(32, s.pieces - i0), slot = lane < n ? slots[i0 + lane] : 0;
+      const float mine = lane < n ? a.part_l[(int64_t)slot * a.slot_rows + r] : -INFINITY;
+      float top = mine;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    const float base = m == -INFINITY ? 0.f : m;
-    float acc[N] = {}, sum = 0.f;
-    for (int i0 = 0; i0 < pieces; i0 += 32) {
-      const float mine = i0 + lane < pieces ? exp2f(lse_of(i0 + lane) - base) : 0.f;
-      sum += warp_sum(mine);
-      const int n = min(32, pieces - i0);
-#pragma unroll 4
-      for (int i = 0; i < n; ++i) {
-        const float wt = __shfl_sync(0xffffffffu, mine, i);
-        if (wt == 0.f) continue;  // (a piece that this row sees nothing of)
-        const float* o = a.part_o + ((int64_t)slot(i0 + i) * a.slot_rows + r) * HD + lane * N;
+      for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      const float next = fmaxf(m, top), base = next == -INFINITY ? 0.f : next, keep = m == -INFINITY ? 0.f : exp2f(m - base);
+      m = next;
+      const float wt = exp2f(mine - base);
+      sum = sum * keep + warp_sum(wt);
 #pragma unroll
-        for (int j = 0; j < N; ++j) acc[j] += wt * o[j];
+      for (int j = 0; j < N; ++j) acc[j] *= keep;
+      for (int i = 0; i < n; i += 4) {
+        float o[4][N], f[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          f[k] = __shfl_sync(0xffffffffu, wt, min(i + k, 31));
+          const float* src = a.part_o + ((int64_t)__shfl_sync(0xffffffffu, slot, min(i + k, n - 1)) * a.slot_rows + r) * HD + lane * N;
+#pragma unroll
+          for (int j = 0; j < N; j += 2) {
+            const float2 v = *reinterpret_cast<const float2*>(src + j);
+            o[k][j] = v.x;
+            o[k][j + 1] = v.y;
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (i + k < n && f[k] != 0.f)  // (0: a piece that this row sees nothing of)
+#pragma unroll
+            for (int j = 0; j < N; ++j) acc[j] += f[k] * o[k][j];
       }
     }
     int token, head, pos;
@@ -250,7 +262,8 @@ attn_join_kernel(const AttnArgs a) {
     T* dst = out + token * a.ldo + head * HD + lane * N;
 #pragma unroll
     for (int j = 0; j < N; ++j) dst[j] = DT<T>::from_f(acc[j] * inv);
-    if (a.lse && lane == 0) a.lse[(int64_t)token * (a.kv_heads * a.group) + head] = (base + log2f(sum)) * 0.69314718055994531f;
+    if (a.lse && lane == 0)
+      a.lse[(int64_t)token * (a.kv_heads * a.group) + head] = ((m == -INFINITY ? 0.f : m) + log2f(sum)) * 0.69314718055994531f;
   }
 }
 
@@ -303,6 +316,8 @@ static size_t plan_view(void* base, int64_t cap, AttnPlanView* v) {
   size_t at = 0;
   v->starts = reinterpret_cast<AttnStart*>(p + at);
   at += (kAttnMaxWorkers + 1) * sizeof(AttnStart);
+  v->slots = reinterpret_cast<int*>(p + at);
+  at += 2 * kAttnMaxWorkers * sizeof(int);
   v->cost = reinterpret_cast<long long*>(p + at);
   at += align16((size_t)(cap + 1) * sizeof(long long));
   v->tiles = reinterpret_cast<AttnTile*>(p + at);
@@ -320,9 +335,9 @@ static int slot_rows(const AttnShape& sh) { return sh.rows_many > sh.rows_few ? 
 
 template <typename T>
 static cudaError_t launch_join(int head_dim, const AttnArgs& a, dim3 grid, cudaStream_t s) {
-  if (head_dim == 64) return launch_dependent(attn_join_kernel<T, 64>, grid, dim3(128), 0, s, a);
-  if (head_dim == 128) return launch_dependent(attn_join_kernel<T, 128>, grid, dim3(128), 0, s, a);
-  return launch_dependent(attn_join_kernel<T, 256>, grid, dim3(128), 0, s, a);
+  if (head_dim == 64) return launch_dependent(attn_join_kernel<T, 64>, grid, dim3(kJoinWarps * 32), 0, s, a);
+  if (head_dim == 128) return launch_dependent(attn_join_kernel<T, 128>, grid, dim3(kJoinWarps * 32), 0, s, a);
+  return launch_dependent(attn_join_kernel<T, 256>, grid, dim3(kJoinWarps * 32), 0, s, a);
 }
 
 }  // namespace sb200
@@ -412,8 +427,7 @@ extern "C" int sb200_paged_attention(void* out, int64_t ldo, float* lse, const v
   if (int rc = sh.dtype == SB200_F32 ? run_attn_simt(sh.head_dim, a, workers, s)
                                      : run_attn_tc(sh.dtype, sh.head_dim, a, sh, workers, s))
     return rc;
-  // rows of a slot over four warps each
-  const dim3 grid((unsigned)workers, (unsigned)(a.slot_rows >= 128 ? 8 : a.slot_rows >= 32 ? 2 : 1));
+  const dim3 grid((unsigned)workers, (unsigned)(a.slot_rows >= 128 ? 16 : (a.slot_rows + kJoinWarps - 1) / kJoinWarps));
   SB_DISPATCH_FLOAT(sh.dtype, SB_CUDA(launch_join<scalar_t>(sh.head_dim, a, grid, s)));
   return SB200_OK;
 }

@@ -40,13 +40,14 @@ struct alignas(16) AttnStart {
   int4 at;        // (tile, head, block); (tiles, 0, 0) behind the last
   AttnTile tile;  // of `at`
   int many;       // tiles of many rows (they come before the others)
-  int pieces;     // > 0: this worker is the first that begins inside the unit `at`, which is cut into so many pieces
+  int pieces;     // > 0: this worker is the first that begins inside the unit `at`, which is cut into so many pieces (see slots)
   int rows;       // rows of q that belong to a request
   int pad;
 };
 
 struct AttnPlanView {
   AttnStart* starts; // [workers + 1]
+  int* slots;        // slots[2 (w - 1) + i]: where piece i of the unit that worker w is the first to begin inside of is left
   long long* cost;   // [tiles + 1] start of every tile on the line
   AttnTile* tiles;
   int tiles_cap;
