@@ -193,16 +193,17 @@ attn_plan_kernel(const PlanArgs a) {
 
 // Joins the pieces of cut units: o = sum_p 2^(l_p - m) o_p / sum_p 2^(l_p - m) with l_p the log2 of piece p's sum, in the
 // order of the keys.  CTA (x, y): the unit that the share of worker x + 1 begins inside of, if that is the first such worker, rows
-// from 8 y on, a warp per row.  Also clears the rows of q that belong to no request, when asked to.  Latency is all: the sums of
-// all pieces are one load (a lane each), the outputs are loaded four at a time.
-constexpr int kJoinWarps = 8;
+// from 2 x 16 y on, 16 lanes per row.  Also clears the rows of q that belong to no request, when asked to.  Latency is all:
+// the sums of up to 16 pieces are one load (a lane each), the outputs are loaded four pieces at a time.  Few large CTAs, as most of
+// them have nothing to do and a launch pays 0.6 ns for each (148 x 16 CTAs of 8 rows: 1.5 us a call more).
+constexpr int kJoinWarps = 16, kJoinLanes = 16, kJoinRows = kJoinWarps * 2;
 
 template <typename T, int HD>
 __global__ void __launch_bounds__(kJoinWarps * 32)
 attn_join_kernel(const AttnArgs a) {
   grid_dependency_begin();
-  constexpr int N = HD / 32;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  constexpr int N = HD / kJoinLanes;
+  const int group = threadIdx.x / kJoinLanes, lane = threadIdx.x % kJoinLanes;
   T* out = reinterpret_cast<T*>(a.out);
   const int w = min((int)blockIdx.x + 1, a.workers);
   const AttnStart s = a.plan.starts[w];
@@ -222,46 +223,53 @@ attn_join_kernel(const AttnArgs a) {
   p.head = s.at.y;
   const int rows = min(p.t.nrows, max(0, (a.num_tokens - p.t.q_row) * a.group - p.t.row0));
   const int* slots = a.plan.slots + 2 * (w - 1);
-  for (int r = blockIdx.y * kJoinWarps + warp; r < rows; r += gridDim.y * kJoinWarps) {
+  for (int r0 = blockIdx.y * kJoinRows; r0 < rows; r0 += gridDim.y * kJoinRows) {
+    const int r = min(r0 + group, rows - 1);  // (both halves of a warp stay together; the last row may be made twice)
     float m = -INFINITY, acc[N] = {}, sum = 0.f;
-    for (int i0 = 0; i0 < s.pieces; i0 += 32) {  // (more than 32: the sums so far are brought to the new maximum)
-      const int n = min(32, s.pieces - i0), slot = lane < n ? slots[i0 + lane] : 0;
+    for (int i0 = 0; i0 < s.pieces; i0 += kJoinLanes) {  // (more than 16: the sums so far are brought to the new maximum)
+      const int n = min(kJoinLanes, s.pieces - i0), slot = lane < n ? slots[i0 + lane] : 0;
       const float mine = lane < n ? a.part_l[(int64_t)slot * a.slot_rows + r] : -INFINITY;
       float top = mine;
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      for (int o = kJoinLanes / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
       const float next = fmaxf(m, top), base = next == -INFINITY ? 0.f : next, keep = m == -INFINITY ? 0.f : exp2f(m - base);
       m = next;
       const float wt = exp2f(mine - base);
-      sum = sum * keep + warp_sum(wt);
+      float part = wt;
+#pragma unroll
+      for (int o = kJoinLanes / 2; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
+      sum = sum * keep + part;
 #pragma unroll
       for (int j = 0; j < N; ++j) acc[j] *= keep;
       for (int i = 0; i < n; i += 4) {
-        float o[4][N], f[4];
+        float4 o[4][N / 4];
+        float f[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          f[k] = __shfl_sync(0xffffffffu, wt, min(i + k, 31));
-          const float* src = a.part_o + ((int64_t)__shfl_sync(0xffffffffu, slot, min(i + k, n - 1)) * a.slot_rows + r) * HD + lane * N;
+          f[k] = __shfl_sync(0xffffffffu, wt, min(i + k, kJoinLanes - 1), kJoinLanes);
+          const int sl = __shfl_sync(0xffffffffu, slot, min(i + k, n - 1), kJoinLanes);
+          const float4* src = reinterpret_cast<const float4*>(a.part_o + ((int64_t)sl * a.slot_rows + r) * HD) + lane;
 #pragma unroll
-          for (int j = 0; j < N; j += 2) {
-            const float2 v = *reinterpret_cast<const float2*>(src + j);
-            o[k][j] = v.x;
-            o[k][j + 1] = v.y;
-          }
+          for (int j = 0; j < N / 4; ++j) o[k][j] = src[j * kJoinLanes];
         }
 #pragma unroll
         for (int k = 0; k < 4; ++k)
           if (i + k < n && f[k] != 0.f)  // (0: a piece that this row sees nothing of)
 #pragma unroll
-            for (int j = 0; j < N; ++j) acc[j] += f[k] * o[k][j];
+            for (int j = 0; j < N / 4; ++j) {
+              acc[4 * j] += f[k] * o[k][j].x; acc[4 * j + 1] += f[k] * o[k][j].y;
+              acc[4 * j + 2] += f[k] * o[k][j].z; acc[4 * j + 3] += f[k] * o[k][j].w;
+            }
       }
     }
     int token, head, pos;
     attn_row(a, p, r, &token, &head, &pos);
     const float inv = attn_inverse(sum, pos);
-    T* dst = out + token * a.ldo + head * HD + lane * N;
+    T* dst = out + token * a.ldo + head * HD + lane * 4;
 #pragma unroll
-    for (int j = 0; j < N; ++j) dst[j] = DT<T>::from_f(acc[j] * inv);
+    for (int j = 0; j < N / 4; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) dst[j * 4 * kJoinLanes + e] = DT<T>::from_f(acc[4 * j + e] * inv);
     if (a.lse && lane == 0)
       a.lse[(int64_t)token * (a.kv_heads * a.group) + head] = ((m == -INFINITY ? 0.f : m) + log2f(sum)) * 0.69314718055994531f;
   }
@@ -427,7 +435,7 @@ extern "C" int sb200_paged_attention(void* out, int64_t ldo, float* lse, const v
   if (int rc = sh.dtype == SB200_F32 ? run_attn_simt(sh.head_dim, a, workers, s)
                                      : run_attn_tc(sh.dtype, sh.head_dim, a, sh, workers, s))
     return rc;
-  const dim3 grid((unsigned)workers, (unsigned)(a.slot_rows >= 128 ? 16 : (a.slot_rows + kJoinWarps - 1) / kJoinWarps));
+  const dim3 grid((unsigned)workers, (unsigned)(a.slot_rows >= 128 ? 4 : 1));
   SB_DISPATCH_FLOAT(sh.dtype, SB_CUDA(launch_join<scalar_t>(sh.head_dim, a, grid, s)));
   return SB200_OK;
 }
