@@ -28,6 +28,8 @@ __device__ __forceinline__ void unit_cost(const AttnShape& sh, int kind, int nro
   else { *block = 20; *fixed = 10; *least = 1; }
 }
 
+constexpr long long kShareMany = 20, kShareFew = 15;
+
 __device__ __forceinline__ long long scan_block(long long v, long long* red, long long* total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   long long x = v;
@@ -144,10 +146,13 @@ attn_plan_kernel(const PlanArgs a) {
   __shared__ int4 at[kAttnMaxWorkers + 1];
   if (threadIdx.x == 0) a.plan.cost[tiles] = carry;
   __syncthreads();
+  // No more workers than have a share worth starting for (in tenths of a microsecond, as unit_cost): a piece more is a start, a
+  // store of its part and a load in the join.
+  const long long busy = max(1ll, min((long long)a.workers, carry / (tiles_many && two ? kShareMany : kShareFew)));
   for (int w = threadIdx.x; w <= a.workers; w += kPlanThreads) {
     int4 out = make_int4(tiles, 0, 0, 0);
-    if (w < a.workers && tiles > 0) {
-      const long long x = carry * w / a.workers;
+    if (w < busy && tiles > 0) {
+      const long long x = carry * w / busy;
       int lo = 0, hi = tiles - 1;
       while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
@@ -192,18 +197,20 @@ attn_plan_kernel(const PlanArgs a) {
 }
 
 // Joins the pieces of cut units: o = sum_p 2^(l_p - m) o_p / sum_p 2^(l_p - m) with l_p the log2 of piece p's sum, in the
-// order of the keys.  CTA (x, y): the unit that the share of worker x + 1 begins inside of, if that is the first such worker, rows
-// from 2 x 16 y on, 16 lanes per row.  Also clears the rows of q that belong to no request, when asked to.  Latency is all:
-// the sums of up to 16 pieces are one load (a lane each), the outputs are loaded four pieces at a time.  Few large CTAs, as most of
-// them have nothing to do and a launch pays 0.6 ns for each (148 x 16 CTAs of 8 rows: 1.5 us a call more).
-constexpr int kJoinWarps = 16, kJoinLanes = 16, kJoinRows = kJoinWarps * 2;
+// order of the keys.  CTA (x, y): the unit that the share of worker x + 1 begins inside of, if that is the first such worker; of
+// its rows a warp takes 8, and 16 columns of them.  Also clears the rows of q that belong to no request, when asked to.  Latency is
+// all: where the pieces are, their sums (for all rows of the CTA at once) and their outputs, eight pieces at a time, are three
+// loads after one another.  Few large CTAs, as most of them have nothing to do and a launch pays 0.6 ns for each.
+constexpr int kJoinWarps = 16;
 
 template <typename T, int HD>
 __global__ void __launch_bounds__(kJoinWarps * 32)
 attn_join_kernel(const AttnArgs a) {
   grid_dependency_begin();
-  constexpr int N = HD / kJoinLanes;
-  const int group = threadIdx.x / kJoinLanes, lane = threadIdx.x % kJoinLanes;
+  constexpr int kWide = HD / 16, kRows = kJoinWarps / kWide * 8;  // warps side by side, rows of a CTA
+  constexpr int kBatch = 64;  // pieces whose sums are held at a time
+  __shared__ int slot[kBatch];
+  __shared__ float weight[kBatch * kRows];
   T* out = reinterpret_cast<T*>(a.out);
   const int w = min((int)blockIdx.x + 1, a.workers);
   const AttnStart s = a.plan.starts[w];
@@ -217,61 +224,53 @@ attn_join_kernel(const AttnArgs a) {
           a.lse[(int64_t)t * (a.kv_heads * a.group) + i] = -INFINITY;
     }
   }
-  if (s.pieces == 0) return;
   AttnPiece p;
   p.t = s.tile;
   p.head = s.at.y;
-  const int rows = min(p.t.nrows, max(0, (a.num_tokens - p.t.q_row) * a.group - p.t.row0));
-  const int* slots = a.plan.slots + 2 * (w - 1);
-  for (int r0 = blockIdx.y * kJoinRows; r0 < rows; r0 += gridDim.y * kJoinRows) {
-    const int r = min(r0 + group, rows - 1);  // (both halves of a warp stay together; the last row may be made twice)
-    float m = -INFINITY, acc[N] = {}, sum = 0.f;
-    for (int i0 = 0; i0 < s.pieces; i0 += kJoinLanes) {  // (more than 16: the sums so far are brought to the new maximum)
-      const int n = min(kJoinLanes, s.pieces - i0), slot = lane < n ? slots[i0 + lane] : 0;
-      const float mine = lane < n ? a.part_l[(int64_t)slot * a.slot_rows + r] : -INFINITY;
-      float top = mine;
-#pragma unroll
-      for (int o = kJoinLanes / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-      const float next = fmaxf(m, top), base = next == -INFINITY ? 0.f : next, keep = m == -INFINITY ? 0.f : exp2f(m - base);
-      m = next;
-      const float wt = exp2f(mine - base);
-      float part = wt;
-#pragma unroll
-      for (int o = kJoinLanes / 2; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
-      sum = sum * keep + part;
-#pragma unroll
-      for (int j = 0; j < N; ++j) acc[j] *= keep;
-      for (int i = 0; i < n; i += 4) {
-        float4 o[4][N / 4];
-        float f[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          f[k] = __shfl_sync(0xffffffffu, wt, min(i + k, kJoinLanes - 1), kJoinLanes);
-          const int sl = __shfl_sync(0xffffffffu, slot, min(i + k, n - 1), kJoinLanes);
-          const float4* src = reinterpret_cast<const float4*>(a.part_o + ((int64_t)sl * a.slot_rows + r) * HD) + lane;
-#pragma unroll
-          for (int j = 0; j < N / 4; ++j) o[k][j] = src[j * kJoinLanes];
+  const int rows = min(p.t.nrows, max(0, (a.num_tokens - p.t.q_row) * a.group - p.t.row0)), pieces = s.pieces;
+  if (pieces == 0 || (int)blockIdx.y * kRows >= rows) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int row = warp / kWide * 8 + (lane & 7), col4 = (warp % kWide) * 4 + (lane >> 3);
+  for (int r0 = blockIdx.y * kRows; r0 < rows; r0 += gridDim.y * kRows) {
+    const int r = r0 + row;
+    float m = -INFINITY, base = 0.f, sum = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int i0 = 0; i0 < pieces; i0 += kBatch) {
+      const int n = min(kBatch, pieces - i0);
+      __syncthreads();
+      if ((int)threadIdx.x < n) slot[threadIdx.x] = a.plan.slots[2 * (w - 1) + i0 + threadIdx.x];
+      __syncthreads();
+      for (int i = threadIdx.x; i < n * kRows; i += blockDim.x) {
+        const int x = r0 + i % kRows;
+        weight[i] = x < rows ? a.part_l[(int64_t)slot[i / kRows] * a.slot_rows + x] : -INFINITY;
+      }
+      __syncthreads();
+      if (r >= rows) continue;
+      float top = m;
+      for (int i = 0; i < n; ++i) top = fmaxf(top, weight[i * kRows + row]);
+      base = top == -INFINITY ? 0.f : top;
+      const float keep = m == -INFINITY ? 0.f : exp2f(m - base);  // (a further batch: what there is comes to the new maximum)
+      m = top;
+      sum *= keep;
+      acc.x *= keep; acc.y *= keep; acc.z *= keep; acc.w *= keep;
+#pragma unroll 8
+      for (int i = 0; i < n; ++i) {
+        const float4 o = *attn_part(a, HD, slot[i], p.t.nrows, r, col4);
+        const float wt = exp2f(weight[i * kRows + row] - base);
+        sum += wt;
+        if (wt != 0.f) {  // (0: a piece that this row sees nothing of)
+          acc.x += wt * o.x; acc.y += wt * o.y; acc.z += wt * o.z; acc.w += wt * o.w;
         }
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          if (i + k < n && f[k] != 0.f)  // (0: a piece that this row sees nothing of)
-#pragma unroll
-            for (int j = 0; j < N / 4; ++j) {
-              acc[4 * j] += f[k] * o[k][j].x; acc[4 * j + 1] += f[k] * o[k][j].y;
-              acc[4 * j + 2] += f[k] * o[k][j].z; acc[4 * j + 3] += f[k] * o[k][j].w;
-            }
       }
     }
+    if (r >= rows) continue;
     int token, head, pos;
     attn_row(a, p, r, &token, &head, &pos);
     const float inv = attn_inverse(sum, pos);
-    T* dst = out + token * a.ldo + head * HD + lane * 4;
-#pragma unroll
-    for (int j = 0; j < N / 4; ++j)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) dst[j * 4 * kJoinLanes + e] = DT<T>::from_f(acc[4 * j + e] * inv);
-    if (a.lse && lane == 0)
-      a.lse[(int64_t)token * (a.kv_heads * a.group) + head] = ((m == -INFINITY ? 0.f : m) + log2f(sum)) * 0.69314718055994531f;
+    T* dst = out + token * a.ldo + head * HD + col4 * 4;
+    dst[0] = DT<T>::from_f(acc.x * inv); dst[1] = DT<T>::from_f(acc.y * inv);
+    dst[2] = DT<T>::from_f(acc.z * inv); dst[3] = DT<T>::from_f(acc.w * inv);
+    if (a.lse && col4 == 0) a.lse[(int64_t)token * (a.kv_heads * a.group) + head] = (base + log2f(sum)) * 0.69314718055994531f;
   }
 }
 
@@ -435,7 +434,7 @@ extern "C" int sb200_paged_attention(void* out, int64_t ldo, float* lse, const v
   if (int rc = sh.dtype == SB200_F32 ? run_attn_simt(sh.head_dim, a, workers, s)
                                      : run_attn_tc(sh.dtype, sh.head_dim, a, sh, workers, s))
     return rc;
-  const dim3 grid((unsigned)workers, (unsigned)(a.slot_rows >= 128 ? 4 : 1));
+  const dim3 grid((unsigned)workers, (unsigned)(a.slot_rows >= 128 ? 8 : 1));
   SB_DISPATCH_FLOAT(sh.dtype, SB_CUDA(launch_join<scalar_t>(sh.head_dim, a, grid, s)));
   return SB200_OK;
 }

@@ -80,7 +80,7 @@ struct AttnArgs {
   float* lse;
   const void* cache;
   const int32_t* kv_indices;
-  float* part_o;       // [2 workers][slot_rows][head_dim]
+  float* part_o;       // [2 workers][slot_rows x head_dim], see attn_part
   float* part_l;       // [2 workers][slot_rows]
   uint32_t* status;
   int64_t num_kv_indices;
@@ -97,7 +97,13 @@ struct AttnPiece {
   int head, b0, b1;   // blocks [b0, b1) of the tile's nblk
   int slot;           // -1: the whole unit
   int lo, hi;         // keys [lo, hi) that some row of the tile sees
+  int stride;         // rows of the tile as planned: what a slot is laid out by
 };
+
+// A slot holds [4 columns][row][4] floats: threads with a row each store 16 bytes side by side.
+__device__ __forceinline__ float4* attn_part(const AttnArgs& a, int head_dim, int slot, int stride, int row, int col4) {
+  return reinterpret_cast<float4*>(a.part_o + (int64_t)slot * a.slot_rows * head_dim) + (col4 * stride + row);
+}
 
 // Walks a worker's share of the line.
 struct AttnWalk {
@@ -132,6 +138,7 @@ struct AttnWalk {
   __device__ __forceinline__ bool next(const AttnArgs& a, AttnPiece* p) {
     if (!more()) return false;
     p->t = tile;
+    p->stride = tile.nrows;
     p->head = cur.y;
     p->b0 = cur.z;
     p->b1 = cur.x == end.x && cur.y == end.y ? end.z : p->t.nblk;

@@ -126,10 +126,9 @@ attn_simt_kernel(const AttnArgs a) {
         } else {
           const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
           const int64_t at = (int64_t)p.slot * a.slot_rows + row;
-          float* dst = a.part_o + at * HD + sub * 4;
 #pragma unroll
           for (int i = 0; i < HD / 32; ++i)
-            *reinterpret_cast<float4*>(dst + i * 32) = make_float4(acc[i].x * inv, acc[i].y * inv, acc[i].z * inv, acc[i].w * inv);
+            *attn_part(a, HD, p.slot, p.stride, row, i * 8 + sub) = make_float4(acc[i].x * inv, acc[i].y * inv, acc[i].z * inv, acc[i].w * inv);
           if (sub == 0) a.part_l[at] = l > 0.f || l != l ? base + log2f(l) : -INFINITY;
         }
       }

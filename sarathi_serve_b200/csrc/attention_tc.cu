@@ -396,8 +396,13 @@ __device__ void few_share(const AttnArgs& a, uint8_t* smem, int worker) {
           const bool some = l > 0.f || l != l;
           const float inv = some ? 1.f / l : 0.f;
           const int64_t at = (int64_t)p.slot * a.slot_rows + r;
+          if constexpr (N == 2)
+            reinterpret_cast<float2*>(attn_part(a, HD, p.slot, p.stride, r, lane / 2))[lane & 1] = make_float2(acc[0] * inv, acc[1] * inv);
+          else
 #pragma unroll
-          for (int j = 0; j < N; ++j) a.part_o[at * HD + lane * N + j] = acc[j] * inv;
+            for (int j = 0; j < N; j += 4)
+              *attn_part(a, HD, p.slot, p.stride, r, lane * (N / 4) + j / 4) =
+                  make_float4(acc[j] * inv, acc[j + 1] * inv, acc[j + 2] * inv, acc[j + 3] * inv);
           if (lane == 0) a.part_l[at] = some ? base + log2f(l) : -INFINITY;
         }
       }
@@ -504,14 +509,24 @@ __device__ __forceinline__ void many_queries(const AttnArgs& a, uint8_t* smem, M
   while (walk.next(a, &p)) {
     if (p.b0 >= p.b1 || (sub == 1 && p.t.nrows <= 128)) continue;
     if (!ptx::mbar_wait_warp(&sy.q_empty[sub], (pieces++ & 1u) ^ 1u, abort_flag)) break;
-#pragma unroll 4
-    for (int i = 0; i < 128; i += RPI) {
-      const int rr = i + first, row = sub * 128 + rr;
+    // lane i knows where rows i, i + 32, ... begin (in units of 16 bytes)
+    uint32_t at[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int row = sub * 128 + i * 32 + lane;
       int token, head, pos;
       attn_row(a, p, row, &token, &head, &pos);
-      const bool real = row < p.t.nrows;
-      cp_async16(dst + rr * 128 + ((c ^ (rr & 7)) << 4), real ? q + token * a.ldq + head * HD : q, real);
+      at[i] = row < p.t.nrows ? (uint32_t)((token * a.ldq + head * HD) >> 3) : ~0u;
     }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll 8
+      for (int j = 0; j < 32; j += RPI) {
+        const uint32_t from = __shfl_sync(0xffffffffu, at[i], j + first);
+        const int rr = i * 32 + j + first;
+        const bool real = from != ~0u;
+        cp_async16(dst + rr * 128 + ((c ^ (rr & 7)) << 4), q + (real ? (int64_t)from * 8 : 0), real);
+      }
     cp_async_commit();
     cp_async_wait<0>();
     ptx::fence_proxy_async_smem();
@@ -746,8 +761,8 @@ __device__ __forceinline__ void many_softmax(const AttnArgs& a, uint8_t* smem, M
     const int64_t at = (int64_t)p.slot * a.slot_rows + r;
     const float base2 = m == -INFINITY ? 0.f : m * scale;
     bool fine = true;
-    const long long mine = !real ? -1 : p.slot < 0 ? token * a.ldo + head * HD : at * HD;  // where this thread's row goes
-    long long quad_off[4];                                                                  // and those of its four lanes
+    const long long mine = real ? token * a.ldo + head * HD : -1;  // where this thread's row goes
+    long long quad_off[4];                                         // and those of its four lanes
 #pragma unroll
     for (int j = 0; j < 4; ++j) quad_off[j] = __shfl_sync(0xffffffffu, mine, (lane & ~3) + j);
     const int lane4 = lane & 3;
@@ -781,17 +796,10 @@ __device__ __forceinline__ void many_softmax(const AttnArgs& a, uint8_t* smem, M
           for (int j = 0; j < 4; ++j)
             if (quad_off[j] >= 0) *reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.out) + quad_off[j] + i0 + h * 32 + lane4 * 8) = v[j];
         }
-      } else {
+      } else if (real) {
+        uint4* dst = reinterpret_cast<uint4*>(attn_part(a, HD, p.slot, p.stride, r, i0 / 4));
 #pragma unroll
-        for (int h = 0; h < 4; ++h) {
-          uint4 v[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) v[j] = make_uint4(o[16 * h + 4 * j], o[16 * h + 4 * j + 1], o[16 * h + 4 * j + 2], o[16 * h + 4 * j + 3]);
-          turn_quad(v, lane4);
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (quad_off[j] >= 0) *reinterpret_cast<uint4*>(a.part_o + quad_off[j] + i0 + h * 16 + lane4 * 4) = v[j];
-        }
+        for (int j = 0; j < 16; ++j) dst[j * p.stride] = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
       }
     }
     if (real) {
@@ -812,8 +820,9 @@ __device__ __forceinline__ void many_softmax(const AttnArgs& a, uint8_t* smem, M
       attn_row(a, p, row, &tk, &hd, &ps);
 #pragma unroll
       for (int j = 0; j < N; ++j) {
-        if (p.slot < 0) reinterpret_cast<T*>(a.out)[tk * a.ldo + hd * HD + lane * N + j] = DT<T>::from_f(o[j] * f);
-        else a.part_o[((int64_t)p.slot * a.slot_rows + row) * HD + lane * N + j] = o[j] * f;
+        const int c = lane * N + j;
+        if (p.slot < 0) reinterpret_cast<T*>(a.out)[tk * a.ldo + hd * HD + c] = DT<T>::from_f(o[j] * f);
+        else reinterpret_cast<float*>(attn_part(a, HD, p.slot, p.stride, row, c / 4))[c & 3] = o[j] * f;
       }
     }
     ptx::tc_fence_before();  // O and S may be written again once the next q_full / p_full is seen
