@@ -9,6 +9,7 @@
 namespace sb200 {
 
 constexpr int kPlanThreads = 1024;
+constexpr int kJoinThreads = 256, kJoinValues = 4 * kJoinThreads;
 
 struct PlanArgs {
   AttnPlanView plan;
@@ -174,22 +175,34 @@ attn_plan_kernel(const PlanArgs a) {
     at[w] = out;
   }
   __syncthreads();
-  for (int w = threadIdx.x; w <= a.workers; w += kPlanThreads) {
+  // One thread per worker from here on (workers < threads).
+  const int w = threadIdx.x;
+  auto same = [&](int x, int y) { return at[x].x == at[y].x && at[x].y == at[y].y; };
+  auto empty = [&](int x) { return same(x, x + 1) && at[x].z == at[x + 1].z; };
+  int own = 0;  // pieces of this worker that are not whole units: one that begins inside a unit, one that ends inside one
+  if (w < a.workers && !empty(w)) own = (at[w].z > 0) + (at[w + 1].z > 0 && !(at[w].z > 0 && same(w, w + 1)));
+  const int slot = (int)scan_block(own, red, &total);
+  const bool first_in = w > 0 && w < a.workers && at[w].z > 0 && !(at[w - 1].z > 0 && same(w - 1, w));
+  const AttnTile d = w <= a.workers && at[min(w, a.workers)].x < tiles ? a.plan.tiles[at[min(w, a.workers)].x] : AttnTile{};
+  const long long unit = scan_block(first_in ? 1 : 0, red, &total);
+  const int units = (int)total;
+  const int groups = first_in ? (d.nrows * sh.head_dim + kJoinValues - 1) / kJoinValues : 0;
+  const int group0 = (int)scan_block(groups, red, &total);
+  if (first_in) {  // (the slot before this worker's first holds the piece before it)
+    int pieces = 1;
+    for (int v = w; v < a.workers && same(v, w); ++v) pieces += !empty(v);
+    a.plan.cuts[unit] = AttnCut{d.q_row, d.row0, d.nrows, d.pos0, at[w].y, slot - 1, pieces, 0};
+    a.plan.cut_first[unit] = group0;
+  }
+  if (w == 0) a.plan.cut_first[units] = (int)total;
+  if (w <= a.workers) {
     AttnStart s;
     s.at = at[w];
-    s.tile = s.at.x < tiles ? a.plan.tiles[s.at.x] : AttnTile{};
+    s.tile = d;
     s.many = two ? tiles_many : 0;
+    s.slot = slot;
     s.rows = a.n ? max(0, min(a.qo_indptr[a.n], a.max_tokens)) : 0;
-    s.pieces = s.pad = 0;
-    auto same = [&](int v) { return at[v].x == s.at.x && at[v].y == s.at.y; };
-    if (w > 0 && w < a.workers && s.at.z > 0 && !(same(w - 1) && at[w - 1].z > 0)) {
-      // The last piece of worker w - 1, then the first of every worker that begins inside the unit, unless the next one begins
-      // at the same place.  (Entries of one unit stay below those of the next: it has at most twice as many as workers.)
-      int* slots = a.plan.slots + 2 * (w - 1);
-      slots[s.pieces++] = 2 * (w - 1) + 1;
-      for (int v = w; v < a.workers && same(v); ++v)
-        if (v + 1 == a.workers || !same(v + 1) || at[v + 1].z > at[v].z) slots[s.pieces++] = 2 * v;
-    }
+    s.units = units;
     const int4* src = reinterpret_cast<const int4*>(&s);
     int4* dst = reinterpret_cast<int4*>(a.plan.starts + w);
     for (int i = 0; i < 4; ++i) dst[i] = src[i];
@@ -197,76 +210,72 @@ attn_plan_kernel(const PlanArgs a) {
 }
 
 // Joins the pieces of cut units: o = sum_p 2^(l_p - m) o_p / sum_p 2^(l_p - m) with l_p the log2 of piece p's sum, in the
-// order of the keys.  CTA (x, y): the unit that the share of worker x + 1 begins inside of, if that is the first such worker; of
-// its rows a warp takes 8, and 16 columns of them.  Also clears the rows of q that belong to no request, when asked to.  Latency is
-// all: where the pieces are, their sums (for all rows of the CTA at once) and their outputs, eight pieces at a time, are three
-// loads after one another.  Few large CTAs, as most of them have nothing to do and a launch pays 0.6 ns for each.
-constexpr int kJoinWarps = 16;
-
+// order of the keys.  The cut units' rows are dealt out in groups of 1024 values, four a thread: neighbouring lanes have neighbouring
+// rows, which is how the slots are laid out.  Also clears the rows of q that belong to no request, when asked to.  Bound by
+// latency: the groups' prefix sums, the unit and its pieces (sums and outputs of eight at a time) are three loads after one another.
 template <typename T, int HD>
-__global__ void __launch_bounds__(kJoinWarps * 32)
+__global__ void __launch_bounds__(kJoinThreads)
 attn_join_kernel(const AttnArgs a) {
   grid_dependency_begin();
-  constexpr int kWide = HD / 16, kRows = kJoinWarps / kWide * 8;  // warps side by side, rows of a CTA
-  constexpr int kBatch = 64;  // pieces whose sums are held at a time
-  __shared__ int slot[kBatch];
-  __shared__ float weight[kBatch * kRows];
+  constexpr int kRows = kJoinValues / HD;
+  __shared__ int first[kAttnMaxWorkers + 1];
   T* out = reinterpret_cast<T*>(a.out);
-  const int w = min((int)blockIdx.x + 1, a.workers);
-  const AttnStart s = a.plan.starts[w];
+  const int units = a.plan.starts[0].units;
+  for (int i = threadIdx.x; i <= a.workers; i += kJoinThreads) first[i] = a.plan.cut_first[i];  // (behind `units`: anything)
   if (a.zero_behind) {
-    const int rows0 = min(s.rows, a.num_tokens), per_row = a.kv_heads * a.group * HD;
-    const int ctas = gridDim.x * gridDim.y, cta = blockIdx.y * gridDim.x + blockIdx.x;
-    for (int t = rows0 + cta; t < a.num_tokens; t += ctas) {
-      for (int i = threadIdx.x; i < per_row; i += blockDim.x) out[t * a.ldo + i] = DT<T>::from_f(0.f);
+    const int rows0 = min(a.plan.starts[0].rows, a.num_tokens), per_row = a.kv_heads * a.group * HD;
+    for (int t = rows0 + blockIdx.x; t < a.num_tokens; t += gridDim.x) {
+      for (int i = threadIdx.x; i < per_row; i += kJoinThreads) out[t * a.ldo + i] = DT<T>::from_f(0.f);
       if (a.lse)
-        for (int i = threadIdx.x; i < a.kv_heads * a.group; i += blockDim.x)
+        for (int i = threadIdx.x; i < a.kv_heads * a.group; i += kJoinThreads)
           a.lse[(int64_t)t * (a.kv_heads * a.group) + i] = -INFINITY;
     }
   }
-  AttnPiece p;
-  p.t = s.tile;
-  p.head = s.at.y;
-  const int rows = min(p.t.nrows, max(0, (a.num_tokens - p.t.q_row) * a.group - p.t.row0)), pieces = s.pieces;
-  if (pieces == 0 || (int)blockIdx.y * kRows >= rows) return;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int row = warp / kWide * 8 + (lane & 7), col4 = (warp % kWide) * 4 + (lane >> 3);
-  for (int r0 = blockIdx.y * kRows; r0 < rows; r0 += gridDim.y * kRows) {
-    const int r = r0 + row;
+  __syncthreads();
+  const int groups = first[units];
+  for (int g = blockIdx.x; g < groups; g += gridDim.x) {
+    int lo = 0, hi = units - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (first[mid] <= g) lo = mid;
+      else hi = mid - 1;
+    }
+    const int4* rec = reinterpret_cast<const int4*>(a.plan.cuts + lo);
+    const int4 u = rec[0], v = rec[1];
+    const AttnCut c = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+    const int r = (g - first[lo]) * kRows + threadIdx.x % kRows, col4 = threadIdx.x / kRows;
+    if (r >= min(c.nrows, max(0, (a.num_tokens - c.q_row) * a.group - c.row0))) continue;
     float m = -INFINITY, base = 0.f, sum = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int i0 = 0; i0 < pieces; i0 += kBatch) {
-      const int n = min(kBatch, pieces - i0);
-      __syncthreads();
-      if ((int)threadIdx.x < n) slot[threadIdx.x] = a.plan.slots[2 * (w - 1) + i0 + threadIdx.x];
-      __syncthreads();
-      for (int i = threadIdx.x; i < n * kRows; i += blockDim.x) {
-        const int x = r0 + i % kRows;
-        weight[i] = x < rows ? a.part_l[(int64_t)slot[i / kRows] * a.slot_rows + x] : -INFINITY;
+    for (int i = 0; i < c.pieces; i += 8) {
+      float l[8];
+      float4 o[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int slot = c.slot + min(i + k, c.pieces - 1);
+        l[k] = i + k < c.pieces ? a.part_l[(int64_t)slot * a.slot_rows + r] : -INFINITY;
+        o[k] = *attn_part(a, HD, slot, c.nrows, r, col4);
       }
-      __syncthreads();
-      if (r >= rows) continue;
       float top = m;
-      for (int i = 0; i < n; ++i) top = fmaxf(top, weight[i * kRows + row]);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) top = fmaxf(top, l[k]);
       base = top == -INFINITY ? 0.f : top;
-      const float keep = m == -INFINITY ? 0.f : exp2f(m - base);  // (a further batch: what there is comes to the new maximum)
+      const float keep = m == -INFINITY ? 0.f : exp2f(m - base);  // (more than eight: what there is comes to the new maximum)
       m = top;
       sum *= keep;
       acc.x *= keep; acc.y *= keep; acc.z *= keep; acc.w *= keep;
-#pragma unroll 8
-      for (int i = 0; i < n; ++i) {
-        const float4 o = *attn_part(a, HD, slot[i], p.t.nrows, r, col4);
-        const float wt = exp2f(weight[i * kRows + row] - base);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float wt = exp2f(l[k] - base);
         sum += wt;
         if (wt != 0.f) {  // (0: a piece that this row sees nothing of)
-          acc.x += wt * o.x; acc.y += wt * o.y; acc.z += wt * o.z; acc.w += wt * o.w;
+          acc.x += wt * o[k].x; acc.y += wt * o[k].y; acc.z += wt * o[k].z; acc.w += wt * o[k].w;
         }
       }
     }
-    if (r >= rows) continue;
-    int token, head, pos;
-    attn_row(a, p, r, &token, &head, &pos);
-    const float inv = attn_inverse(sum, pos);
+    const int row = c.row0 + r, tok = a.by_group.div(row);
+    const int token = c.q_row + tok, head = c.head * a.group + (row - tok * a.group);
+    const float inv = attn_inverse(sum, c.pos0 + tok);
     T* dst = out + token * a.ldo + head * HD + col4 * 4;
     dst[0] = DT<T>::from_f(acc.x * inv); dst[1] = DT<T>::from_f(acc.y * inv);
     dst[2] = DT<T>::from_f(acc.z * inv); dst[3] = DT<T>::from_f(acc.w * inv);
@@ -323,8 +332,10 @@ static size_t plan_view(void* base, int64_t cap, AttnPlanView* v) {
   size_t at = 0;
   v->starts = reinterpret_cast<AttnStart*>(p + at);
   at += (kAttnMaxWorkers + 1) * sizeof(AttnStart);
-  v->slots = reinterpret_cast<int*>(p + at);
-  at += 2 * kAttnMaxWorkers * sizeof(int);
+  v->cuts = reinterpret_cast<AttnCut*>(p + at);
+  at += kAttnMaxWorkers * sizeof(AttnCut);
+  v->cut_first = reinterpret_cast<int*>(p + at);
+  at += align16((kAttnMaxWorkers + 1) * sizeof(int));
   v->cost = reinterpret_cast<long long*>(p + at);
   at += align16((size_t)(cap + 1) * sizeof(long long));
   v->tiles = reinterpret_cast<AttnTile*>(p + at);
@@ -342,9 +353,9 @@ static int slot_rows(const AttnShape& sh) { return sh.rows_many > sh.rows_few ? 
 
 template <typename T>
 static cudaError_t launch_join(int head_dim, const AttnArgs& a, dim3 grid, cudaStream_t s) {
-  if (head_dim == 64) return launch_dependent(attn_join_kernel<T, 64>, grid, dim3(kJoinWarps * 32), 0, s, a);
-  if (head_dim == 128) return launch_dependent(attn_join_kernel<T, 128>, grid, dim3(kJoinWarps * 32), 0, s, a);
-  return launch_dependent(attn_join_kernel<T, 256>, grid, dim3(kJoinWarps * 32), 0, s, a);
+  if (head_dim == 64) return launch_dependent(attn_join_kernel<T, 64>, grid, dim3(kJoinThreads), 0, s, a);
+  if (head_dim == 128) return launch_dependent(attn_join_kernel<T, 128>, grid, dim3(kJoinThreads), 0, s, a);
+  return launch_dependent(attn_join_kernel<T, 256>, grid, dim3(kJoinThreads), 0, s, a);
 }
 
 }  // namespace sb200
@@ -434,7 +445,7 @@ extern "C" int sb200_paged_attention(void* out, int64_t ldo, float* lse, const v
   if (int rc = sh.dtype == SB200_F32 ? run_attn_simt(sh.head_dim, a, workers, s)
                                      : run_attn_tc(sh.dtype, sh.head_dim, a, sh, workers, s))
     return rc;
-  const dim3 grid((unsigned)workers, (unsigned)(a.slot_rows >= 128 ? 8 : 1));
+  const dim3 grid((unsigned)(workers * 4));  // as many as are resident
   SB_DISPATCH_FLOAT(sh.dtype, SB_CUDA(launch_join<scalar_t>(sh.head_dim, a, grid, s)));
   return SB200_OK;
 }

@@ -40,14 +40,21 @@ struct alignas(16) AttnStart {
   int4 at;        // (tile, head, block); (tiles, 0, 0) behind the last
   AttnTile tile;  // of `at`
   int many;       // tiles of many rows (they come before the others)
-  int pieces;     // > 0: this worker is the first that begins inside the unit `at`, which is cut into so many pieces (see slots)
+  int slot;       // of its first piece that is not a whole unit; slots of one unit follow one another in the order of the keys
   int rows;       // rows of q that belong to a request
-  int pad;
+  int units;      // cut units
+};
+
+// A unit that is cut, for the join.
+struct alignas(16) AttnCut {
+  int q_row, row0, nrows, pos0;  // as in its tile
+  int head, slot, pieces, pad;   // its pieces are in the slots from `slot` on
 };
 
 struct AttnPlanView {
   AttnStart* starts; // [workers + 1]
-  int* slots;        // slots[2 (w - 1) + i]: where piece i of the unit that worker w is the first to begin inside of is left
+  AttnCut* cuts;     // [workers]
+  int* cut_first;    // [workers + 1] first group of rows of every cut unit (see attn_join_kernel); the last entry: their number
   long long* cost;   // [tiles + 1] start of every tile on the line
   AttnTile* tiles;
   int tiles_cap;
@@ -80,7 +87,7 @@ struct AttnArgs {
   float* lse;
   const void* cache;
   const int32_t* kv_indices;
-  float* part_o;       // [2 workers][slot_rows x head_dim], see attn_part
+  float* part_o;       // [2 workers] slots of [slot_rows x head_dim], see attn_part
   float* part_l;       // [2 workers][slot_rows]
   uint32_t* status;
   int64_t num_kv_indices;
@@ -109,14 +116,15 @@ __device__ __forceinline__ float4* attn_part(const AttnArgs& a, int head_dim, in
 struct AttnWalk {
   int4 cur, end;
   AttnTile tile;  // of cur
-  int worker, many;
-  __device__ __forceinline__ AttnWalk(const AttnArgs& a, int w) : worker(w) {
+  int many, slot;
+  __device__ __forceinline__ AttnWalk(const AttnArgs& a, int w) {
     const int4* s = reinterpret_cast<const int4*>(a.plan.starts + w);
     const int4 x = s[0], u = s[1], v = s[2], e = s[3];
     end = reinterpret_cast<const int4*>(a.plan.starts + w + 1)[0];
     cur = x;
     tile = AttnTile{u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
     many = e.x;
+    slot = e.y;
   }
   __device__ __forceinline__ void fetch(const AttnArgs& a) {
     if (!more()) return;
@@ -128,6 +136,8 @@ struct AttnWalk {
   __device__ __forceinline__ void only_many() { if (end.x >= many) end = make_int4(many, 0, 0, 0); }
   __device__ __forceinline__ void only_few(const AttnArgs& a) {
     if (cur.x < many) {
+      // pieces that are passed over keep their slots: the first, and the last if the share ends among them
+      if (more() && cur.z > 0) ++slot;
       cur = make_int4(many, 0, 0, 0);
       fetch(a);
     }
@@ -143,7 +153,7 @@ struct AttnWalk {
     p->b0 = cur.z;
     p->b1 = cur.x == end.x && cur.y == end.y ? end.z : p->t.nblk;
     const bool head_cut = p->b0 > 0, tail_cut = p->b1 < p->t.nblk;
-    p->slot = head_cut ? 2 * worker : tail_cut ? 2 * worker + 1 : -1;
+    p->slot = head_cut || tail_cut ? slot++ : -1;
     // q may have fewer rows than the plan was made for (tokens x group stays below 2^30)
     p->t.nrows = min(p->t.nrows, max(0, (a.num_tokens - p->t.q_row) * a.group - p->t.row0));
     const int first = a.by_group.div(p->t.row0), last = a.by_group.div(p->t.row0 + max(p->t.nrows, 1) - 1);
