@@ -212,12 +212,12 @@ attn_plan_kernel(const PlanArgs a) {
 // Joins the pieces of cut units: o = sum_p 2^(l_p - m) o_p / sum_p 2^(l_p - m) with l_p the log2 of piece p's sum, in the
 // order of the keys.  The cut units' rows are dealt out in groups of 1024 values, four a thread: neighbouring lanes have neighbouring
 // rows, which is how the slots are laid out.  Also clears the rows of q that belong to no request, when asked to.  Bound by
-// latency: the groups' prefix sums, the unit and its pieces (sums and outputs of eight at a time) are three loads after one another.
+// latency: the groups' prefix sums, the unit and its pieces (sums and outputs of four at a time) are three loads after one another.
 template <typename T, int HD>
-__global__ void __launch_bounds__(kJoinThreads)
+__global__ void __launch_bounds__(kJoinThreads, 5)
 attn_join_kernel(const AttnArgs a) {
   grid_dependency_begin();
-  constexpr int kRows = kJoinValues / HD;
+  constexpr int kRows = kJoinValues / HD, kBatch = 4;
   __shared__ int first[kAttnMaxWorkers + 1];
   T* out = reinterpret_cast<T*>(a.out);
   const int units = a.plan.starts[0].units;
@@ -247,25 +247,25 @@ attn_join_kernel(const AttnArgs a) {
     if (r >= min(c.nrows, max(0, (a.num_tokens - c.q_row) * a.group - c.row0))) continue;
     float m = -INFINITY, base = 0.f, sum = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int i = 0; i < c.pieces; i += 8) {
-      float l[8];
-      float4 o[8];
+    for (int i = 0; i < c.pieces; i += kBatch) {
+      float l[kBatch];
+      float4 o[kBatch];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
+      for (int k = 0; k < kBatch; ++k) {
         const int slot = c.slot + min(i + k, c.pieces - 1);
         l[k] = i + k < c.pieces ? a.part_l[(int64_t)slot * a.slot_rows + r] : -INFINITY;
         o[k] = *attn_part(a, HD, slot, c.nrows, r, col4);
       }
       float top = m;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) top = fmaxf(top, l[k]);
+      for (int k = 0; k < kBatch; ++k) top = fmaxf(top, l[k]);
       base = top == -INFINITY ? 0.f : top;
-      const float keep = m == -INFINITY ? 0.f : exp2f(m - base);  // (more than eight: what there is comes to the new maximum)
+      const float keep = m == -INFINITY ? 0.f : exp2f(m - base);  // (a further batch: what there is comes to the new maximum)
       m = top;
       sum *= keep;
       acc.x *= keep; acc.y *= keep; acc.z *= keep; acc.w *= keep;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
+      for (int k = 0; k < kBatch; ++k) {
         const float wt = exp2f(l[k] - base);
         sum += wt;
         if (wt != 0.f) {  // (0: a piece that this row sees nothing of)
@@ -445,7 +445,7 @@ extern "C" int sb200_paged_attention(void* out, int64_t ldo, float* lse, const v
   if (int rc = sh.dtype == SB200_F32 ? run_attn_simt(sh.head_dim, a, workers, s)
                                      : run_attn_tc(sh.dtype, sh.head_dim, a, sh, workers, s))
     return rc;
-  const dim3 grid((unsigned)(workers * 4));  // as many as are resident
+  const dim3 grid((unsigned)(workers * 5));  // as many as are resident
   SB_DISPATCH_FLOAT(sh.dtype, SB_CUDA(launch_join<scalar_t>(sh.head_dim, a, grid, s)));
   return SB200_OK;
 }
