@@ -24,9 +24,19 @@ struct PlanArgs {
 // count at the share of HBM that an SM has when all of them stream.
 __device__ __forceinline__ void unit_cost(const AttnShape& sh, int kind, int nrows, int* block, int* fixed, int* least) {
   const bool wide = sh.head_dim > 64;
-  if (kind == ATTN_MANY) { *block = nrows > 128 ? (wide ? 17 : 15) : (wide ? 15 : 14); *fixed = 45; *least = 2; }
-  else if (kind == ATTN_FEW) { *block = sh.head_dim == 256 ? 39 : wide ? 15 : 10; *fixed = 22; *least = 2; }
-  else { *block = 20; *fixed = 10; *least = 1; }
+  if (sh.dtype == SB200_F32) {
+    *block = (kind == ATTN_MANY ? 70 : 20) * sh.head_dim / 64;
+    *fixed = 20;
+    *least = 1;
+  } else if (kind == ATTN_MANY) {
+    *block = nrows > 128 ? (wide ? 17 : 15) : (wide ? 15 : 14);
+    *fixed = 45;
+    *least = 2;
+  } else {
+    *block = sh.head_dim == 256 ? 30 : wide ? 15 : 10;
+    *fixed = 22;
+    *least = 2;
+  }
 }
 
 constexpr long long kShareMany = 20, kShareFew = 15;
@@ -62,7 +72,7 @@ __global__ void __launch_bounds__(kPlanThreads)
 attn_plan_kernel(const PlanArgs a) {
   grid_dependency_begin();
   extern __shared__ int smem_i[];
-  int* first = smem_i;               // [n + 1] first tile of every request that has tiles of many rows (or the only kind),
+  int* first = smem_i;               // [n + 1] first tile of every request that has tiles of many rows,
   int* few = smem_i + a.n + 1;       // and of those with few: these come behind all others
   __shared__ long long red[33];
   const AttnShape& sh = a.sh;
@@ -74,16 +84,14 @@ attn_plan_kernel(const PlanArgs a) {
   };
   auto kind_of = [&](int qlen, int* rows) {
     const long long all = (long long)qlen * sh.group;
-    if (sh.few_limit < 0) { *rows = sh.rows_many; return (int)ATTN_SIMT; }
     if (all <= sh.few_limit) { *rows = sh.rows_few; return (int)ATTN_FEW; }
     *rows = sh.rows_many;
     return (int)ATTN_MANY;
   };
-  const bool two = sh.few_limit >= 0 && sh.few_limit < INT32_MAX;
   auto tiles_of = [&](int r, bool want_few) {
     int q0, rows;
     const int q = span(r, &q0);
-    const bool is_few = kind_of(q, &rows) == ATTN_FEW && two;
+    const bool is_few = kind_of(q, &rows) == ATTN_FEW;
     return is_few == want_few ? ((long long)q * sh.group + rows - 1) / rows : 0;
   };
   long long total, many_total = 0;
@@ -149,7 +157,7 @@ attn_plan_kernel(const PlanArgs a) {
   __syncthreads();
   // No more workers than have a share worth starting for (in tenths of a microsecond, as unit_cost): a piece more is a start, a
   // store of its part and a load in the join.
-  const long long busy = max(1ll, min((long long)a.workers, carry / (tiles_many && two ? kShareMany : kShareFew)));
+  const long long busy = max(1ll, min((long long)a.workers, carry / (tiles_many ? kShareMany : kShareFew)));
   for (int w = threadIdx.x; w <= a.workers; w += kPlanThreads) {
     int4 out = make_int4(tiles, 0, 0, 0);
     if (w < busy && tiles > 0) {
@@ -199,7 +207,7 @@ attn_plan_kernel(const PlanArgs a) {
     AttnStart s;
     s.at = at[w];
     s.tile = d;
-    s.many = two ? tiles_many : 0;
+    s.many = tiles_many;
     s.slot = slot;
     s.rows = a.n ? max(0, min(a.qo_indptr[a.n], a.max_tokens)) : 0;
     s.units = units;
@@ -314,15 +322,17 @@ static int attn_shape(const sb200_attention_shape* s, AttnShape* sh, const char*
   // Tiles of 256 rows on tcgen05 fetch keys in boxes of whole swizzle atoms (8 rows); pages that are no multiple of 8, and
   // heads of 256, whose two outputs and scores do not fit TMEM together, stay with tiles of 16 rows.
   const bool many = s->dtype != SB200_F32 && s->head_dim <= 128 && s->page_size % 8 == 0;
-  sh->rows_many = s->dtype == SB200_F32 ? 32 : many ? 256 : 16;
-  sh->rows_few = 16;
-  sh->few_limit = s->dtype == SB200_F32 ? -1 : many ? 16 : INT32_MAX;
+  const bool f32 = s->dtype == SB200_F32;
+  sh->rows_many = f32 ? 32 : many ? 256 : 16;
+  sh->rows_few = f32 ? 4 : 16;
+  sh->few_limit = f32 ? 8 : many ? 16 : INT32_MAX;
   return SB200_OK;
 }
 
 // Tiles of at most `rows` rows: every request may end in a partial one.
 static int64_t tiles_cap(const AttnShape& sh, const sb200_attention_shape* s) {
-  return (int64_t)s->max_tokens * sh.group / sh.rows_many + s->max_requests + 1;
+  const int64_t few = sh.few_limit < INT32_MAX ? (sh.few_limit + sh.rows_few - 1) / sh.rows_few : 1;
+  return (int64_t)s->max_tokens * sh.group / sh.rows_many + few * s->max_requests + 1;
 }
 
 static size_t align16(size_t v) { return (v + 15) & ~size_t(15); }

@@ -22,7 +22,7 @@ constexpr int kAttnBlock = 128;       // keys of a block
 constexpr int kAttnMaxWorkers = 256;  // (B200: 148 SMs)
 
 // How the rows of a tile are computed.
-enum { ATTN_SIMT = 0, ATTN_FEW = 1, ATTN_MANY = 2 };
+enum { ATTN_FEW = 1, ATTN_MANY = 2 };
 
 struct AttnTile {
   int q_row;    // first row of the request's tokens in q
@@ -64,7 +64,7 @@ struct AttnShape {
   int heads, kv_heads, group, head_dim, page_size, dtype, window;
   int rows_many;   // rows of a tile, and up to how many rows a request takes the kernel for few rows
   int rows_few;
-  int few_limit;   // -1: every tile is ATTN_SIMT; INT32_MAX: ATTN_FEW
+  int few_limit;   // INT32_MAX: all
 };
 
 // n / d for 0 <= n < 2^31 as a product: with 2^(s - 1) < d <= 2^s and m = floor(2^(31 + s) / d) + 1, m d exceeds 2^(31 + s) by at
@@ -191,6 +191,12 @@ __device__ __forceinline__ float attn_inverse(float l, int pos) {
   if (l > 0.f || l != l) return 1.f / l;
   return pos < 0 ? 0.f : __int_as_float(0x7fc00000);
 }
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool real) {
+  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 int run_attn_simt(int head_dim, const AttnArgs& a, int workers, cudaStream_t s);
 int run_attn_tc(int dtype, int head_dim, const AttnArgs& a, const AttnShape& sh, int workers, cudaStream_t s);

@@ -1,152 +1,368 @@
 // Attention on the FMA pipes: fp32 throughout (the parity configuration wants more than tf32 products).
 //
-// A CTA of 256 threads holds a tile of 32 query rows and walks the keys of its piece 32 at a time: keys and values through
-// shared memory as fp32, four scores a thread (8 lanes share a row), running maximum and sum per row, and HD / 8 output
-// columns a thread in registers.  Bound by shared memory and FMA alike: in both products a wavefront of 128 bytes feeds
-// 128 multiply-adds.
+// Many rows: a CTA of 256 threads holds a tile of 32 query rows and walks the keys of its piece 32 at a time: keys and values
+// through shared memory, asked for one step ahead, four scores a thread (8 lanes share a row), running maximum and sum per
+// row, and HD / 8 output columns a thread in registers.  Bound by shared memory and FMA alike: in both products a wavefront of
+// 128 bytes feeds 128 multiply-adds.
+//
+// Few rows (a request of up to 8 rows, 4 a unit): bound by HBM.  As in attention_tc.cu the eight warps stream keys in turn, each
+// through a ring of its own that asynchronous copies fill; a key belongs to HD / 8 lanes, which hold 8 columns of queries and
+// outputs of all four rows in registers, so that a warp works on 1 to 4 keys at a time and reads each byte once.
+// (32 decodes of 256 to 2048 tokens and a chunk of 256, heads of 64: 250 us with tiles of 32 rows only.)
 #include "attention.cuh"
 
 namespace sb200 {
 
 constexpr int kSimtRows = 32, kSimtKeys = 32, kSimtThreads = 256;
+constexpr int kFew32Rows = 4, kFew32Warps = kSimtThreads / 32, kFew32Stages = 3;
+
+template <int HD> struct Few32 {
+  static constexpr int KEYS = 1024 / HD;              // of a step: 4 KB of keys, then their values
+  static constexpr int HALF = KEYS * HD * 4;
+  static constexpr int RING = kFew32Warps * kFew32Stages * 2 * HALF;
+  static constexpr int JOIN = kFew32Warps * kFew32Rows * HD * 4;
+  static constexpr int SMEM = RING + JOIN + 2 * kFew32Warps * kFew32Rows * 4;
+};
 
 template <int HD> constexpr size_t simt_smem() {
-  return (size_t)(2 * 32 * (HD + 4) + 32 * HD + 32 * 33) * sizeof(float);
+  constexpr size_t many = (size_t)(2 * 32 * (HD + 4) + 32 * HD + 32 * 33) * sizeof(float);
+  return many > (size_t)Few32<HD>::SMEM ? many : (size_t)Few32<HD>::SMEM;
 }
 
-template <typename T, int HD>
-__global__ void __launch_bounds__(kSimtThreads, 2)
-attn_simt_kernel(const AttnArgs a) {
-  grid_dependency_begin();
-  extern __shared__ float smem_f[];
-  constexpr int LD = HD + 4, N = Vec16<T>::N, VPR = HD / N;
-  float* sq = smem_f;                 // [32][LD]
+// Writes N (2, 4 or 8) neighbouring columns, from `col` on, of row r of a piece: sums o made with the maximum `base`, l their sum.
+template <int HD, int N>
+__device__ __forceinline__ void simt_store(const AttnArgs& a, const AttnPiece& p, int r, int col, const float* o, float base, float l, bool first) {
+  int token, head, pos;
+  attn_row(a, p, r, &token, &head, &pos);
+  const bool some = l > 0.f || l != l;
+  const float inv = p.slot < 0 ? attn_inverse(l, pos) : some ? 1.f / l : 0.f;
+  float* dst = p.slot < 0 ? reinterpret_cast<float*>(a.out) + token * a.ldo + head * HD + col : nullptr;
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    if (p.slot < 0) dst[j] = o[j] * inv;
+    else reinterpret_cast<float*>(attn_part(a, HD, p.slot, p.stride, r, (col + j) >> 2))[(col + j) & 3] = o[j] * inv;
+  }
+  if (first) {
+    if (p.slot >= 0) a.part_l[(int64_t)p.slot * a.slot_rows + r] = some ? base + log2f(l) : -INFINITY;
+    else if (a.lse) a.lse[(int64_t)token * (a.kv_heads * a.group) + head] = (base + log2f(l)) * 0.69314718055994531f;
+  }
+}
+
+template <int HD>
+__device__ void simt_many(const AttnArgs& a, float* smem, AttnWalk walk) {
+  constexpr int LD = HD + 4, VPR = HD / 4, PER = 2 * kSimtKeys * VPR / kSimtThreads;
+  float* sq = smem;                   // [32][LD]
   float* sk = sq + kSimtRows * LD;    // [32][LD]
   float* sv = sk + kSimtKeys * LD;    // [32][HD]
   float* sp = sv + kSimtKeys * HD;    // [32][33]
   const int tid = threadIdx.x, row = tid >> 3, sub = tid & 7;
-  const T* q = reinterpret_cast<const T*>(a.q);
-  const T* cache = reinterpret_cast<const T*>(a.cache);
+  const float* q = reinterpret_cast<const float*>(a.q);
+  const float* cache = reinterpret_cast<const float*>(a.cache);
   const int64_t ldc = (int64_t)a.kv_heads * HD;
-
-  for (int w = blockIdx.x; w < a.workers; w += gridDim.x) {
-    AttnWalk walk(a, w);
-    AttnPiece p;
-    while (walk.next(a, &p)) {
-      __syncthreads();  // the previous piece has been read
-      for (int i = tid; i < kSimtRows * VPR; i += kSimtThreads) {
-        const int r = i / VPR, v = i - r * VPR;
-        int token, head, pos;
-        attn_row(a, p, min(r, max(p.t.nrows - 1, 0)), &token, &head, &pos);
-        Vec16<T> x;
-        if (r < p.t.nrows) x = ld16(q + token * a.ldq + head * HD + v * N);
-#pragma unroll
-        for (int e = 0; e < N; ++e) sq[r * LD + v * N + e] = r < p.t.nrows ? DT<T>::to_f(x.v[e]) : 0.f;
-      }
+  AttnPiece p;
+  while (walk.next(a, &p)) {
+    __syncthreads();  // the previous piece has been read
+    for (int i = tid; i < kSimtRows * VPR; i += kSimtThreads) {
+      const int r = i / VPR, v = i - r * VPR;
       int token, head, pos;
-      attn_row(a, p, min(row, max(p.t.nrows - 1, 0)), &token, &head, &pos);
-      const int seen_lo = a.window > 0 ? pos + 1 - a.window : 0;
-      float m = -INFINITY, l = 0.f;
-      float4 acc[HD / 32];
+      attn_row(a, p, r, &token, &head, &pos);
+      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (r < p.t.nrows) x = *reinterpret_cast<const float4*>(q + token * a.ldq + head * HD + v * 4);
+      *reinterpret_cast<float4*>(sq + r * LD + v * 4) = x;
+    }
+    int token, head, pos;
+    attn_row(a, p, min(row, max(p.t.nrows - 1, 0)), &token, &head, &pos);
+    const int seen_lo = a.window > 0 ? pos + 1 - a.window : 0;
+    float m = -INFINITY, l = 0.f;
+    float4 acc[HD / 32];
 #pragma unroll
-      for (int i = 0; i < HD / 32; ++i) acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-      const int k0 = max(p.lo, (p.t.blk_lo + p.b0) * kAttnBlock) & ~(kSimtKeys - 1), k1 = min(p.hi, (p.t.blk_lo + p.b1) * kAttnBlock);
-      for (int kb = k0; kb < k1; kb += kSimtKeys) {
-        __syncthreads();
-        for (int i = tid; i < 2 * kSimtKeys * VPR; i += kSimtThreads) {
-          const bool val = i >= kSimtKeys * VPR;
-          const int j = val ? i - kSimtKeys * VPR : i, r = j / VPR, v = j - r * VPR, key = kb + r;
-          const int at = key >= p.lo && key < p.hi ? attn_key_row(a, p.t.page_at, key) : -1;
-          Vec16<T> x;
-          x.raw = make_uint4(0, 0, 0, 0);
-          if (at >= 0) x = ld16(cache + (int64_t)(at + (val ? a.page_size : 0)) * ldc + p.head * HD + v * N);
-          float* dst = val ? sv + r * HD + v * N : sk + r * LD + v * N;
+    for (int i = 0; i < HD / 32; ++i) acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    const int k0 = max(p.lo, (p.t.blk_lo + p.b0) * kAttnBlock) & ~(kSimtKeys - 1), k1 = min(p.hi, (p.t.blk_lo + p.b1) * kAttnBlock);
+    float4 ahead[PER];  // this thread's share of the next step's keys (the first half) and values
+    auto ask = [&](int kb) {
 #pragma unroll
-          for (int e = 0; e < N; ++e) dst[e] = DT<T>::to_f(x.v[e]);
-        }
-        __syncthreads();
-        float s[4] = {};
+      for (int i = 0; i < PER; ++i) {
+        const int j = (i % (PER / 2)) * kSimtThreads + tid, r = j / VPR, v = j - r * VPR, key = kb + r;
+        const int at = key >= p.lo && key < p.hi ? attn_key_row(a, p.t.page_at, key) : -1;
+        ahead[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (at >= 0) ahead[i] = *reinterpret_cast<const float4*>(cache + (int64_t)(at + (i < PER / 2 ? 0 : a.page_size)) * ldc + p.head * HD + v * 4);
+      }
+    };
+    if (k0 < k1) ask(k0);
+    for (int kb = k0; kb < k1; kb += kSimtKeys) {
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const int j = (i % (PER / 2)) * kSimtThreads + tid, r = j / VPR, v = j - r * VPR;
+        *reinterpret_cast<float4*>(i < PER / 2 ? sk + r * LD + v * 4 : sv + r * HD + v * 4) = ahead[i];
+      }
+      __syncthreads();
+      if (kb + kSimtKeys < k1) ask(kb + kSimtKeys);
+      float s[4] = {};
 #pragma unroll 4
-        for (int c = 0; c < HD; c += 4) {
-          const float4 x = *reinterpret_cast<const float4*>(sq + row * LD + c);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float4 y = *reinterpret_cast<const float4*>(sk + (sub + 8 * i) * LD + c);
-            s[i] += x.x * y.x + x.y * y.y + x.z * y.z + x.w * y.w;
-          }
-        }
-        float top = -INFINITY;
+      for (int c = 0; c < HD; c += 4) {
+        const float4 x = *reinterpret_cast<const float4*>(sq + row * LD + c);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int key = kb + sub + 8 * i;
-          s[i] = key <= pos && key >= seen_lo ? s[i] * a.scale_log2 : -INFINITY;
-          top = fmaxf(top, s[i]);
+          const float4 y = *reinterpret_cast<const float4*>(sk + (sub + 8 * i) * LD + c);
+          s[i] += x.x * y.x + x.y * y.y + x.z * y.z + x.w * y.w;
         }
+      }
+      float top = -INFINITY;
 #pragma unroll
-        for (int o = 1; o < 8; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        const float now = fmaxf(m, top), base = now == -INFINITY ? 0.f : now, keep = exp2f(m - base);
-        m = now;
-        l *= keep;
+      for (int i = 0; i < 4; ++i) {
+        const int key = kb + sub + 8 * i;
+        s[i] = key <= pos && key >= seen_lo ? s[i] * a.scale_log2 : -INFINITY;
+        top = fmaxf(top, s[i]);
+      }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          s[i] = exp2f(s[i] - base);
-          l += s[i];
-          sp[row * 33 + sub + 8 * i] = s[i];
-        }
+      for (int o = 1; o < 8; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      const float now = fmaxf(m, top), base = now == -INFINITY ? 0.f : now, keep = exp2f(m - base);
+      m = now;
+      l *= keep;
 #pragma unroll
-        for (int i = 0; i < HD / 32; ++i) { acc[i].x *= keep; acc[i].y *= keep; acc[i].z *= keep; acc[i].w *= keep; }
-        __syncwarp();
+      for (int i = 0; i < 4; ++i) {
+        s[i] = exp2f(s[i] - base);
+        l += s[i];
+        sp[row * 33 + sub + 8 * i] = s[i];
+      }
+#pragma unroll
+      for (int i = 0; i < HD / 32; ++i) { acc[i].x *= keep; acc[i].y *= keep; acc[i].z *= keep; acc[i].w *= keep; }
+      __syncwarp();
 #pragma unroll 4
-        for (int k = 0; k < kSimtKeys; ++k) {
-          const float pk = sp[row * 33 + k];
-          if (pk == 0.f) continue;  // a key that the row does not see contributes nothing, whatever its value holds
+      for (int k = 0; k < kSimtKeys; ++k) {
+        const float pk = sp[row * 33 + k];
+        if (pk == 0.f) continue;  // a key that the row does not see contributes nothing, whatever its value holds
 #pragma unroll
-          for (int i = 0; i < HD / 32; ++i) {
-            const float4 v = *reinterpret_cast<const float4*>(sv + k * HD + i * 32 + sub * 4);
-            acc[i].x += pk * v.x; acc[i].y += pk * v.y; acc[i].z += pk * v.z; acc[i].w += pk * v.w;
-          }
-        }
-        __syncwarp();
-      }
-#pragma unroll
-      for (int o = 1; o < 8; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-      if (row < p.t.nrows) {
-        const float base = m == -INFINITY ? 0.f : m;
-        if (p.slot < 0) {
-          const float inv = attn_inverse(l, pos);
-          T* dst = reinterpret_cast<T*>(a.out) + token * a.ldo + head * HD + sub * 4;
-#pragma unroll
-          for (int i = 0; i < HD / 32; ++i) {
-            dst[i * 32] = DT<T>::from_f(acc[i].x * inv);
-            dst[i * 32 + 1] = DT<T>::from_f(acc[i].y * inv);
-            dst[i * 32 + 2] = DT<T>::from_f(acc[i].z * inv);
-            dst[i * 32 + 3] = DT<T>::from_f(acc[i].w * inv);
-          }
-          if (a.lse && sub == 0) a.lse[(int64_t)token * (a.kv_heads * a.group) + head] = (base + log2f(l)) * 0.69314718055994531f;
-        } else {
-          const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
-          const int64_t at = (int64_t)p.slot * a.slot_rows + row;
-#pragma unroll
-          for (int i = 0; i < HD / 32; ++i)
-            *attn_part(a, HD, p.slot, p.stride, row, i * 8 + sub) = make_float4(acc[i].x * inv, acc[i].y * inv, acc[i].z * inv, acc[i].w * inv);
-          if (sub == 0) a.part_l[at] = l > 0.f || l != l ? base + log2f(l) : -INFINITY;
+        for (int i = 0; i < HD / 32; ++i) {
+          const float4 v = *reinterpret_cast<const float4*>(sv + k * HD + i * 32 + sub * 4);
+          acc[i].x += pk * v.x; acc[i].y += pk * v.y; acc[i].z += pk * v.z; acc[i].w += pk * v.w;
         }
       }
+      __syncwarp();
+    }
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+    if (row < p.t.nrows) {
+#pragma unroll
+      for (int i = 0; i < HD / 32; ++i)
+        simt_store<HD, 4>(a, p, row, i * 32 + sub * 4, reinterpret_cast<const float*>(&acc[i]), m == -INFINITY ? 0.f : m, l, i == 0 && sub == 0);
     }
   }
 }
 
-template <typename T, int HD>
+// The steps of a warp, for the loads and for the sums alike.
+template <int HD> struct Few32Steps {
+  AttnWalk walk;
+  AttnPiece p;
+  int key, end;
+  __device__ __forceinline__ explicit Few32Steps(const AttnWalk& w) : walk(w), key(0), end(0) {}
+  __device__ __forceinline__ bool next_piece(const AttnArgs& a, int warp) {
+    if (!walk.next(a, &p)) return false;
+    constexpr int K = Few32<HD>::KEYS;
+    key = (max(p.lo, (p.t.blk_lo + p.b0) * kAttnBlock) & ~(K - 1)) + warp * K;
+    end = min(p.hi, (p.t.blk_lo + p.b1) * kAttnBlock);
+    return true;
+  }
+};
+
+template <int HD>
+__device__ void simt_few(const AttnArgs& a, float* smem, const AttnWalk& walk) {
+  using F = Few32<HD>;
+  constexpr int R = kFew32Rows, LPK = HD / 8, KPW = 32 / LPK, CPR = HD / 4, kStep = kFew32Warps * F::KEYS;
+  static_assert(F::KEYS == 4 * KPW, "a step is four turns of the warp");
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane % LPK, mine = lane / LPK;
+  uint8_t* bytes = reinterpret_cast<uint8_t*>(smem);
+  float* ring = reinterpret_cast<float*>(bytes + warp * (kFew32Stages * 2 * F::HALF));
+  float* join = reinterpret_cast<float*>(bytes + F::RING);                // [warp][row][HD]
+  float* stat_m = reinterpret_cast<float*>(bytes + F::RING + F::JOIN);    // [warp][row]
+  float* stat_l = stat_m + kFew32Warps * R;
+  const float* cache = reinterpret_cast<const float*>(a.cache);
+  const int64_t ldc = (int64_t)a.kv_heads * HD;
+
+  Few32Steps<HD> ld(walk);
+  bool more = true;
+  int row_next = -1, head_next = 0, put = 0;
+  auto look_up = [&]() {  // lane i: the row of key i of the step after the next
+    while (more && ld.key >= ld.end) more = ld.next_piece(a, warp);
+    if (!more) return;
+    const int key = ld.key + lane % F::KEYS;
+    row_next = key >= ld.p.lo && key < ld.p.hi ? attn_key_row(a, ld.p.t.page_at, key) : -1;
+    head_next = ld.p.head;
+    ld.key += kStep;
+  };
+  auto load = [&]() {
+    if (more) {
+      const int rows = row_next, head = head_next;
+      const uint32_t dst = ptx::smem_u32(ring) + put * (2 * F::HALF);
+#pragma unroll
+      for (int i = 0; i < F::KEYS * CPR / 32; ++i) {
+        const int c = i * 32 + lane, k = c / CPR, row = __shfl_sync(0xffffffffu, rows, k);
+        const float* src = cache + (int64_t)max(row, 0) * ldc + head * HD + (c % CPR) * 4;
+        cp_async16(dst + c * 16, src, row >= 0);
+        cp_async16(dst + F::HALF + c * 16, src + (row >= 0 ? a.page_size * ldc : 0), row >= 0);
+      }
+      if (++put == kFew32Stages) put = 0;
+      look_up();
+    }
+    cp_async_commit();
+  };
+  look_up();
+#pragma unroll 1
+  for (int i = 0; i < kFew32Stages - 1; ++i) load();
+
+  Few32Steps<HD> st(walk);
+  int get = 0;
+  while (st.next_piece(a, warp)) {
+    const AttnPiece& p = st.p;
+    float4 q[R][2], o[R][2];
+    float m[R], l[R];
+    int pos[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      int token, head;
+      attn_row(a, p, min(r, max(p.t.nrows - 1, 0)), &token, &head, &pos[r]);
+      const float* src = reinterpret_cast<const float*>(a.q) + token * a.ldq + head * HD + sub * 4;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        q[r][h] = o[r][h] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (r < p.t.nrows) q[r][h] = *reinterpret_cast<const float4*>(src + h * (HD / 2));
+      }
+      m[r] = -INFINITY;
+      l[r] = 0.f;
+    }
+    const int pos_first = p.t.pos0 + a.by_group.div(p.t.row0), pos_last = p.hi - 1;
+    for (; st.key < st.end; st.key += kStep) {
+      load();
+      cp_async_wait<kFew32Stages - 1>();
+      __syncwarp();
+      const float* sk = ring + get * (2 * F::HALF / 4) + mine * HD + sub * 4;
+      const float* sv = sk + F::HALF / 4;
+      if (++get == kFew32Stages) get = 0;
+      const bool all = st.key + F::KEYS - 1 <= pos_first && (a.window == 0 || st.key > pos_last - a.window);
+      float s[4][R];
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const float4 x = *reinterpret_cast<const float4*>(sk + t * KPW * HD), y = *reinterpret_cast<const float4*>(sk + t * KPW * HD + HD / 2);
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          float d = q[r][0].x * x.x + q[r][0].y * x.y + q[r][0].z * x.z + q[r][0].w * x.w;
+          d += q[r][1].x * y.x + q[r][1].y * y.y + q[r][1].z * y.z + q[r][1].w * y.w;
+          s[t][r] = d;
+        }
+      }
+#pragma unroll
+      for (int x = 1; x < LPK; x <<= 1)
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+          for (int r = 0; r < R; ++r) s[t][r] += __shfl_xor_sync(0xffffffffu, s[t][r], x);
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        float top = m[r];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          s[t][r] *= a.scale_log2;
+          const int key = st.key + t * KPW + mine;
+          if (!all && (key > pos[r] || (a.window > 0 && key <= pos[r] - a.window))) s[t][r] = -INFINITY;
+          top = fmaxf(top, s[t][r]);
+        }
+        const float base = top == -INFINITY ? 0.f : top, keep = exp2f(m[r] - base);
+        m[r] = top;
+        l[r] *= keep;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) { o[r][h].x *= keep; o[r][h].y *= keep; o[r][h].z *= keep; o[r][h].w *= keep; }
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          s[t][r] = exp2f(s[t][r] - base);
+          l[r] += s[t][r];
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const float4 x = *reinterpret_cast<const float4*>(sv + t * KPW * HD), y = *reinterpret_cast<const float4*>(sv + t * KPW * HD + HD / 2);
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          const float w = s[t][r];
+          if (all || w != 0.f) {  // a key that the row does not see contributes nothing, whatever its value holds
+            o[r][0].x += w * x.x; o[r][0].y += w * x.y; o[r][0].z += w * x.z; o[r][0].w += w * x.w;
+            o[r][1].x += w * y.x; o[r][1].y += w * y.y; o[r][1].z += w * y.z; o[r][1].w += w * y.w;
+          }
+        }
+      }
+      __syncwarp();  // the stage may be filled again
+    }
+    // ---- join: the lanes of a warp that have the same columns, then the warps
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      float top = m[r];
+#pragma unroll
+      for (int x = LPK; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+      const float keep = m[r] == -INFINITY ? 0.f : exp2f(m[r] - top);
+      m[r] = top;
+      l[r] *= keep;
+      float* v[8] = {&o[r][0].x, &o[r][0].y, &o[r][0].z, &o[r][0].w, &o[r][1].x, &o[r][1].y, &o[r][1].z, &o[r][1].w};
+#pragma unroll
+      for (int e = 0; e < 8; ++e) *v[e] *= keep;
+#pragma unroll
+      for (int x = LPK; x < 32; x <<= 1) {
+        l[r] += __shfl_xor_sync(0xffffffffu, l[r], x);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) *v[e] += __shfl_xor_sync(0xffffffffu, *v[e], x);
+      }
+      if (mine == 0) {
+        *reinterpret_cast<float4*>(join + (warp * R + r) * HD + sub * 4) = o[r][0];
+        *reinterpret_cast<float4*>(join + (warp * R + r) * HD + HD / 2 + sub * 4) = o[r][1];
+      }
+      if (lane == 0) { stat_m[warp * R + r] = m[r]; stat_l[warp * R + r] = l[r]; }
+    }
+    __syncthreads();
+    if (warp < p.t.nrows) {
+      constexpr int N = HD / 32;
+      float top = -INFINITY, sum = 0.f, acc[N] = {};
+#pragma unroll
+      for (int w = 0; w < kFew32Warps; ++w) top = fmaxf(top, stat_m[w * R + warp]);
+      const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+      for (int w = 0; w < kFew32Warps; ++w) {
+        const float mw = stat_m[w * R + warp];
+        if (mw == -INFINITY) { sum += stat_l[w * R + warp]; continue; }
+        const float f = exp2f(mw - base);
+        sum += f * stat_l[w * R + warp];
+#pragma unroll
+        for (int j = 0; j < N; ++j) acc[j] += f * join[(w * R + warp) * HD + lane * N + j];
+      }
+      simt_store<HD, N>(a, p, warp, lane * N, acc, base, sum, lane == 0);
+    }
+    __syncthreads();
+  }
+  cp_async_wait<0>();
+}
+
+// One CTA per SM: its share's tiles of many rows first, then those of few.
+template <int HD>
+__global__ void __launch_bounds__(kSimtThreads, 1)
+attn_simt_kernel(const __grid_constant__ AttnArgs a) {
+  grid_dependency_begin();
+  extern __shared__ float smem_f[];
+  if ((int)blockIdx.x >= a.workers) return;
+  AttnWalk walk(a, blockIdx.x), few = walk;
+  walk.only_many();
+  simt_many<HD>(a, smem_f, walk);
+  __syncthreads();
+  few.only_few(a);
+  simt_few<HD>(a, smem_f, few);
+}
+
+template <int HD>
 static int launch_simt(const AttnArgs& a, int workers, cudaStream_t s) {
-  SB_CUDA(cudaFuncSetAttribute(attn_simt_kernel<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)simt_smem<HD>()));
-  SB_CUDA(launch_dependent(attn_simt_kernel<T, HD>, dim3((unsigned)workers), dim3(kSimtThreads), simt_smem<HD>(), s, a));
+  SB_CUDA(cudaFuncSetAttribute(attn_simt_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)simt_smem<HD>()));
+  SB_CUDA(launch_dependent(attn_simt_kernel<HD>, dim3((unsigned)workers), dim3(kSimtThreads), simt_smem<HD>(), s, a));
   return SB200_OK;
 }
 
 int run_attn_simt(int head_dim, const AttnArgs& a, int workers, cudaStream_t s) {
-  return head_dim == 64    ? launch_simt<float, 64>(a, workers, s)
-         : head_dim == 128 ? launch_simt<float, 128>(a, workers, s)
-                           : launch_simt<float, 256>(a, workers, s);
+  return head_dim == 64 ? launch_simt<64>(a, workers, s) : head_dim == 128 ? launch_simt<128>(a, workers, s) : launch_simt<256>(a, workers, s);
 }
 
 }  // namespace sb200

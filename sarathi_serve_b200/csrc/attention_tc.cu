@@ -28,12 +28,6 @@ template <int HD> struct Few {
 };
 
 // ------------------------------------------------------------------ warp-wide pieces
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool real) {
-  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-
 // `ex2.approx`: relative error 2^-22, 2^-inf = 0.
 __device__ __forceinline__ float pow2(float x) {
   float y;
