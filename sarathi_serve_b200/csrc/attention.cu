@@ -25,7 +25,7 @@ struct PlanArgs {
 __device__ __forceinline__ void unit_cost(const AttnShape& sh, int kind, int nrows, int* block, int* fixed, int* least) {
   const bool wide = sh.head_dim > 64;
   if (sh.dtype == SB200_F32) {
-    *block = (kind == ATTN_MANY ? 70 : 20) * sh.head_dim / 64;
+    *block = (kind == ATTN_MANY ? 130 : 15) * sh.head_dim / 64;
     *fixed = 20;
     *least = 1;
   } else if (kind == ATTN_MANY) {
@@ -323,7 +323,7 @@ static int attn_shape(const sb200_attention_shape* s, AttnShape* sh, const char*
   // heads of 256, whose two outputs and scores do not fit TMEM together, stay with tiles of 16 rows.
   const bool many = s->dtype != SB200_F32 && s->head_dim <= 128 && s->page_size % 8 == 0;
   const bool f32 = s->dtype == SB200_F32;
-  sh->rows_many = f32 ? 32 : many ? 256 : 16;
+  sh->rows_many = f32 ? 64 : many ? 256 : 16;
   sh->rows_few = f32 ? 4 : 16;
   sh->few_limit = f32 ? 8 : many ? 16 : INT32_MAX;
   return SB200_OK;

@@ -1,9 +1,9 @@
 // Attention on the FMA pipes: fp32 throughout (the parity configuration wants more than tf32 products).
 //
-// Many rows: a CTA of 256 threads holds a tile of 32 query rows and walks the keys of its piece 32 at a time: keys and values
-// through shared memory, asked for one step ahead, four scores a thread (8 lanes share a row), running maximum and sum per
-// row, and HD / 8 output columns a thread in registers.  Bound by shared memory and FMA alike: in both products a wavefront of
-// 128 bytes feeds 128 multiply-adds.
+// Many rows: a CTA of 256 threads holds a tile of 64 query rows and walks the keys of its piece 64 (heads of 256: 32) at a time:
+// keys and values through shared memory, asked for one step ahead; a thread has 4 rows x 4 keys of the scores and 4 rows x
+// HD / 16 columns of the output, so that a load of 16 bytes from shared memory feeds 8 multiply-adds or more (with 1 x 4
+// the kernel was bound by those loads: 19 us for 128 keys x 32 rows with heads of 64).
 //
 // Few rows (a request of up to 8 rows, 4 a unit): bound by HBM.  As in attention_tc.cu the eight warps stream keys in turn, each
 // through a ring of its own that asynchronous copies fill; a key belongs to HD / 8 lanes, which hold 8 columns of queries and
@@ -13,7 +13,7 @@
 
 namespace sb200 {
 
-constexpr int kSimtRows = 32, kSimtKeys = 32, kSimtThreads = 256;
+constexpr int kSimtRows = 64, kSimtThreads = 256;
 constexpr int kFew32Rows = 4, kFew32Warps = kSimtThreads / 32, kFew32Stages = 3;
 
 template <int HD> struct Few32 {
@@ -24,9 +24,14 @@ template <int HD> struct Few32 {
   static constexpr int SMEM = RING + JOIN + 2 * kFew32Warps * kFew32Rows * 4;
 };
 
+template <int HD> struct Many32 {
+  static constexpr int KEYS = HD == 256 ? 32 : 64;
+  static constexpr int LD = HD + 4, LDP = kSimtRows + 4;
+  static constexpr int SMEM = (kSimtRows * LD + KEYS * LD + KEYS * HD + KEYS * LDP) * 4;
+};
+
 template <int HD> constexpr size_t simt_smem() {
-  constexpr size_t many = (size_t)(2 * 32 * (HD + 4) + 32 * HD + 32 * 33) * sizeof(float);
-  return many > (size_t)Few32<HD>::SMEM ? many : (size_t)Few32<HD>::SMEM;
+  return Many32<HD>::SMEM > Few32<HD>::SMEM ? Many32<HD>::SMEM : Few32<HD>::SMEM;
 }
 
 // Writes N (2, 4 or 8) neighbouring columns, from `col` on, of row r of a piece: sums o made with the maximum `base`, l their sum.
@@ -50,12 +55,13 @@ __device__ __forceinline__ void simt_store(const AttnArgs& a, const AttnPiece& p
 
 template <int HD>
 __device__ void simt_many(const AttnArgs& a, float* smem, AttnWalk walk) {
-  constexpr int LD = HD + 4, VPR = HD / 4, PER = 2 * kSimtKeys * VPR / kSimtThreads;
-  float* sq = smem;                   // [32][LD]
-  float* sk = sq + kSimtRows * LD;    // [32][LD]
-  float* sv = sk + kSimtKeys * LD;    // [32][HD]
-  float* sp = sv + kSimtKeys * HD;    // [32][33]
-  const int tid = threadIdx.x, row = tid >> 3, sub = tid & 7;
+  using M = Many32<HD>;
+  constexpr int VPR = HD / 4, PER = M::KEYS * VPR / kSimtThreads, KT = M::KEYS / 16, CT = HD / 64;
+  float* sq = smem;                        // [64][LD]
+  float* sk = sq + kSimtRows * M::LD;      // [KEYS][LD]
+  float* sv = sk + M::KEYS * M::LD;        // [KEYS][HD]
+  float* sp = sv + M::KEYS * HD;           // [KEYS][LDP]: probabilities, rows side by side
+  const int tid = threadIdx.x, rg = tid >> 4, cg = tid & 15;  // rows 4 rg .. + 3; keys cg + 16 i, columns 4 cg + 64 i
   const float* q = reinterpret_cast<const float*>(a.q);
   const float* cache = reinterpret_cast<const float*>(a.cache);
   const int64_t ldc = (int64_t)a.kv_heads * HD;
@@ -68,85 +74,127 @@ __device__ void simt_many(const AttnArgs& a, float* smem, AttnWalk walk) {
       attn_row(a, p, r, &token, &head, &pos);
       float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
       if (r < p.t.nrows) x = *reinterpret_cast<const float4*>(q + token * a.ldq + head * HD + v * 4);
-      *reinterpret_cast<float4*>(sq + r * LD + v * 4) = x;
+      *reinterpret_cast<float4*>(sq + r * M::LD + v * 4) = x;
     }
-    int token, head, pos;
-    attn_row(a, p, min(row, max(p.t.nrows - 1, 0)), &token, &head, &pos);
-    const int seen_lo = a.window > 0 ? pos + 1 - a.window : 0;
-    float m = -INFINITY, l = 0.f;
-    float4 acc[HD / 32];
+    float m[4], l[4];
+    int pos[4];
+    float4 acc[4][CT];
 #pragma unroll
-    for (int i = 0; i < HD / 32; ++i) acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-    const int k0 = max(p.lo, (p.t.blk_lo + p.b0) * kAttnBlock) & ~(kSimtKeys - 1), k1 = min(p.hi, (p.t.blk_lo + p.b1) * kAttnBlock);
-    float4 ahead[PER];  // this thread's share of the next step's keys (the first half) and values
+    for (int j = 0; j < 4; ++j) {
+      int token, head;
+      attn_row(a, p, min(rg * 4 + j, max(p.t.nrows - 1, 0)), &token, &head, &pos[j]);
+      m[j] = -INFINITY;
+      l[j] = 0.f;
+#pragma unroll
+      for (int i = 0; i < CT; ++i) acc[j][i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    const int pos_first = p.t.pos0 + a.by_group.div(p.t.row0), pos_last = p.hi - 1;
+    const int k0 = max(p.lo, (p.t.blk_lo + p.b0) * kAttnBlock) & ~(M::KEYS - 1), k1 = min(p.hi, (p.t.blk_lo + p.b1) * kAttnBlock);
+    float4 next_k[PER], next_v[PER];  // this thread's share of the next step
     auto ask = [&](int kb) {
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
-        const int j = (i % (PER / 2)) * kSimtThreads + tid, r = j / VPR, v = j - r * VPR, key = kb + r;
+        const int j = i * kSimtThreads + tid, r = j / VPR, v = j - r * VPR, key = kb + r;
         const int at = key >= p.lo && key < p.hi ? attn_key_row(a, p.t.page_at, key) : -1;
-        ahead[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (at >= 0) ahead[i] = *reinterpret_cast<const float4*>(cache + (int64_t)(at + (i < PER / 2 ? 0 : a.page_size)) * ldc + p.head * HD + v * 4);
+        next_k[i] = next_v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (at >= 0) {
+          const float* src = cache + (int64_t)at * ldc + p.head * HD + v * 4;
+          next_k[i] = *reinterpret_cast<const float4*>(src);
+          next_v[i] = *reinterpret_cast<const float4*>(src + a.page_size * ldc);
+        }
       }
     };
     if (k0 < k1) ask(k0);
-    for (int kb = k0; kb < k1; kb += kSimtKeys) {
+    for (int kb = k0; kb < k1; kb += M::KEYS) {
       __syncthreads();
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
-        const int j = (i % (PER / 2)) * kSimtThreads + tid, r = j / VPR, v = j - r * VPR;
-        *reinterpret_cast<float4*>(i < PER / 2 ? sk + r * LD + v * 4 : sv + r * HD + v * 4) = ahead[i];
+        const int j = i * kSimtThreads + tid, r = j / VPR, v = j - r * VPR;
+        *reinterpret_cast<float4*>(sk + r * M::LD + v * 4) = next_k[i];
+        *reinterpret_cast<float4*>(sv + r * HD + v * 4) = next_v[i];
       }
       __syncthreads();
-      if (kb + kSimtKeys < k1) ask(kb + kSimtKeys);
-      float s[4] = {};
-#pragma unroll 4
+      if (kb + M::KEYS < k1) ask(kb + M::KEYS);
+      float s[4][KT] = {};
+#pragma unroll 2
       for (int c = 0; c < HD; c += 4) {
-        const float4 x = *reinterpret_cast<const float4*>(sq + row * LD + c);
+        float4 x[4], y[KT];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float4 y = *reinterpret_cast<const float4*>(sk + (sub + 8 * i) * LD + c);
-          s[i] += x.x * y.x + x.y * y.y + x.z * y.z + x.w * y.w;
+        for (int j = 0; j < 4; ++j) x[j] = *reinterpret_cast<const float4*>(sq + (rg * 4 + j) * M::LD + c);
+#pragma unroll
+        for (int i = 0; i < KT; ++i) y[i] = *reinterpret_cast<const float4*>(sk + (cg + 16 * i) * M::LD + c);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int i = 0; i < KT; ++i) s[j][i] += x[j].x * y[i].x + x[j].y * y[i].y + x[j].z * y[i].z + x[j].w * y[i].w;
+      }
+      const bool all = kb + M::KEYS - 1 <= pos_first && (a.window == 0 || kb > pos_last - a.window);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float top = m[j];
+#pragma unroll
+        for (int i = 0; i < KT; ++i) {
+          const int key = kb + cg + 16 * i;
+          s[j][i] *= a.scale_log2;
+          if (!all && (key > pos[j] || (a.window > 0 && key <= pos[j] - a.window))) s[j][i] = -INFINITY;
+          top = fmaxf(top, s[j][i]);
         }
-      }
-      float top = -INFINITY;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int key = kb + sub + 8 * i;
-        s[i] = key <= pos && key >= seen_lo ? s[i] * a.scale_log2 : -INFINITY;
-        top = fmaxf(top, s[i]);
-      }
+        for (int o = 1; o < 16; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const float base = top == -INFINITY ? 0.f : top, keep = exp2f(m[j] - base);
+        m[j] = top;
+        l[j] *= keep;
 #pragma unroll
-      for (int o = 1; o < 8; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-      const float now = fmaxf(m, top), base = now == -INFINITY ? 0.f : now, keep = exp2f(m - base);
-      m = now;
-      l *= keep;
+        for (int i = 0; i < KT; ++i) {
+          s[j][i] = exp2f(s[j][i] - base);
+          l[j] += s[j][i];
+        }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        s[i] = exp2f(s[i] - base);
-        l += s[i];
-        sp[row * 33 + sub + 8 * i] = s[i];
+        for (int i = 0; i < CT; ++i) { acc[j][i].x *= keep; acc[j][i].y *= keep; acc[j][i].z *= keep; acc[j][i].w *= keep; }
       }
 #pragma unroll
-      for (int i = 0; i < HD / 32; ++i) { acc[i].x *= keep; acc[i].y *= keep; acc[i].z *= keep; acc[i].w *= keep; }
-      __syncwarp();
+      for (int i = 0; i < KT; ++i)
+        *reinterpret_cast<float4*>(sp + (cg + 16 * i) * M::LDP + rg * 4) = make_float4(s[0][i], s[1][i], s[2][i], s[3][i]);
+      __syncwarp();  // the rows of a warp are its own
+      if (all) {
 #pragma unroll 4
-      for (int k = 0; k < kSimtKeys; ++k) {
-        const float pk = sp[row * 33 + k];
-        if (pk == 0.f) continue;  // a key that the row does not see contributes nothing, whatever its value holds
+        for (int k = 0; k < M::KEYS; ++k) {
+          const float4 w = *reinterpret_cast<const float4*>(sp + k * M::LDP + rg * 4);
 #pragma unroll
-        for (int i = 0; i < HD / 32; ++i) {
-          const float4 v = *reinterpret_cast<const float4*>(sv + k * HD + i * 32 + sub * 4);
-          acc[i].x += pk * v.x; acc[i].y += pk * v.y; acc[i].z += pk * v.z; acc[i].w += pk * v.w;
+          for (int i = 0; i < CT; ++i) {
+            const float4 v = *reinterpret_cast<const float4*>(sv + k * HD + cg * 4 + 64 * i);
+            acc[0][i].x += w.x * v.x; acc[0][i].y += w.x * v.y; acc[0][i].z += w.x * v.z; acc[0][i].w += w.x * v.w;
+            acc[1][i].x += w.y * v.x; acc[1][i].y += w.y * v.y; acc[1][i].z += w.y * v.z; acc[1][i].w += w.y * v.w;
+            acc[2][i].x += w.z * v.x; acc[2][i].y += w.z * v.y; acc[2][i].z += w.z * v.z; acc[2][i].w += w.z * v.w;
+            acc[3][i].x += w.w * v.x; acc[3][i].y += w.w * v.y; acc[3][i].z += w.w * v.z; acc[3][i].w += w.w * v.w;
+          }
+        }
+      } else {  // a key that a row does not see contributes nothing to it, whatever its value holds
+#pragma unroll 1
+        for (int k = 0; k < M::KEYS; ++k) {
+          const float* w = sp + k * M::LDP + rg * 4;
+#pragma unroll
+          for (int i = 0; i < CT; ++i) {
+            const float4 v = *reinterpret_cast<const float4*>(sv + k * HD + cg * 4 + 64 * i);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const float x = w[j];
+              if (x != 0.f) { acc[j][i].x += x * v.x; acc[j][i].y += x * v.y; acc[j][i].z += x * v.z; acc[j][i].w += x * v.w; }
+            }
+          }
         }
       }
       __syncwarp();
     }
 #pragma unroll
-    for (int o = 1; o < 8; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-    if (row < p.t.nrows) {
+    for (int j = 0; j < 4; ++j) {
 #pragma unroll
-      for (int i = 0; i < HD / 32; ++i)
-        simt_store<HD, 4>(a, p, row, i * 32 + sub * 4, reinterpret_cast<const float*>(&acc[i]), m == -INFINITY ? 0.f : m, l, i == 0 && sub == 0);
+      for (int o = 1; o < 16; o <<= 1) l[j] += __shfl_xor_sync(0xffffffffu, l[j], o);
+      const int r = rg * 4 + j;
+      if (r < p.t.nrows)
+#pragma unroll
+        for (int i = 0; i < CT; ++i)
+          simt_store<HD, 4>(a, p, r, i * 64 + cg * 4, reinterpret_cast<const float*>(&acc[j][i]), m[j] == -INFINITY ? 0.f : m[j], l[j], i == 0 && cg == 0);
     }
   }
 }
