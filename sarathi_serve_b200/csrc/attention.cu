@@ -9,6 +9,7 @@
 namespace sb200 {
 
 constexpr int kPlanThreads = 1024;
+constexpr int kNearTiles = 1024;
 constexpr int kJoinThreads = 256, kJoinValues = 4 * kJoinThreads;
 
 struct PlanArgs {
@@ -75,6 +76,7 @@ attn_plan_kernel(const PlanArgs a) {
   int* first = smem_i;               // [n + 1] first tile of every request that has tiles of many rows,
   int* few = smem_i + a.n + 1;       // and of those with few: these come behind all others
   __shared__ long long red[33];
+  __shared__ long long near[kNearTiles];  // costs of the first tiles: the search below reads them one after the other
   const AttnShape& sh = a.sh;
   const int per = (a.n + kPlanThreads - 1) / kPlanThreads, r0 = min(a.n, (int)threadIdx.x * per), r1 = min(a.n, r0 + per);
   auto span = [&](int r, int* q0) {
@@ -149,7 +151,10 @@ attn_plan_kernel(const PlanArgs a) {
       c = ((long long)d.nblk * block + fixed) * sh.kv_heads;
     }
     const long long at = carry + scan_block(c, red, &total);
-    if (t < tiles) a.plan.cost[t] = at;
+    if (t < tiles) {
+      a.plan.cost[t] = at;
+      if (t < kNearTiles) near[t] = at;
+    }
     carry += total;
   }
   __shared__ int4 at[kAttnMaxWorkers + 1];
@@ -165,13 +170,13 @@ attn_plan_kernel(const PlanArgs a) {
       int lo = 0, hi = tiles - 1;
       while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
-        if (a.plan.cost[mid] <= x) lo = mid;
+        if ((mid < kNearTiles ? near[mid] : a.plan.cost[mid]) <= x) lo = mid;
         else hi = mid - 1;
       }
       const AttnTile d = a.plan.tiles[lo];
       int block, fixed, least;
       unit_cost(sh, d.kind, d.nrows, &block, &fixed, &least);
-      const long long unit = (long long)d.nblk * block + fixed, rem = x - a.plan.cost[lo];
+      const long long unit = (long long)d.nblk * block + fixed, rem = x - (lo < kNearTiles ? near[lo] : a.plan.cost[lo]);
       int head = (int)(rem / unit);
       const long long in = rem - head * unit;
       int blk = in <= fixed / 2 ? 0 : (int)min((in - fixed / 2 + block / 2) / block, (long long)d.nblk);

@@ -404,7 +404,8 @@ attn_simt_kernel(const __grid_constant__ AttnArgs a) {
 
 template <int HD>
 static int launch_simt(const AttnArgs& a, int workers, cudaStream_t s) {
-  SB_CUDA(cudaFuncSetAttribute(attn_simt_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)simt_smem<HD>()));
+  static std::atomic<uint64_t> allowed{0};
+  SB_CUDA(allow_smem(reinterpret_cast<const void*>(attn_simt_kernel<HD>), (int)simt_smem<HD>(), &allowed));
   SB_CUDA(launch_dependent(attn_simt_kernel<HD>, dim3((unsigned)workers), dim3(kSimtThreads), simt_smem<HD>(), s, a));
   return SB200_OK;
 }

@@ -907,8 +907,9 @@ static int launch_tc(const AttnArgs& a, bool many, int workers, cudaStream_t s) 
     const int rc = make_tmap_4d(&map, DT<T>::id, a.cache, dims, strides, box);
     if (rc) return rc;
   }
-  SB_CUDA(cudaFuncSetAttribute(attn_tc_kernel<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  static std::atomic<uint64_t> allowed{0};
   auto kern = attn_tc_kernel<T, HD>;  // (waits for its predecessor by hand)
+  SB_CUDA(allow_smem(reinterpret_cast<const void*>(kern), smem, &allowed));
   SB_CUDA(launch_dependent(kern, dim3((unsigned)workers), dim3(tc_threads<HD>()), smem, s, a, map));
   return SB200_OK;
 }

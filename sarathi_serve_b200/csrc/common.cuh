@@ -13,6 +13,8 @@
 #include <cuda_bf16.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "../../include/sarathi_b200.h"
 
 namespace sb200 {
@@ -155,6 +157,19 @@ __host__ __device__ inline bool aligned16(const void* p) { return (reinterpret_c
 
 // Number of SMs of the current device (cached per process).
 int sm_count();
+
+// Lets a kernel have `bytes` of dynamic shared memory: asked of the runtime once per kernel and device (`done`: a bit per
+// device, static beside the launch), as the call costs a fifth of a launch.
+inline cudaError_t allow_smem(const void* kernel, int bytes, std::atomic<uint64_t>* done) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+  if (done->load(std::memory_order_relaxed) & bit) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) done->fetch_or(bit, std::memory_order_relaxed);
+  return e;
+}
 
 #define SB_DISPATCH_FLOAT(dt, ...)                                            \
   switch (dt) {                                                               \

@@ -112,8 +112,7 @@ def resize_block_tables(block_tables: torch.Tensor, num_blocks: torch.Tensor, se
     return granted
 
 
-class BatchLayout(NamedTuple):
-    """Index arrays of a step (see ``batch_layout``)."""
+class _BatchArrays(NamedTuple):
     qo_indptr: torch.Tensor      # int32 [n + 1]
     kv_lens: torch.Tensor        # int32 [n]
     kv_indptr: torch.Tensor      # int32 [n + 1]
@@ -122,6 +121,12 @@ class BatchLayout(NamedTuple):
     batch_indices: torch.Tensor  # int32 [num_tokens]
     positions: torch.Tensor      # int64 [num_tokens]
     kv_slots: torch.Tensor       # int64 [num_tokens]
+
+
+class BatchLayout(_BatchArrays):
+    """Index arrays of a step (see ``batch_layout``).  ``_for``: the sizes and device that ``batch_layout`` made or checked them
+    for, with their addresses, so that a step that writes them again need not look at eight tensors."""
+    _for = None
 
 
 def batch_layout(query_lens: torch.Tensor, context_lens: torch.Tensor, block_tables: torch.Tensor, page_size: int, num_pages: int,
@@ -145,13 +150,19 @@ def batch_layout(query_lens: torch.Tensor, context_lens: torch.Tensor, block_tab
     T, width, dev = int(num_tokens), block_tables.shape[1], query_lens.device
     if T < 0:
         raise RuntimeError(f"{what}: num_tokens is negative")
+    sizes = (n, width, T, dev)
     if out is None:
-        # one allocation each for the two types; int32 parts one after the other
-        ints = torch.empty(4 * n + 2 + n * width + T, dtype=torch.int32, device=dev)
-        a, b, c, d, e, f = ints.split([n + 1, n, n + 1, n * width, n, T])
+        # one allocation each for the two types; the parts of either one after the other
+        parts = [n + 1, n, n + 1, n * width, n, T]
+        ints = torch.empty(sum(parts), dtype=torch.int32, device=dev)
         longs = torch.empty(2, T, dtype=torch.int64, device=dev)
-        out = BatchLayout(a, b, c, d, e, f, longs[0], longs[1])
-    else:
+        out = BatchLayout(*torch.split_with_sizes(ints, parts), *longs.unbind(0))
+        at, pointers = ints.data_ptr(), []
+        for k in parts:
+            pointers.append(at)
+            at += 4 * k
+        out._for = (sizes, (*pointers, longs.data_ptr(), longs.data_ptr() + 8 * T), parts[3])
+    elif getattr(out, "_for", None) is None or out._for[0] != sizes or out._for[1][0] != out[0].data_ptr():
         N.require_current(*out)
         for name, t, k in zip(BatchLayout._fields, out, (n + 1, n, n + 1, -1, n, T)):
             _int32("out." + name, t, k, what)
@@ -160,8 +171,9 @@ def batch_layout(query_lens: torch.Tensor, context_lens: torch.Tensor, block_tab
         for t in out[6:]:
             if t.dtype != torch.int64 or t.shape != (T,) or not t.is_contiguous():
                 raise RuntimeError(f"{what}: out.positions and out.kv_slots must be contiguous int64 tensors of {T} elements")
-    N.check(N.lib().sb200_batch_layout(N.ptr(query_lens), N.ptr(context_lens), N.ptr(block_tables), _table_stride(block_tables), n, width,
-                                       int(page_size), int(num_pages), T, N.ptr(out.qo_indptr), N.ptr(out.kv_lens),
-                                       N.ptr(out.kv_indptr), N.ptr(out.kv_indices), out.kv_indices.numel(), N.ptr(out.last_page_len),
-                                       N.ptr(out.batch_indices), N.ptr(out.positions), N.ptr(out.kv_slots), N.stream_ptr()), what)
+        out._for = (sizes, tuple(t.data_ptr() for t in out), out.kv_indices.numel())
+    _, (qo, kv, indptr, indices, last, req, pos, slot), capacity = out._for
+    N.check(N.lib().sb200_batch_layout(query_lens.data_ptr(), context_lens.data_ptr(), block_tables.data_ptr(), _table_stride(block_tables),
+                                       n, width, int(page_size), int(num_pages), T, qo, kv, indptr, indices, capacity, last, req, pos,
+                                       slot, N.stream_ptr()), what)
     return out
