@@ -128,10 +128,13 @@ __device__ __forceinline__ void turn_quad(uint4 (&v)[4], int lane4) {
   swap(v[1], v[3], 2, up2);
 }
 
-// One row's output recomputed key by key: what a product with P = 0 cannot do is to leave out a value that is not finite.
-// Called by a warp for a row whose output came out not finite; m is the maximum that the row's sum l was made with.
+// What a product with P = 0 cannot do is to leave out a value that is not finite.  Called by a warp for a row of which some columns
+// came out not finite; o: this lane's columns lane * HD / 32 ..., m: the maximum that the row's sum was made with.  Only keys that
+// the tile has and the row does not see can have spoilt it: if one of them is not finite in such a column, the column is
+// made again, key by key (true is returned); if none is, the result stands.  So a value that is not finite costs the rows that see
+// it a look at their tile's last keys, and only the rows of its own tile before it the long way.
 template <typename T, int HD>
-__device__ __noinline__ void attn_repair_row(const AttnArgs& a, const AttnPiece& p, int r, float m, float* o) {
+__device__ __noinline__ bool attn_repair_row(const AttnArgs& a, const AttnPiece& p, int r, float m, float* o) {
   constexpr int N = HD / 32;
   const int lane = threadIdx.x & 31;
   int token, head, pos;
@@ -139,11 +142,27 @@ __device__ __noinline__ void attn_repair_row(const AttnArgs& a, const AttnPiece&
   const T* q = reinterpret_cast<const T*>(a.q) + token * a.ldq + head * HD + lane * N;
   const T* cache = reinterpret_cast<const T*>(a.cache) + p.head * HD + lane * N;
   const int64_t ldc = (int64_t)a.kv_heads * HD;
-  float x[N];
+  const int begin = max(p.lo, (p.t.blk_lo + p.b0) * kAttnBlock), end = min(p.hi, (p.t.blk_lo + p.b1) * kAttnBlock);
+  const int k0 = max(begin, a.window > 0 ? pos + 1 - a.window : 0), k1 = min(end, pos + 1);  // what the row sees of the piece
+  bool spoilt[N] = {};
+  auto look = [&](int from, int to) {
+    for (int key = from; key < to; ++key) {
+      const int at = attn_key_row(a, p.t.page_at, key);
+      if (at < 0) continue;
 #pragma unroll
-  for (int j = 0; j < N; ++j) { x[j] = DT<T>::to_f(q[j]); o[j] = 0.f; }
-  const int k0 = max(a.window > 0 ? max(0, pos + 1 - a.window) : 0, (p.t.blk_lo + p.b0) * kAttnBlock);
-  const int k1 = min(pos + 1, (p.t.blk_lo + p.b1) * kAttnBlock);
+      for (int j = 0; j < N; ++j)
+        if (!(fabsf(o[j]) < INFINITY) && !(fabsf(DT<T>::to_f(cache[(at + a.page_size) * ldc + j])) < INFINITY)) spoilt[j] = true;
+    }
+  };
+  look(begin, min(k0, end));
+  look(max(k1, begin), end);
+  bool any = false;
+#pragma unroll
+  for (int j = 0; j < N; ++j) any = any || spoilt[j];
+  if (!__any_sync(0xffffffffu, any)) return false;
+  float x[N], y[N];
+#pragma unroll
+  for (int j = 0; j < N; ++j) { x[j] = DT<T>::to_f(q[j]); y[j] = 0.f; }
   for (int key = k0; key < k1; ++key) {
     const int at = attn_key_row(a, p.t.page_at, key);
     float s = 0.f;
@@ -152,8 +171,12 @@ __device__ __noinline__ void attn_repair_row(const AttnArgs& a, const AttnPiece&
     s = warp_sum(s);
     const float pr = DT<T>::to_f(DT<T>::from_f(pow2(s * a.scale_log2 - m)));
 #pragma unroll
-    for (int j = 0; j < N; ++j) o[j] += pr * (at >= 0 ? DT<T>::to_f(cache[(at + a.page_size) * ldc + j]) : 0.f);
+    for (int j = 0; j < N; ++j) y[j] += pr * (at >= 0 ? DT<T>::to_f(cache[(at + a.page_size) * ldc + j]) : 0.f);
   }
+#pragma unroll
+  for (int j = 0; j < N; ++j)
+    if (spoilt[j]) o[j] = y[j];
+  return true;
 }
 
 // The steps of 16 keys that a warp loads (or computes) for the pieces of its CTA's share, one after the other.
@@ -374,7 +397,7 @@ __device__ void few_share(const AttnArgs& a, uint8_t* smem, int worker) {
         bool fine = true;
 #pragma unroll
         for (int j = 0; j < N; ++j) fine = fine && fabsf(acc[j]) < INFINITY;
-        if (!__all_sync(0xffffffffu, fine)) {
+        if (!__all_sync(0xffffffffu, fine) && l == l) {
           const AttnPiece copy = p;  // (p itself stays in registers)
           attn_repair_row<T, HD>(a, copy, r, base, acc);
         }
@@ -800,23 +823,31 @@ __device__ __forceinline__ void many_softmax(const AttnArgs& a, uint8_t* smem, M
       if (p.slot >= 0) a.part_l[at] = some ? base2 + log2f(l) : -INFINITY;
       else if (a.lse) a.lse[(int64_t)token * (a.kv_heads * a.group) + head] = (base2 + log2f(l)) * 0.69314718055994531f;
     }
-    uint32_t bad = __ballot_sync(0xffffffffu, real && !fine);
+    uint32_t bad = __ballot_sync(0xffffffffu, real && !fine && l == l);  // (a sum that is no number spoils the whole row, rightly)
+    __syncwarp();
     while (bad) {
       const int who = __ffs(bad) - 1;
       bad &= bad - 1;
       constexpr int N = HD / 32;
       const AttnPiece copy = p;  // (p itself stays in registers)
-      float o[N];
       const int row = sub * 128 + quarter * 32 + who;
-      const float f = __shfl_sync(0xffffffffu, inv, who);
-      attn_repair_row<T, HD>(a, copy, row, __shfl_sync(0xffffffffu, base2, who), o);
       int tk, hd, ps;
       attn_row(a, p, row, &tk, &hd, &ps);
+      T* dst = reinterpret_cast<T*>(a.out) + tk * a.ldo + hd * HD;
+      auto part = [&](int c) { return reinterpret_cast<float*>(attn_part(a, HD, p.slot, p.stride, row, c / 4)) + (c & 3); };
+      float o[N];  // what the row's thread has just stored
+#pragma unroll
+      for (int j = 0; j < N; ++j) o[j] = p.slot < 0 ? DT<T>::to_f(dst[lane * N + j]) : *part(lane * N + j);
+      bool ok[N];
+#pragma unroll
+      for (int j = 0; j < N; ++j) ok[j] = fabsf(o[j]) < INFINITY;
+      const float f = __shfl_sync(0xffffffffu, inv, who);
+      if (!attn_repair_row<T, HD>(a, copy, row, __shfl_sync(0xffffffffu, base2, who), o)) continue;
 #pragma unroll
       for (int j = 0; j < N; ++j) {
-        const int c = lane * N + j;
-        if (p.slot < 0) reinterpret_cast<T*>(a.out)[tk * a.ldo + hd * HD + c] = DT<T>::from_f(o[j] * f);
-        else reinterpret_cast<float*>(attn_part(a, HD, p.slot, p.stride, row, c / 4))[c & 3] = o[j] * f;
+        if (ok[j]) continue;
+        if (p.slot < 0) dst[lane * N + j] = DT<T>::from_f(o[j] * f);
+        else *part(lane * N + j) = o[j] * f;
       }
     }
     ptx::tc_fence_before();  // O and S may be written again once the next q_full / p_full is seen

@@ -188,6 +188,33 @@ def test_values_that_a_row_does_not_see(dtype, hd, bad):
             assert d[fine.view(c["total"], -1)].max() <= 0, (window, new, before, at)
 
 
+@pytest.mark.parametrize("dtype,hd", [(torch.bfloat16, 128), (torch.float16, 64)])
+def test_a_value_that_is_not_finite_in_a_long_context(dtype, hd):
+    """Seen by every row of a chunk: their results are not finite in its column, the other columns are as they were."""
+    from sarathi_serve_b200 import attention_ops
+    c = make(12, dtype, 4, 2, hd, 16, [(200, 5000), (1, 3000)])
+    for r, at in ((0, 17), (1, 2990)):
+        c["cache"][c["table"][r, at // 16], 1, at % 16, 0, 7] = float("inf")
+    plan, _ = plan_of(c)
+    check(c, attention_ops.paged_attention(c["q"], c["cache"], plan, hd ** -0.5), hd ** -0.5)
+
+
+@pytest.mark.parametrize("dtype,hd,kv_heads,pages", [(torch.bfloat16, 128, 8, 70000), (torch.float32, 64, 8, 140000)])
+def test_cache_beyond_32_bits_of_elements(dtype, hd, kv_heads, pages):
+    """Pages whose elements lie beyond 2^31, in all kinds of tiles."""
+    from sarathi_serve_b200 import attention_ops
+    batch, page = [(1, 300), (70, 130), (5, 20)], 16
+    c = make(13, dtype, 2 * kv_heads, kv_heads, hd, page, batch)
+    big = torch.empty(pages, 2, page, kv_heads, hd, dtype=dtype, device="cuda")
+    assert big.numel() > 2 ** 31
+    used = c["pool"]
+    big[pages - used:] = c["cache"]
+    c.update(cache=big, table=torch.where(c["table"] >= 0, c["table"] + (pages - used), c["table"]), pool=pages)
+    plan, lay = plan_of(c)
+    assert int(lay.kv_slots.max()) * kv_heads * hd > 2 ** 31 - 2 ** 24
+    check(c, attention_ops.paged_attention(c["q"], c["cache"], plan, hd ** -0.5), hd ** -0.5)
+
+
 @pytest.mark.parametrize("dtype,hd", [(torch.bfloat16, 128), (torch.float16, 64), (torch.float32, 128)])
 def test_keys_that_are_not_numbers(dtype, hd):
     """A NaN in a key makes the rows that see it NaN, wherever it lies in a block, and leaves the others alone."""
