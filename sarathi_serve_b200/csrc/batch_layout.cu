@@ -5,8 +5,8 @@
 // (sarathi/core/block_space_manager, sarathi/model_executor/attention/flashinfer_attention_wrapper.py), which walk the
 // sequences in Python every step.
 //
-// Both kernels are bound by latency (their floor is well below a microsecond for a step of a few hundred requests), so each
-// is ONE launch: every CTA computes the prefix sums over the requests for itself, into shared memory, and the items (pages,
+// Both kernels are bound by latency (their floor is well below a microsecond for a step of a few hundred requests; the layout
+// of 212 requests with 1997 tokens takes 5.6 us), so each is ONE launch: every CTA computes the prefix sums over the requests for itself, into shared memory, and the items (pages,
 // tokens) are then dealt out flat -- an item finds its request by binary search -- so that one request with thousands of
 // pages takes no longer than thousands of requests with one.
 #include "common.cuh"
@@ -74,16 +74,22 @@ __device__ __forceinline__ int pages_wanted(int len, int page, int width) {
 
 // One CTA, or a cluster of them when many pages may move.  Given-back pages are pushed in request order and grants pop in
 // request order; a grant that reaches into the pages just pushed reads them from the table they come from, so that the two
-// halves need no barrier between them -- only the counters, which every CTA reads, are written behind one.
-// 128 requests that grow by a token: 3.1 us a launch; 512 requests with 74000 pages to move: see the kernel's launch.
-__global__ void __launch_bounds__(kLayoutThreads)
+// halves need no barrier between them -- only the counters, which every CTA reads, are written behind one.  A page is a search
+// in shared memory, a load and a store after one another, about 1.3 us: a thread has four of them under way.
+// 128 requests of which a few start a page: 4.3 us; 512 requests with 74000 pages to move: 15 us (one page at a time: 24.6; a cluster of
+// four: 25).
+constexpr int kTablesThreads = 1024;
+
+__global__ void __launch_bounds__(kTablesThreads)
 resize_tables_kernel(const TablesArgs a) {
   grid_dependency_begin();
   extern __shared__ int smem_i[];
   __shared__ long long red[33];
   int* give = smem_i;              // exclusive prefix sums of the pages given back, and of the pages asked for
   int* take = smem_i + a.n + 1;
-  const int per = (a.n + kLayoutThreads - 1) / kLayoutThreads, r0 = min(a.n, (int)threadIdx.x * per), r1 = min(a.n, r0 + per);
+  int* owned = smem_i + 2 * (a.n + 1);   // pages that every request has, and wants
+  int* wanted = owned + a.n;
+  const int per = (a.n + kTablesThreads - 1) / kTablesThreads, r0 = min(a.n, (int)threadIdx.x * per), r1 = min(a.n, r0 + per);
   const int ctas = gridDim.x, cta = blockIdx.x;
 
   auto both = [&](int r, int* have, int* want) {  // (a negative length: the request is left alone)
@@ -95,6 +101,8 @@ resize_tables_kernel(const TablesArgs a) {
   for (int r = r0; r < r1; ++r) {
     int have, want;
     both(r, &have, &want);
+    owned[r] = have;
+    wanted[r] = want;
     if (want < have) g += have - want;
     else if (want <= a.width) t += want - have;
   }
@@ -103,8 +111,7 @@ resize_tables_kernel(const TablesArgs a) {
   long long tp = block_exclusive_scan(t, red, &all_take);
   const int n0 = clampi(*a.num_free, 0, a.capacity);
   for (int r = r0; r < r1; ++r) {
-    int have, want;
-    both(r, &have, &want);
+    const int have = owned[r], want = wanted[r];
     give[r] = (int)gp;
     take[r] = (int)tp;
     if (want < have) gp += have - want;
@@ -121,23 +128,39 @@ resize_tables_kernel(const TablesArgs a) {
 
   auto given_page = [&](int e) {
     const int r = owner_of(give, a.n, e);
-    int have, want;
-    both(r, &have, &want);
-    return a.tables[r * a.ld + want + (e - give[r])];
+    return a.tables[r * a.ld + wanted[r] + (e - give[r])];
   };
-  const int first = cta * kLayoutThreads + threadIdx.x, step = ctas * kLayoutThreads;
-  for (int e = first; e < given; e += step) a.free_blocks[n0 + e] = given_page(e);
-  for (int e = first; e < taken; e += step) {
-    const int r = owner_of(take, a.n, e), at = avail - 1 - e;
-    const int page = at >= n0 ? given_page(at - n0) : a.free_blocks[at];
-    a.tables[r * a.ld + clampi(a.num_blocks[r], 0, a.width) + (e - take[r])] = page;
+  const int first = cta * kTablesThreads + threadIdx.x, step = ctas * kTablesThreads;
+  constexpr int kAhead = 4;
+  for (int e0 = first; e0 < given; e0 += kAhead * step) {
+    int page[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i)
+      if (e0 + i * step < given) page[i] = given_page(e0 + i * step);
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i)
+      if (e0 + i * step < given) a.free_blocks[n0 + e0 + i * step] = page[i];
+  }
+  for (int e0 = first; e0 < taken; e0 += kAhead * step) {
+    int page[kAhead];
+    int32_t* to[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int e = e0 + i * step, at = avail - 1 - e;
+      if (e >= taken) continue;
+      const int r = owner_of(take, a.n, e);
+      page[i] = at >= n0 ? given_page(at - n0) : a.free_blocks[at];
+      to[i] = a.tables + (r * a.ld + owned[r] + (e - take[r]));
+    }
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i)
+      if (e0 + i * step < taken) *to[i] = page[i];
   }
   if (ctas > 1) ptx::cluster_sync_all();
   else __syncthreads();
   if (cta == 0) {
-    for (int r = threadIdx.x; r < a.n; r += kLayoutThreads) {
-      int have, want;
-      both(r, &have, &want);
+    for (int r = threadIdx.x; r < a.n; r += kTablesThreads) {
+      const int have = owned[r], want = wanted[r];
       const bool ok = want < have ? give[r + 1] <= given : want == have || (want <= a.width && take[r + 1] <= taken);
       a.granted[r] = ok ? 1 : 0;
       a.num_blocks[r] = ok ? want : have;
@@ -226,13 +249,13 @@ batch_layout_kernel(const LayoutArgs a) {
 
 using namespace sb200;
 
-static size_t layout_smem(int n) { return 2 * (size_t)(n + 1) * sizeof(int); }
+static size_t layout_smem(int n, int arrays) { return (size_t)arrays * (n + 1) * sizeof(int); }
 
 extern "C" int sb200_resize_block_tables(int32_t* block_tables, int64_t ld, int32_t* num_blocks, const int32_t* seq_lens,
                                          int32_t* free_blocks, int32_t* num_free, int32_t* granted, int num_requests, int width,
                                          int64_t capacity, int page_size, sb200_stream_t stream) {
   SB_CHECK_ARG(num_requests >= 0 && width >= 0 && capacity >= 0 && page_size > 0 && ld >= width && width < INT32_MAX &&
-                   capacity <= INT32_MAX && (int64_t)num_requests * width <= INT32_MAX,
+                   capacity <= INT32_MAX && (int64_t)num_requests * width <= INT32_MAX / 2,
                "resize_block_tables: bad sizes (%d requests, %d blocks each, %lld free)", num_requests, width, (long long)capacity);
   if (num_requests > kMaxRequests) {
     set_error("resize_block_tables: %d requests, at most %d are supported", num_requests, kMaxRequests);
@@ -244,12 +267,12 @@ extern "C" int sb200_resize_block_tables(int32_t* block_tables, int64_t ld, int3
   TablesArgs a = {block_tables, ld, num_blocks, seq_lens, free_blocks, num_free, granted, num_requests, width, (int)capacity, page_size};
   // Eight CTAs where the tables could hold so many pages that a prompt's worth of them may move in one step.
   const int ctas = (int64_t)num_requests * width > 16384 ? 8 : 1;
-  const size_t smem = layout_smem(num_requests);
+  const size_t smem = layout_smem(num_requests, 4);
   if (smem > 48 * 1024)
     SB_CUDA(cudaFuncSetAttribute(resize_tables_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(ctas);
-  cfg.blockDim = dim3(kLayoutThreads);
+  cfg.blockDim = dim3(kTablesThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = (cudaStream_t)stream;
   cudaLaunchAttribute attr[2];
@@ -289,7 +312,7 @@ extern "C" int sb200_batch_layout(const int32_t* query_lens, const int32_t* cont
   if (items < num_requests + 1) items = num_requests + 1;
   int64_t ctas = (items + kLayoutThreads - 1) / kLayoutThreads;
   if (ctas > sm_count()) ctas = sm_count();
-  const size_t smem = layout_smem(num_requests);
+  const size_t smem = layout_smem(num_requests, 2);
   if (smem > 48 * 1024)
     SB_CUDA(cudaFuncSetAttribute(batch_layout_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   SB_CUDA(launch_dependent(batch_layout_kernel, dim3((unsigned)ctas), dim3(kLayoutThreads), smem, (cudaStream_t)stream, a));
