@@ -869,44 +869,45 @@ __global__ void __launch_bounds__(tc_threads<HD>(), 1)
 attn_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUtensorMap map) {
   extern __shared__ uint8_t smem_tc[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_tc) + 1023) & ~uintptr_t(1023));
-  ptx::grid_dependency_wait();
   if constexpr (HD == 256) {
+    ptx::grid_dependency_wait();
     ptx::grid_launch_dependents();
     few_share<T, HD>(a, smem, blockIdx.x);
   } else {
+    // Barriers and TMEM before the wait, whether the share will need them or not: under the end of the kernel before.
     __shared__ __align__(8) ManySync sy;
     const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0);
+    if (threadIdx.x == 0) {
+      for (int i = 0; i < Many<HD>::STAGES; ++i) { ptx::mbar_init(&sy.full[i], 1); ptx::mbar_init(&sy.empty[i], 1); }
+      for (int i = 0; i < 2; ++i) {
+        ptx::mbar_init(&sy.q_full[i], 1); ptx::mbar_init(&sy.q_empty[i], 1); ptx::mbar_init(&sy.turn[i], 1);
+        ptx::mbar_init(&sy.p_full[i][0], 4); ptx::mbar_init(&sy.p_full[i][1], 4);
+      }
+      ptx::mbar_init(&sy.drain, 1);
+      sy.abort_word = 0;
+      ptx::mbar_fence_init();
+      if (a.page_size % 8 == 0) ptx::prefetch_tensormap(&map);  // (otherwise there is none)
+    }
+    if (warp == 8) { ptx::tmem_alloc(&sy.tmem, 512); ptx::tmem_relinquish(); }
+    ptx::tc_fence_before();
+    __syncthreads();
+    ptx::tc_fence_after();
+    ptx::grid_launch_dependents();  // the TMEM is ours
+    ptx::grid_dependency_wait();
     AttnWalk walk(a, blockIdx.x);
     walk.only_many();
     const bool many = walk.more();  // the same for the whole CTA
-    if (many) {
-      if (threadIdx.x == 0) {
-        for (int i = 0; i < Many<HD>::STAGES; ++i) { ptx::mbar_init(&sy.full[i], 1); ptx::mbar_init(&sy.empty[i], 1); }
-        for (int i = 0; i < 2; ++i) {
-          ptx::mbar_init(&sy.q_full[i], 1); ptx::mbar_init(&sy.q_empty[i], 1); ptx::mbar_init(&sy.turn[i], 1);
-          ptx::mbar_init(&sy.p_full[i][0], 4); ptx::mbar_init(&sy.p_full[i][1], 4);
-        }
-        ptx::mbar_init(&sy.drain, 1);
-        sy.abort_word = 0;
-        ptx::mbar_fence_init();
-        ptx::prefetch_tensormap(&map);
-      }
-      if (warp == 8) { ptx::tmem_alloc(&sy.tmem, 512); ptx::tmem_relinquish(); }
-      ptx::tc_fence_before();
-      __syncthreads();
-      ptx::tc_fence_after();
-    }
-    ptx::grid_launch_dependents();  // the TMEM is ours
     __syncwarp();
     if (warp >= 8) {
       ptx::registers_shrink<72>();
-      if (!many) return;
-      if (warp == 9) many_load<HD>(a, &map, smem, sy, walk);
-      else if (warp >= 10) many_queries<T, HD>(a, smem, sy, walk, warp - 10);
-      else if (warp == 8) many_multiply<T, HD>(a, smem, sy, walk);
-      __syncwarp();
-      ptx::tc_fence_before();
-      __syncthreads();
+      if (many) {
+        if (warp == 9) many_load<HD>(a, &map, smem, sy, walk);
+        else if (warp >= 10) many_queries<T, HD>(a, smem, sy, walk, warp - 10);
+        else if (warp == 8) many_multiply<T, HD>(a, smem, sy, walk);
+        __syncwarp();
+        ptx::tc_fence_before();
+        __syncthreads();
+      }
       if (warp == 8) {
         ptx::tc_fence_after();
         ptx::tmem_dealloc(sy.tmem, 512);
