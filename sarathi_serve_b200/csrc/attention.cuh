@@ -178,6 +178,22 @@ __device__ __forceinline__ int attn_key_row(const AttnArgs& a, int page_at, int 
   return (unsigned)page < (unsigned)a.num_pages ? page * 2 * a.page_size + (key - p * a.page_size) : -1;
 }
 
+// The same in two halves, for loads that run ahead: the entry of kv_indices is asked for now (whatever it says is looked at
+// later, so that nothing waits for it), the row is made when its turn comes.
+struct AttnAhead {
+  int page, slot;  // slot < 0: a key that no row sees
+  __device__ __forceinline__ void ask(const AttnArgs& a, int page_at, int key, bool seen) {
+    const int p = a.by_page.div(max(key, 0));
+    const long long at = (long long)page_at + p;
+    seen = seen && at < a.num_kv_indices;
+    page = seen ? a.kv_indices[at] : -1;
+    slot = seen ? key - p * a.page_size : -1;
+  }
+  __device__ __forceinline__ int row(const AttnArgs& a) const {
+    return slot >= 0 && (unsigned)page < (unsigned)a.num_pages ? page * 2 * a.page_size + slot : -1;
+  }
+};
+
 // Where row r of a piece's tile goes: (token row, q head).
 __device__ __forceinline__ void attn_row(const AttnArgs& a, const AttnPiece& p, int r, int* token, int* head, int* pos) {
   const int row = p.t.row0 + r, tok = a.by_group.div(row);

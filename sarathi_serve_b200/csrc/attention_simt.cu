@@ -230,18 +230,19 @@ __device__ void simt_few(const AttnArgs& a, float* smem, const AttnWalk& walk) {
 
   Few32Steps<HD> ld(walk);
   bool more = true;
-  int row_next = -1, head_next = 0, put = 0;
-  auto look_up = [&]() {  // lane i: the row of key i of the step after the next
+  AttnAhead next;
+  int head_next = 0, put = 0;
+  auto look_up = [&]() {  // lane i: the page of key i of the step after the next
     while (more && ld.key >= ld.end) more = ld.next_piece(a, warp);
     if (!more) return;
     const int key = ld.key + lane % F::KEYS;
-    row_next = key >= ld.p.lo && key < ld.p.hi ? attn_key_row(a, ld.p.t.page_at, key) : -1;
+    next.ask(a, ld.p.t.page_at, key, key >= ld.p.lo && key < ld.p.hi);
     head_next = ld.p.head;
     ld.key += kStep;
   };
   auto load = [&]() {
     if (more) {
-      const int rows = row_next, head = head_next;
+      const int rows = next.row(a), head = head_next;
       const uint32_t dst = ptx::smem_u32(ring) + put * (2 * F::HALF);
 #pragma unroll
       for (int i = 0; i < F::KEYS * CPR / 32; ++i) {

@@ -211,22 +211,23 @@ __device__ void few_share(const AttnArgs& a, uint8_t* smem, int worker) {
   const int64_t ldc = (int64_t)a.kv_heads * HD;
   constexpr int kStep = F::WARPS * kFewKeys;
 
-  // loads: one step ahead of the copies runs the look-up of the keys' rows (lane i: key i of the step)
+  // loads: one step ahead of the copies the pages of the keys are asked for (lane i: key i of the step)
   FewSteps<HD> ld(a, worker);
   bool more = true;
-  int row_next = -1, head_next = 0;
+  AttnAhead next;
+  int head_next = 0;
   auto look_up = [&]() {
     while (more && ld.key >= ld.end) more = ld.next_piece(a, warp);
     if (!more) return;
     const int key = ld.key + (lane & 15);
-    row_next = key >= ld.p.lo && key < ld.p.hi ? attn_key_row(a, ld.p.t.page_at, key) : -1;
+    next.ask(a, ld.p.t.page_at, key, key >= ld.p.lo && key < ld.p.hi);
     head_next = ld.p.head;
     ld.key += kStep;
   };
   int put = 0;
   auto load = [&]() {
     if (more) {
-      const int rows = row_next, head = head_next;
+      const int rows = next.row(a), head = head_next;
       const uint32_t dst = ring + put * (2 * F::HALF);
       const int sub = lane / CPR, chunk = lane % CPR;
 #pragma unroll
