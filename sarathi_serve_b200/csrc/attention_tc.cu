@@ -857,8 +857,8 @@ __device__ __forceinline__ void many_softmax(const AttnArgs& a, uint8_t* smem, M
 }
 
 template <int HD> constexpr int tc_threads() { return HD == 256 ? Few<HD>::WARPS * 32 : 384; }
-template <int HD> constexpr int tc_smem() {
-  if constexpr (HD == 256) return Few<HD>::SMEM;
+template <int HD> constexpr int tc_smem() {  // (1024: the kernel aligns its start)
+  if constexpr (HD == 256) return Few<HD>::SMEM + 1024;
   else return (Few<HD>::SMEM > Many<HD>::SMEM ? Few<HD>::SMEM : Many<HD>::SMEM) + 1024;
 }
 
