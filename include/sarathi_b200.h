@@ -235,8 +235,8 @@ int sb200_kv_cache_append(void* cache, const void* k, int64_t ldk, const void* v
  * pop theirs from its top, in order.  A request that wants more than `width` pages gets none and costs none; one that the
  * remaining pages do not suffice for gets none, nor do those that grow after it: granted[r] is 1 where request r has what it
  * asked for and 0 where it was left as it was.  A negative length leaves a request alone (granted).  Pages whose push would
- * pass `capacity` stay with their request (granted 0).  Entries beyond num_blocks / *num_free keep what they held.  Rows must
- * not overlap.  Nothing is read on the host.  Counterpart in the reference: the block manager's lists
+ * pass `capacity` stay with their request (granted 0).  Entries beyond num_blocks / *num_free keep what they held.  Neither
+ * rows nor arrays may overlap.  Nothing is read on the host.  Counterpart in the reference: the block manager's lists
  * (sarathi/core/block_space_manager), host code. */
 int sb200_resize_block_tables(int32_t* block_tables, int64_t ld, int32_t* num_blocks, const int32_t* seq_lens,
                               int32_t* free_blocks, int32_t* num_free, int32_t* granted, int num_requests, int width,
@@ -249,7 +249,7 @@ int sb200_resize_block_tables(int32_t* block_tables, int64_t ld, int32_t* num_bl
  *   per row: batch_indices (request, -1 for padding), positions (int64, 0 for padding), kv_slots as sb200_kv_cache_slots
  *   (-1 for padding and for pages outside [0, num_pages)).
  * Negative lengths count as zero; a context is cut to what the table has room for, and new tokens to what is then left in the
- * table and in num_tokens.  Replaces the host loops of begin_forward
+ * table and in num_tokens.  No array that is written may overlap another one.  Replaces the host loops of begin_forward
  * (sarathi/model_executor/attention/flashinfer_attention_wrapper.py). */
 int sb200_batch_layout(const int32_t* query_lens, const int32_t* context_lens, const int32_t* block_tables, int64_t ld,
                        int num_requests, int width, int page_size, int64_t num_pages, int64_t num_tokens, int32_t* qo_indptr,
@@ -280,6 +280,7 @@ typedef struct sb200_attention_shape {
  * sum_j exp(scale q . k[j]).  Scores, maxima, sums and outputs are fp32 until the one rounding at the end; fp16 / bf16
  * round the probabilities once more, for the second product.  A row that sees no key is zero (lse -inf).  Rows that belong to no
  * request are left as they were, or cleared if zero_rows_behind.  Pages outside [0, num_pages) read as zeros.
+ * out must not overlap q (columns of one buffer may interleave if ldq = ldo) or the cache.
  * workspace (sb200_attention_workspace_bytes): parts of rows whose keys are shared out; written before it is read in every
  * call.  A plan and a workspace serve one call at a time: not two streams at once.  `status` (device word): as sb200_gemm_colpar.
  * Replaces: BatchPrefillWithPagedKVCacheWrapper.plan / run,

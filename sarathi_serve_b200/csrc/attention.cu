@@ -411,6 +411,14 @@ static int attn_workers() {
   return n < kAttnMaxWorkers ? n : kAttnMaxWorkers;
 }
 
+// Do `rows` rows of `row` bytes each, ldx and ldy bytes apart, meet anywhere?  (Columns of one buffer interleave without meeting.)
+static bool rows_meet(const void* x, uint64_t ldx, const void* y, uint64_t ldy, uint64_t rows, uint64_t row) {
+  if (!ranges_meet(x, (rows - 1) * ldx + row, y, (rows - 1) * ldy + row)) return false;
+  if (ldx != ldy || rows == 1) return true;
+  const uint64_t a = reinterpret_cast<uintptr_t>(x), b = reinterpret_cast<uintptr_t>(y), apart = (a < b ? b - a : a - b) % ldx;
+  return apart < row || apart > ldx - row;
+}
+
 static int slot_rows(const AttnShape& sh) { return sh.rows_many > sh.rows_few ? sh.rows_many : sh.rows_few; }
 
 template <typename T>
@@ -483,6 +491,10 @@ extern "C" int sb200_paged_attention(void* out, int64_t ldo, float* lse, const v
   SB_CHECK_ARG(workspace && aligned16(workspace) && workspace_bytes >= sb200_attention_workspace_bytes(shape),
                "paged_attention: the workspace must be 16-byte aligned and hold %lld bytes", (long long)sb200_attention_workspace_bytes(shape));
   SB_CHECK_ARG(isfinite(scale), "paged_attention: the scale is not a finite number");
+  const uint64_t out_bytes = (uint64_t)((num_tokens - 1) * ldo + row) * es;
+  const uint64_t cache_bytes = (uint64_t)num_pages * 2 * sh.page_size * sh.kv_heads * sh.head_dim * es;
+  SB_CHECK_ARG(!rows_meet(q, ldq * es, out, ldo * es, num_tokens, row * es) && !ranges_meet(out, out_bytes, cache, cache_bytes),
+               "paged_attention: out must not overlap q or the cache");
   AttnArgs a = {};
   plan_view(const_cast<void*>(plan), tiles_cap(sh, shape), &a.plan);
   a.q = q; a.ldq = ldq; a.out = out; a.ldo = ldo; a.lse = lse; a.cache = cache;

@@ -228,7 +228,7 @@ batch_layout_kernel(const LayoutArgs a) {
       req = owner_of(rows, a.n, t);
       pos = context(req) + t - rows[req];
       const int page = a.tables[req * a.ld + pos / a.page_size];
-      if (page >= 0 && page < a.num_pages) slot = (int64_t)page * (2 * a.page_size) + pos % a.page_size;
+      if (page >= 0 && page < a.num_pages) slot = (int64_t)page * 2 * a.page_size + pos % a.page_size;
     }
     a.batch_indices[t] = req;
     a.positions[t] = pos;
@@ -249,6 +249,23 @@ batch_layout_kernel(const LayoutArgs a) {
 
 using namespace sb200;
 
+// A range of memory that a call reads or writes.
+struct Range {
+  const void* at;
+  uint64_t bytes;
+};
+
+// Does any of the written ranges meet another one of them, or one of those that are read?
+template <int W, int R> static bool any_meet(const Range (&written)[W], const Range (&read)[R]) {
+  for (int i = 0; i < W; ++i) {
+    for (int j = i + 1; j < W; ++j)
+      if (ranges_meet(written[i].at, written[i].bytes, written[j].at, written[j].bytes)) return true;
+    for (int j = 0; j < R; ++j)
+      if (ranges_meet(written[i].at, written[i].bytes, read[j].at, read[j].bytes)) return true;
+  }
+  return false;
+}
+
 static size_t layout_smem(int n, int arrays) { return (size_t)arrays * (n + 1) * sizeof(int); }
 
 extern "C" int sb200_resize_block_tables(int32_t* block_tables, int64_t ld, int32_t* num_blocks, const int32_t* seq_lens,
@@ -264,6 +281,11 @@ extern "C" int sb200_resize_block_tables(int32_t* block_tables, int64_t ld, int3
   if (num_requests == 0) return SB200_OK;
   SB_CHECK_ARG((block_tables || width == 0) && num_blocks && seq_lens && (free_blocks || capacity == 0) && num_free && granted,
                "resize_block_tables: null pointer");
+  const uint64_t n = num_requests;
+  const Range written[] = {{block_tables, width ? ((n - 1) * ld + width) * 4 : 0}, {num_blocks, n * 4}, {free_blocks, (uint64_t)capacity * 4},
+                           {num_free, 4}, {granted, n * 4}};
+  const Range read[] = {{seq_lens, n * 4}};
+  SB_CHECK_ARG(!any_meet(written, read), "resize_block_tables: the arrays must not overlap");
   TablesArgs a = {block_tables, ld, num_blocks, seq_lens, free_blocks, num_free, granted, num_requests, width, (int)capacity, page_size};
   // Eight CTAs where the tables could hold so many pages that a prompt's worth of them may move in one step.
   const int ctas = (int64_t)num_requests * width > 16384 ? 8 : 1;
@@ -305,6 +327,12 @@ extern "C" int sb200_batch_layout(const int32_t* query_lens, const int32_t* cont
                    (kv_capacity == 0 || kv_indices) && ((int64_t)num_requests * width == 0 || block_tables) &&
                    (num_tokens == 0 || (batch_indices && positions && kv_slots)),
                "batch_layout: null pointer");
+  // (every CTA reads the lengths for itself while others may have written theirs: last step's kv_lens, say, must be copied first)
+  const uint64_t n = num_requests, t = num_tokens;
+  const Range written[] = {{qo_indptr, (n + 1) * 4}, {kv_lens, n * 4}, {kv_indptr, (n + 1) * 4}, {kv_indices, (uint64_t)kv_capacity * 4},
+                           {last_page_len, n * 4}, {batch_indices, t * 4}, {positions, t * 8}, {kv_slots, t * 8}};
+  const Range read[] = {{query_lens, n * 4}, {context_lens, n * 4}, {block_tables, n && width ? ((n - 1) * ld + width) * 4 : 0}};
+  SB_CHECK_ARG(!any_meet(written, read), "batch_layout: the arrays it writes must not overlap each other or those it reads");
   LayoutArgs a = {query_lens, context_lens, block_tables, ld, qo_indptr, kv_lens, kv_indptr, kv_indices, last_page_len, batch_indices,
                   positions, kv_slots, num_requests, width, page_size, (int)num_pages, (int)num_tokens, kv_capacity};
   // One item a thread, up to a CTA per SM: the prefix sums that each CTA makes cost as much as a few items.

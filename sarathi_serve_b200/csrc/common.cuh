@@ -153,6 +153,12 @@ __device__ __forceinline__ float block_sum_once(float v, float* red) {
   return warp_sum(lane < nw ? red[lane] : 0.f);
 }
 
+// Do two ranges of memory meet?  (none: sizes of 0 bytes)
+inline bool ranges_meet(const void* a, uint64_t na, const void* b, uint64_t nb) {
+  const uint64_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return na && nb && x < y + nb && y < x + na;
+}
+
 __host__ __device__ inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 // Number of SMs of the current device (cached per process).

@@ -94,7 +94,7 @@ def resize_block_tables(block_tables: torch.Tensor, num_blocks: torch.Tensor, se
     finished) pushes its last pages on the stack ``free_blocks[:num_free]``; then requests that grow pop theirs from its top,
     in request order.  Returns ``granted`` int32 [n]: 0 where the stack (or the table's width) did not suffice and the request
     was left as it was -- from the first such request on, none that needs pages gets any, unless it was its own table that was
-    too narrow.  A negative length leaves a request alone.  All tensors int32 on the GPU; ``num_free`` has one element."""
+    too narrow.  A negative length leaves a request alone.  All tensors int32 on the GPU, none overlapping another; ``num_free`` has one element."""
     what = "resize_block_tables"
     N.require_current(block_tables, num_blocks, seq_lens, free_blocks, num_free, granted)
     n = num_blocks.numel()
@@ -140,7 +140,7 @@ def batch_layout(query_lens: torch.Tensor, context_lens: torch.Tensor, block_tab
 
     Negative lengths count as zero.  A context is cut to what its block table has room for, and the new tokens to what is then
     left of it and of ``num_tokens``.  ``out``: the result of an earlier call of the same sizes, written again (buffers of a CUDA
-    graph)."""
+    graph); its arrays must not be inputs too (``context_lens=out.kv_lens.clone()`` for the step after)."""
     what = "batch_layout"
     n = query_lens.numel()
     N.require_current(query_lens, context_lens, block_tables)

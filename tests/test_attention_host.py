@@ -64,6 +64,40 @@ def test_calls_that_are_refused():
     assert lay(n=8193, w=0, ld=0) == 2
 
 
+@pytest.mark.skipif(torch.cuda.is_available(), reason="makes calls on addresses that are not device memory")
+def test_arrays_that_overlap_are_refused():
+    """A result on top of its own input would be read by one SM after another has written it."""
+    lib = N.lib()
+    refused = lambda rc: rc == 1 and b"overlap" in lib.sb200_last_error()
+    s = shape()
+    sp, ws = ctypes.byref(s), lib.sb200_attention_workspace_bytes(ctypes.byref(s))
+    page = 2 * 16 * 2 * 128 * 2  # bytes
+    q, cache, far = 1 << 20, 1 << 30, 1 << 40
+    call = lambda out, ldo=1536, T=8: lib.sb200_paged_attention(out, ldo, None, q, 1536, T, cache, 10, 4096, sp, 4096, 10, 0.1, 0, far, ws,
+                                                                None, None)
+    # 8 rows of 1024 elements of 2 bytes, 1536 elements apart
+    for out in (q, q + 16, q + 2032, q - 2032, q + 7 * 3072, q + 3072 - 16, q + 3 * 3072 + 1040):
+        assert refused(call(out)), out
+    assert refused(call(q, T=1)) and refused(call(q + 2032, T=1)) and refused(call(q - 2 * 3072, ldo=2048))
+    for out in (cache, cache + 10 * page - 16, cache - 7 * 3072):
+        assert refused(call(out)), out
+
+    a = [1 << (20 + i) for i in range(11)]
+    tables = lambda t=a[0], nb=a[1], sl=a[2], f=a[3], nf=a[4], g=a[5]: lib.sb200_resize_block_tables(t, 8, nb, sl, f, nf, g, 4, 8, 100, 16, None)
+    for bad in (dict(g=a[1]), dict(g=a[4] - 12), dict(nf=a[3] + 396), dict(sl=a[1] + 8), dict(f=a[0] + 31 * 4), dict(g=a[2])):
+        assert refused(tables(**bad)), bad
+    names = ("query", "context", "table", "qo", "kv", "indptr", "indices", "last", "req", "pos", "slot")
+    good = dict(zip(names, a))
+
+    def lay(**k):
+        x = {**good, **k}
+        return lib.sb200_batch_layout(x["query"], x["context"], x["table"], 8, 4, 8, 16, 10, 8, x["qo"], x["kv"], x["indptr"], x["indices"],
+                                      40, x["last"], x["req"], x["pos"], x["slot"], None)
+    for bad in (dict(context=good["kv"]), dict(query=good["kv"] + 12), dict(context=good["qo"] + 16), dict(table=good["indices"] + 39 * 4),
+                dict(pos=good["slot"] + 56), dict(last=good["kv"]), dict(req=good["pos"] - 28)):
+        assert refused(lay(**bad)), bad
+
+
 def test_wrappers_want_gpu_tensors():
     from sarathi_serve_b200 import kv_cache_ops
     i = lambda *s: torch.zeros(*s, dtype=torch.int32)

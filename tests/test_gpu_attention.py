@@ -263,6 +263,21 @@ def test_rows_behind_the_last_request_and_strides():
         assert (wide[:, 4 * hd:] == 3).all() and (wide[c["total"]:] == 3).all() and (lse[c["total"]:] == 5).all()
 
 
+def test_queries_and_results_in_one_buffer():
+    """Side by side they do not overlap; on top of each other they are refused."""
+    from sarathi_serve_b200 import attention_ops
+    c = make(16, torch.bfloat16, 4, 2, 128, 16, [(150, 30), (1, 200), (9, 0)])
+    plan, _ = plan_of(c)
+    wide = torch.zeros(c["T"], 1024, dtype=torch.bfloat16, device="cuda")
+    wide[:, :512] = c["q"]
+    out = attention_ops.paged_attention(wide[:, :512], c["cache"], plan, 0.1, out=wide[:, 512:])
+    check(c, out, 0.1)
+    assert torch.equal(wide[:, :512], c["q"])
+    for out in (wide[:, :512], wide[:, 256:768], c["cache"].view(-1, 512)[:c["T"]]):
+        with pytest.raises(RuntimeError, match="overlap"):
+            attention_ops.paged_attention(wide[:, :512], c["cache"], plan, 0.1, out=out)
+
+
 def test_lengths_that_the_caller_got_wrong():
     """More new tokens than the cache holds (their first rows see nothing), page ids outside the cache, q with fewer rows
     than planned, a list that ends early: defined results, nothing out of range."""
@@ -438,3 +453,22 @@ def test_resize_block_tables(n, width, page, spare, capacity):
         live = [dev[0][r, :int(dev[1][r])].tolist() for r in range(n)]
         ids = sum(live, []) + dev[3][:int(dev[4])].tolist()
         assert len(set(ids)) == len(ids), "a page has two owners"
+
+
+def test_layout_of_the_next_step():
+    """Last step's lengths are the next step's contexts: as a copy, not in place."""
+    from sarathi_serve_b200 import kv_cache_ops
+    i = lambda x: torch.tensor(x, dtype=torch.int32).cuda()
+    table = torch.arange(40, dtype=torch.int32).view(4, 10).cuda()
+    lay = kv_cache_ops.batch_layout(i([5, 1, 0, 30]), i([0, 9, 3, 40]), table, 8, 40, 40)
+    with pytest.raises(RuntimeError, match="overlap"):
+        kv_cache_ops.batch_layout(i([1, 1, 1, 1]), lay.kv_lens, table, 8, 40, 40, out=lay)
+    kv_cache_ops.batch_layout(i([1, 1, 1, 1]), lay.kv_lens.clone(), table, 8, 40, 40, out=lay)
+    assert lay.kv_lens.tolist() == [6, 11, 4, 71] and lay.positions[:4].tolist() == [5, 10, 3, 70]
+
+
+def test_slots_of_very_large_pages():
+    from sarathi_serve_b200 import kv_cache_ops
+    i = lambda x: torch.tensor(x, dtype=torch.int32).cuda()
+    lay = kv_cache_ops.batch_layout(i([2]), i([5]), i([[3]]), 1 << 30, 4, 3)
+    assert lay.kv_slots.tolist() == [3 * 2 ** 31 + 5, 3 * 2 ** 31 + 6, -1]
