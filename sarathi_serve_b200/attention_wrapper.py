@@ -19,7 +19,7 @@ class PagedAttentionWrapper:
     """Paged caches of ``num_layers`` layers and the plan of the current step.
 
     Everything a step changes lies in buffers of fixed address, sized for ``max_requests`` requests of ``max_blocks`` pages and
-    ``max_tokens`` rows: ``begin_forward`` fills them on the current stream (two launches), and whatever was captured with this
+    ``max_tokens`` rows: ``begin_forward`` fills them on the current stream (copies and two kernels), and whatever was captured with this
     wrapper -- ``graph_runner.LayerGraph``, ``model_runner.ModelGraphRunner`` -- can be replayed after it, for any step of as
     many rows.  One step at a time: replays and ``begin_forward`` belong on one stream."""
 
@@ -52,8 +52,10 @@ class PagedAttentionWrapper:
                       num_tokens: int) -> None:
         """The next step: request r adds ``query_lens[r]`` tokens to the ``context_lens[r]`` it has in the cache, in pages
         ``block_tables[r]``, in a batch padded to ``num_tokens`` rows (of a graph: the rows it was captured with).  int32
-        tensors, on the device or (pinned) on the host, of at most ``max_requests`` requests and ``max_blocks`` pages each; nothing
-        is synchronised."""
+        tensors, on the device or on the host, of at most ``max_requests`` requests and ``max_blocks`` pages each.  Nothing is
+        synchronised: pinned host tensors are read when the stream gets there, so they keep their values until then.  A request
+        whose length reaches behind its pages sees zeros there and stores nothing; tokens behind row ``num_tokens`` are no part
+        of the step's results."""
         if not 0 <= num_tokens <= self.max_tokens:
             raise RuntimeError(f"begin_forward: {num_tokens} rows, made for at most {self.max_tokens}")
         n = query_lens.numel()
@@ -68,7 +70,10 @@ class PagedAttentionWrapper:
         N.require_current(self.query_lens)
         self.query_lens[:n].copy_(query_lens.reshape(-1), non_blocking=True)
         self.context_lens[:n].copy_(context_lens.reshape(-1), non_blocking=True)
-        self.block_tables[:n, :block_tables.shape[1]].copy_(block_tables, non_blocking=True)
+        width = block_tables.shape[1]
+        self.block_tables[:n, :width].copy_(block_tables, non_blocking=True)
+        if width < self.max_blocks:  # what the step before left there is no page of this one
+            self.block_tables[:n, width:].fill_(-1)
         if n < self.max_requests:
             self.query_lens[n:].zero_()
             self.context_lens[n:].zero_()

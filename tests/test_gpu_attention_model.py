@@ -194,6 +194,32 @@ def test_two_plans_on_two_streams():
         assert all(torch.equal(o, want) for o in outs[i])
 
 
+def test_a_step_with_fewer_pages_than_the_one_before():
+    """Block tables that get narrower leave nothing behind: what a request is short of are zeros, not the pages of another."""
+    from sarathi_serve_b200.attention_wrapper import PagedAttentionWrapper
+    w = PagedAttentionWrapper(4, 2, 64, 16, 10, 1, torch.float16, max_requests=2, max_tokens=8, max_blocks=4)
+    i = lambda x: torch.tensor(x, dtype=torch.int32)
+    g = torch.Generator().manual_seed(8)
+    w.kv_caches[0].copy_(torch.randn(w.kv_caches[0].shape, generator=g))
+    w.begin_forward(i([1, 1]), i([60, 50]), i([[1, 2, 3, 4], [5, 6, 7, 8]]), 8)
+    assert w.layout.kv_slots.tolist() == [4 * 32 + 12, 8 * 32 + 2] + [-1] * 6
+    w.begin_forward(i([1, 1]), i([20, 50]), i([[1, 2], [5, 6]]), 8)  # the second has 51 tokens, and pages for 32
+    assert w.layout.kv_slots.tolist() == [2 * 32 + 4] + [-1] * 7
+    cache = w.kv_caches[0].clone()
+    q = torch.randn(8, 4 * 64, generator=g).half().cuda()
+    got = w.forward(q, torch.ones(8, 128, dtype=torch.float16, device="cuda"), torch.ones(8, 128, dtype=torch.float16, device="cuda"), 0, 0.1)
+    assert torch.equal(w.kv_caches[0][7:], cache[7:]) and torch.equal(w.kv_caches[0][5:7], cache[5:7])
+    keys = torch.cat([cache[5:7].transpose(0, 1).reshape(2, 32, 2, 64), torch.zeros(2, 19, 2, 64, dtype=torch.float16, device="cuda")], 1).double()
+    k, v = keys.repeat_interleave(2, dim=2)
+    q1 = q[1].double().view(4, 64)
+    p = torch.softmax(0.1 * torch.einsum("hd,khd->hk", q1, k), -1)
+    want, W = torch.einsum("hk,khd->hd", p, v).reshape(-1), torch.einsum("hk,khd->hd", p, v.abs()).reshape(-1)
+    # roundings of the result and the probabilities; scores, powers of two and sums in fp32; probabilities below fp16's smallest step
+    A = 0.1 * torch.einsum("hd,khd->hk", q1.abs(), k.abs()).max()
+    tol = 2.0 ** -11 * (want.abs() + W) + 2 * ((80 * A + 67) * 2.0 ** -24 + 2.0 ** -21) * W + 51 * 2.0 ** -25 * v.abs().max()
+    assert ((got[1].double() - want).abs() <= tol).all()
+
+
 def test_wrapper_refusals():
     from sarathi_serve_b200 import attention_ops, kv_cache_ops
     from sarathi_serve_b200.attention_wrapper import PagedAttentionWrapper
