@@ -21,7 +21,8 @@ class AttentionPlan:
 
     ``num_heads`` / ``num_kv_heads``: of this rank; ``window``: a token sees itself and the ``window - 1`` tokens before it (0:
     all of them).  ``max_requests`` and ``max_tokens`` bound the steps the plan is updated with.  A plan serves one step at a
-    time: its calls belong on one stream (or ordered by events), and so do the graphs that captured them.  A graph keeps reading
+    time: a call on another stream than the one before waits for that one, and the graphs that captured such calls belong on one
+    stream (or ordered by events).  A graph keeps reading
     the ``kv_indices`` that the plan had when it was captured: write later steps' layouts to the same arrays
     (``batch_layout(..., out=)``)."""
 
@@ -44,6 +45,23 @@ class AttentionPlan:
         self.buffer = torch.empty(plan_bytes, dtype=torch.uint8, device=device)
         self.workspace = torch.empty(lib.sb200_attention_workspace_bytes(self._shape), dtype=torch.uint8, device=device)
         self.kv_indices: Optional[torch.Tensor] = None
+        self._stream: Optional[torch.cuda.Stream] = None
+        self._stream_ptr: Optional[int] = None
+
+    def stream(self) -> Optional[int]:
+        """The current stream, behind whatever the plan's calls have queued on the one they used last.  (A kernel that read a plan
+        that is still being written would follow numbers that mean nothing.)  Not while a graph is captured: its replays are the
+        caller's to order."""
+        here = N.stream_ptr()
+        if here != self._stream_ptr and not torch.cuda.is_current_stream_capturing():
+            now = torch.cuda.current_stream()
+            if self._stream is not None:
+                now.wait_stream(self._stream)
+                for t in (self.buffer, self.workspace, self.kv_indices):
+                    if t is not None:
+                        t.record_stream(now)
+            self._stream, self._stream_ptr = now, here
+        return here
 
     def update(self, layout: Optional[BatchLayout] = None, *, qo_indptr: Optional[torch.Tensor] = None,
                kv_lens: Optional[torch.Tensor] = None, kv_indptr: Optional[torch.Tensor] = None,
@@ -60,7 +78,7 @@ class AttentionPlan:
                            ("kv_indices", kv_indices, -1)):
             _int32(name, t, k, "AttentionPlan.update")
         N.check(N.lib().sb200_attention_plan(self.buffer.data_ptr(), self.buffer.numel(), self._shape, qo_indptr.data_ptr(),
-                                             kv_lens.data_ptr(), kv_indptr.data_ptr(), n, kv_indices.numel(), N.stream_ptr()),
+                                             kv_lens.data_ptr(), kv_indptr.data_ptr(), n, kv_indices.numel(), self.stream()),
                 "attention_plan")
         self.kv_indices = kv_indices
         return self
@@ -100,5 +118,5 @@ def paged_attention(q: torch.Tensor, paged_kv_cache: torch.Tensor, plan: Attenti
                                           q2.stride(0) if T > 1 else row, T, paged_kv_cache.data_ptr(), paged_kv_cache.shape[0],
                                           plan.buffer.data_ptr(), plan._shape, kv.data_ptr(), kv.numel(), scale, 1 if clear else 0,
                                           plan.workspace.data_ptr(), plan.workspace.numel(),
-                                          dense_ops.status_word(q.device).data_ptr(), N.stream_ptr()), "paged_attention")
+                                          dense_ops.status_word(q.device).data_ptr(), plan.stream()), "paged_attention")
     return out

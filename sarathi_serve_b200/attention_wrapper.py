@@ -68,6 +68,7 @@ class PagedAttentionWrapper:
             if t.dtype != torch.int32:
                 raise RuntimeError("begin_forward: query_lens, context_lens and block_tables must be int32")
         N.require_current(self.query_lens)
+        self.plan.stream()
         self.query_lens[:n].copy_(query_lens.reshape(-1), non_blocking=True)
         self.context_lens[:n].copy_(context_lens.reshape(-1), non_blocking=True)
         width = block_tables.shape[1]
@@ -91,6 +92,7 @@ class PagedAttentionWrapper:
 
     def fused_kv_append(self, layer_cache_idx: int):
         """(paged cache, slots) for the qkv projection's epilogue: the layer stores its own keys and values."""
+        self.plan.stream()
         self._appended = layer_cache_idx
         return self.kv_caches[layer_cache_idx], self.layout.kv_slots[:self.num_tokens]
 
@@ -101,6 +103,7 @@ class PagedAttentionWrapper:
         if T > self.max_tokens:
             raise RuntimeError(f"PagedAttentionWrapper: {T} rows, made for at most {self.max_tokens}")
         cache = self.kv_caches[layer_cache_idx]
+        self.plan.stream()
         if self._appended != layer_cache_idx:
             kv_cache_ops.append_rows(cache, key, value, self.layout.kv_slots[:T])
         self._appended = None

@@ -194,6 +194,47 @@ def test_two_plans_on_two_streams():
         assert all(torch.equal(o, want) for o in outs[i])
 
 
+def test_a_plan_used_on_another_stream_than_it_was_made_on():
+    """The plan, and the wrapper's index arrays, are still being written when the other stream's call is issued: it waits."""
+    from sarathi_serve_b200 import attention_ops, kv_cache_ops
+    from sarathi_serve_b200.attention_wrapper import PagedAttentionWrapper
+    i = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    w = PagedAttentionWrapper(8, 2, 128, 16, 64, 1, torch.bfloat16, max_requests=3, max_tokens=128, max_blocks=20)
+    g = torch.Generator().manual_seed(2)
+    cache = torch.randn(w.kv_caches[0].shape, generator=g).bfloat16().cuda()
+    q, k, v = (torch.randn(128, n, generator=g).bfloat16().cuda() for n in (1024, 256, 256))
+    table = torch.arange(60, dtype=torch.int32, device="cuda").view(3, 20)
+    steps = [(i([100, 1, 3]), i([20, 300, 0]), table), (i([1, 1, 90]), i([120, 7, 200]), table.flip(0).contiguous())]
+    want = []
+    for s in steps:
+        w.kv_caches[0].copy_(cache)
+        w.begin_forward(*s, 128)
+        want.append(w.forward(q, k, v, 0, 0.1))
+    w.kv_caches[0].copy_(cache)
+    other = torch.cuda.Stream()
+    a, b = torch.randn(2, 4096, 4096, device="cuda")
+    torch.cuda.synchronize()
+    for s, x in zip(steps, want):
+        for _ in range(20):
+            a = torch.tanh(a @ b)  # some milliseconds on the current stream
+        w.begin_forward(*s, 128)
+        with torch.cuda.stream(other):
+            got = w.forward(q, k, v, 0, 0.1)
+            w.kv_caches[0].copy_(cache)
+            assert torch.equal(got, x)
+    lay = kv_cache_ops.batch_layout(*steps[0], 16, 64, 128)
+    plan = attention_ops.AttentionPlan(8, 2, 128, 16, torch.bfloat16, 3, 128)
+    torch.cuda.synchronize()
+    for _ in range(20):
+        a = torch.tanh(a @ b)
+    plan.update(lay)
+    with torch.cuda.stream(other):
+        got = attention_ops.paged_attention(q, cache, plan, 0.1)
+    plan.update(kv_cache_ops.batch_layout(*steps[1], 16, 64, 128))  # (back again: behind that call)
+    torch.cuda.synchronize()
+    assert torch.equal(got, attention_ops.paged_attention(q, cache, plan.update(lay), 0.1))
+
+
 def test_a_step_with_fewer_pages_than_the_one_before():
     """Block tables that get narrower leave nothing behind: what a request is short of are zeros, not the pages of another."""
     from sarathi_serve_b200.attention_wrapper import PagedAttentionWrapper
