@@ -73,13 +73,13 @@ def test_arrays_that_overlap_are_refused():
     sp, ws = ctypes.byref(s), lib.sb200_attention_workspace_bytes(ctypes.byref(s))
     page = 2 * 16 * 2 * 128 * 2  # bytes
     q, cache, far = 1 << 20, 1 << 30, 1 << 40
-    call = lambda out, ldo=1536, T=8: lib.sb200_paged_attention(out, ldo, None, q, 1536, T, cache, 10, 4096, sp, 4096, 10, 0.1, 0, far, ws,
+    call = lambda out, ldo=1280, T=8: lib.sb200_paged_attention(out, ldo, None, q, 1280, T, cache, 10, 4096, sp, 4096, 10, 0.1, 0, far, ws,
                                                                 None, None)
-    # 8 rows of 1024 elements of 2 bytes, 1536 elements apart
-    for out in (q, q + 16, q + 2032, q - 2032, q + 7 * 3072, q + 3072 - 16, q + 3 * 3072 + 1040):
+    # 8 rows of 1024 elements of 2 bytes, 1280 elements apart
+    for out in (q, q + 16, q + 2032, q - 2032, q + 7 * 2560, q + 2560 - 16, q + 3 * 2560 + 1040):
         assert refused(call(out)), out
-    assert refused(call(q, T=1)) and refused(call(q + 2032, T=1)) and refused(call(q - 2 * 3072, ldo=2048))
-    for out in (cache, cache + 10 * page - 16, cache - 7 * 3072):
+    assert refused(call(q, T=1)) and refused(call(q + 2032, T=1)) and refused(call(q - 2 * 2560, ldo=2048))
+    for out in (cache, cache + 10 * page - 16, cache - 7 * 2560):
         assert refused(call(out)), out
 
     a = [1 << (20 + i) for i in range(11)]
