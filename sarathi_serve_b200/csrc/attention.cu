@@ -20,27 +20,28 @@ struct PlanArgs {
   AttnShape sh;
 };
 
-// What a block of keys, and a unit apart from its blocks, costs a CTA, in tenths of a microsecond, and the least blocks of a
-// piece.  Measured with every SM at the same kind: units of 1 to 64 blocks, and several of them one after the other.  Few rows
-// count at the share of HBM that an SM has when all of them stream.
+// What a block of keys, and a unit apart from its blocks, costs a CTA, in hundredths of a microsecond, and the least blocks of a
+// piece.  Fitted to when the CTAs ended in 17 steps, most of them mixed, their keys in HBM: 0.2 us a block more for many rows than where
+// every SM does them, a window's masks at both ends 2 us a unit.  Few rows count at the share of HBM that an SM has when all of them
+// stream.
 __device__ __forceinline__ void unit_cost(const AttnShape& sh, int kind, int nrows, int* block, int* fixed, int* least) {
   const bool wide = sh.head_dim > 64;
   if (sh.dtype == SB200_F32) {
-    *block = (kind == ATTN_MANY ? 130 : 15) * sh.head_dim / 64;
-    *fixed = 20;
+    *block = (kind == ATTN_MANY ? 1300 : 150) * sh.head_dim / 64;
+    *fixed = 200;
     *least = 1;
   } else if (kind == ATTN_MANY) {
-    *block = nrows > 128 ? (wide ? 17 : 15) : (wide ? 15 : 14);
-    *fixed = 45;
+    *block = nrows > 128 ? (wide ? 192 : 170) : (wide ? 170 : 150);
+    *fixed = (wide ? 508 : 480) + (sh.window > 0 ? 200 : 0);
     *least = 2;
   } else {
-    *block = sh.head_dim == 256 ? 30 : wide ? 15 : 10;
-    *fixed = 22;
+    *block = sh.head_dim == 256 ? 300 : wide ? 150 : 100;
+    *fixed = wide ? 260 : 220;
     *least = 2;
   }
 }
 
-constexpr long long kShareMany = 20, kShareFew = 15, kJoinMany = 50, kJoinFew = 25;
+constexpr long long kShareMany = 200, kShareFew = 150, kJoinMany = 500, kJoinFew = 250;
 
 __device__ __forceinline__ long long scan_block(long long v, long long* red, long long* total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -160,7 +161,7 @@ attn_plan_kernel(const PlanArgs a) {
   __shared__ int4 at[kAttnMaxWorkers + 1];
   if (threadIdx.x == 0) a.plan.cost[tiles] = carry;
   __syncthreads();
-  // No more workers than have a share worth starting for (in tenths of a microsecond, as unit_cost): a piece more is a start, a
+  // No more workers than have a share worth starting for (in hundredths of a microsecond, as unit_cost): a piece more is a start, a
   // store of its part and a load in the join.
   const long long busy = max(1ll, min((long long)a.workers, carry / (tiles_many ? kShareMany : kShareFew)));
   // No more units than workers: every unit can have workers of its own, each with one piece of it.  That saves a worker the second
@@ -210,10 +211,23 @@ attn_plan_kernel(const PlanArgs a) {
       for (int w = (int)total + threadIdx.x; w <= a.workers; w += kPlanThreads) at[w] = make_int4(tiles, 0, 0, 0);
     }
   }
+  // A share that begins inside a unit has a start more than the line says, a dearer one among the units of many rows: the workers
+  // that do those get as much less to do.  (In units of 1/1024 worker.  512 rows with 64 decodes of 512 to 8192 tokens: the last
+  // worker done after 221 us, half of them after 182, without this and with the costs of a step of many rows only.)
+  const long long line_many = tiles_many < tiles ? a.plan.cost[tiles_many] : carry, line_few = carry - line_many;
+  long long workers_many = 0;
+  if (line_many > 0) {
+    int block, fixed_many, fixed_few, least;
+    unit_cost(sh, ATTN_MANY, sh.rows_many, &block, &fixed_many, &least);
+    unit_cost(sh, ATTN_FEW, sh.rows_few, &block, &fixed_few, &least);
+    const long long equal = carry / busy, own = max(equal - line_few * max(0, fixed_many - fixed_few) / carry, equal / 2 + 1);
+    workers_many = line_few == 0 ? busy * 1024 : min(line_many * 1024 / own, busy * 1024 - 1);
+  }
   for (int w = aligned ? a.workers + 1 : (int)threadIdx.x; w <= a.workers; w += kPlanThreads) {
     int4 out = make_int4(tiles, 0, 0, 0);
     if (w < busy && tiles > 0) {
-      const long long x = carry * w / busy;
+      const long long x = w * 1024 <= workers_many ? line_many * (w * 1024) / max(workers_many, 1ll)
+                                                   : line_many + line_few * (w * 1024 - workers_many) / (busy * 1024 - workers_many);
       int lo = 0, hi = tiles - 1;
       while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
