@@ -686,8 +686,8 @@ __device__ __forceinline__ void many_softmax(const AttnArgs& a, uint8_t* smem, M
     int token, head, pos;
     attn_row(a, p, min(r, max(p.t.nrows - 1, 0)), &token, &head, &pos);
     float m = -INFINITY, l = 0.f;
-    // keys that all rows of this half see need no mask
-    const int pos_first = p.t.pos0 + a.by_group.div(p.t.row0 + sub * 128), pos_last = p.hi - 1;
+    // the warp's first and last position: keys that all of its rows see need no mask
+    const int pos_warp_lo = __shfl_sync(0xffffffffu, pos, 0), pos_warp_hi = __shfl_sync(0xffffffffu, pos, 31);
     for (int b = p.b0; b < p.b1; ++b) {
       ptx::mbar_wait_lanes(&sy.turn[sub], phase, abort_flag);
       phase ^= 1u;
@@ -699,17 +699,24 @@ __device__ __forceinline__ void many_softmax(const AttnArgs& a, uint8_t* smem, M
         for (int i = 0; i < 128; ++i) raw[i] = __float_as_uint(__uint_as_float(raw[i]) * (a.scale_log2 < 0.f ? -1.f : 0.f));
       }
       const int key = (p.t.blk_lo + b) * kAttnBlock;
-      if (!(key + kAttnBlock - 1 <= pos_first && (a.window == 0 || key > pos_last - a.window))) {
+      // (32 keys at a time, and none that all rows of the warp see.  Chunks of 500 and 100 decodes, heads of 64, window 1000: 69.6 -> 65.5 us)
+      if (key + kAttnBlock - 1 > pos_warp_lo) {
         const int hi = pos - key;
 #pragma unroll
-        for (int i = 0; i < 128; ++i)
-          if (i > hi) raw[i] = 0xff800000u;
-        if (a.window > 0) {
-          const int lo = hi - a.window;
+        for (int c = 0; c < 128; c += 32)
+          if (key + c + 31 > pos_warp_lo)
 #pragma unroll
-          for (int i = 0; i < 128; ++i)
-            if (i <= lo) raw[i] = 0xff800000u;
-        }
+            for (int i = c; i < c + 32; ++i)
+              if (i > hi) raw[i] = 0xff800000u;
+      }
+      if (a.window > 0 && key <= pos_warp_hi - a.window) {
+        const int lo = pos - a.window - key;
+#pragma unroll
+        for (int c = 0; c < 128; c += 32)
+          if (key + c <= pos_warp_hi - a.window)
+#pragma unroll
+            for (int i = c; i < c + 32; ++i)
+              if (i <= lo) raw[i] = 0xff800000u;
       }
       // The probabilities of the first 64 keys are made with the maximum as it stands while the block's own is being found, and made
       // again in the rare case that it has grown too far.  (The maximum first, then the exponentials: 250 clocks of 2900 a block more.)
