@@ -8,7 +8,8 @@
 // Few rows (a request of up to 8 rows, 4 a unit): bound by HBM.  As in attention_tc.cu the eight warps stream keys in turn, each
 // through a ring of its own that asynchronous copies fill; a key belongs to HD / 8 lanes, which hold 8 columns of queries and
 // outputs of all four rows in registers, so that a warp works on 1 to 4 keys at a time and reads each byte once.
-// (32 decodes of 256 to 2048 tokens and a chunk of 256, heads of 64: 250 us with tiles of 32 rows only.)
+// (32 decodes of 256 to 2048 tokens and a chunk of 256, heads of 64: 39 us, with tiles of 32 rows only 250.  What bounds it now are the
+// chunk's tiles: 6.5 us for 64 rows and 64 keys, a third of the FMA rate.)
 #include "attention.cuh"
 
 namespace sb200 {

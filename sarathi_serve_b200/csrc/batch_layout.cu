@@ -6,9 +6,9 @@
 // sequences in Python every step.
 //
 // Both kernels are bound by latency (their floor is well below a microsecond for a step of a few hundred requests; the layout
-// of 212 requests with 1997 tokens takes 5.6 us), so each is ONE launch: every CTA computes the prefix sums over the requests for itself, into shared memory, and the items (pages,
-// tokens) are then dealt out flat -- an item finds its request by binary search -- so that one request with thousands of
-// pages takes no longer than thousands of requests with one.
+// of 212 requests with 1997 tokens takes 5.6 us), so each is ONE launch: every CTA computes the prefix sums over the requests for
+// itself, into shared memory, and the items (pages, tokens) are then dealt out flat -- an item finds its request by binary search --
+// so that one request with thousands of pages takes no longer than thousands of requests with one.
 #include "common.cuh"
 #include "sm100_ptx.cuh"
 
