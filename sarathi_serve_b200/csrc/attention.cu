@@ -289,15 +289,34 @@ attn_plan_kernel(const PlanArgs a) {
 // rows, which is how the slots are laid out.  Also clears the rows of q that belong to no request, when asked to.  Bound by
 // latency: the groups' prefix sums, the unit and its pieces (sums and outputs of four at a time) are three loads after one another:
 // 2 to 4 us for decodes, 20 with a cut unit of 256 rows on every SM.
+// What it reads of the plan it reads ahead of its wait: the attention kernel lets it start only when its own wait is over, and the plan
+// was complete then.
 template <typename T, int HD>
 __global__ void __launch_bounds__(kJoinThreads, 5)
 attn_join_kernel(const AttnArgs a) {
-  grid_dependency_begin();
   constexpr int kRows = kJoinValues / HD, kBatch = 4;
   __shared__ int first[kAttnMaxWorkers + 1];
   T* out = reinterpret_cast<T*>(a.out);
-  const int units = a.plan.starts[0].units;
-  for (int i = threadIdx.x; i <= a.workers; i += kJoinThreads) first[i] = a.plan.cut_first[i];  // (behind `units`: anything)
+  const int units = __ldcg(&a.plan.starts[0].units);
+  for (int i = threadIdx.x; i <= a.workers; i += kJoinThreads) first[i] = __ldcg(a.plan.cut_first + i);  // (behind `units`: anything)
+  __syncthreads();
+  const int groups = first[units];
+  int lo = 0;
+  int4 u, v;  // the cut unit of group g
+  auto look_up = [&](int g) {
+    int hi = units - 1;
+    lo = 0;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (first[mid] <= g) lo = mid;
+      else hi = mid - 1;
+    }
+    const int4* rec = reinterpret_cast<const int4*>(a.plan.cuts + lo);
+    u = __ldcg(rec);
+    v = __ldcg(rec + 1);
+  };
+  if ((int)blockIdx.x < groups) look_up(blockIdx.x);
+  grid_dependency_begin();
   if (a.zero_behind) {
     const int rows0 = min(a.plan.starts[0].rows, a.num_tokens), per_row = a.kv_heads * a.group * HD;
     for (int t = rows0 + blockIdx.x; t < a.num_tokens; t += gridDim.x) {
@@ -307,17 +326,8 @@ attn_join_kernel(const AttnArgs a) {
           a.lse[(int64_t)t * (a.kv_heads * a.group) + i] = -INFINITY;
     }
   }
-  __syncthreads();
-  const int groups = first[units];
   for (int g = blockIdx.x; g < groups; g += gridDim.x) {
-    int lo = 0, hi = units - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (first[mid] <= g) lo = mid;
-      else hi = mid - 1;
-    }
-    const int4* rec = reinterpret_cast<const int4*>(a.plan.cuts + lo);
-    const int4 u = rec[0], v = rec[1];
+    if (g != (int)blockIdx.x) look_up(g);
     const AttnCut c = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
     const int r = (g - first[lo]) * kRows + threadIdx.x % kRows, col4 = threadIdx.x / kRows;
     if (r >= min(c.nrows, max(0, (a.num_tokens - c.q_row) * a.group - c.row0))) continue;
@@ -439,9 +449,8 @@ static int slot_rows(const AttnShape& sh) { return sh.rows_many > sh.rows_few ? 
 
 template <typename T>
 static cudaError_t launch_join(int head_dim, const AttnArgs& a, dim3 grid, cudaStream_t s) {
-  if (head_dim == 64) return launch_dependent(attn_join_kernel<T, 64>, grid, dim3(kJoinThreads), 0, s, a);
-  if (head_dim == 128) return launch_dependent(attn_join_kernel<T, 128>, grid, dim3(kJoinThreads), 0, s, a);
-  return launch_dependent(attn_join_kernel<T, 256>, grid, dim3(kJoinThreads), 0, s, a);
+  auto kern = head_dim == 64 ? attn_join_kernel<T, 64> : head_dim == 128 ? attn_join_kernel<T, 128> : attn_join_kernel<T, 256>;
+  return launch_dependent(kern, grid, dim3(kJoinThreads), 0, s, a);
 }
 
 }  // namespace sb200

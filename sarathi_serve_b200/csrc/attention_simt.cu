@@ -393,7 +393,8 @@ __device__ void simt_few(const AttnArgs& a, float* smem, const AttnWalk& walk) {
 template <int HD>
 __global__ void __launch_bounds__(kSimtThreads, 1)
 attn_simt_kernel(const __grid_constant__ AttnArgs a) {
-  grid_dependency_begin();
+  ptx::grid_dependency_wait();
+  ptx::grid_launch_dependents();  // (the join reads the plan at once)
   extern __shared__ float smem_f[];
   if ((int)blockIdx.x >= a.workers) return;
   AttnWalk walk(a, blockIdx.x), few = walk;
@@ -408,7 +409,8 @@ template <int HD>
 static int launch_simt(const AttnArgs& a, int workers, cudaStream_t s) {
   static std::atomic<uint64_t> allowed{0};
   SB_CUDA(allow_smem(reinterpret_cast<const void*>(attn_simt_kernel<HD>), (int)simt_smem<HD>(), &allowed));
-  SB_CUDA(launch_dependent(attn_simt_kernel<HD>, dim3((unsigned)workers), dim3(kSimtThreads), simt_smem<HD>(), s, a));
+  auto kern = attn_simt_kernel<HD>;  // (waits for its predecessor by hand)
+  SB_CUDA(launch_dependent(kern, dim3((unsigned)workers), dim3(kSimtThreads), simt_smem<HD>(), s, a));
   return SB200_OK;
 }
 

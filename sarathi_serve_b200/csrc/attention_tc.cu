@@ -909,8 +909,8 @@ attn_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUten
     ptx::tc_fence_before();
     __syncthreads();
     ptx::tc_fence_after();
-    ptx::grid_launch_dependents();  // the TMEM is ours
     ptx::grid_dependency_wait();
+    ptx::grid_launch_dependents();  // (the TMEM is ours, and the plan that the join reads at once is complete)
     AttnWalk walk(a, blockIdx.x);
     walk.only_many();
     const bool many = walk.more();  // the same for the whole CTA
