@@ -72,14 +72,15 @@ def append_paged_kv_cache(append_key: torch.Tensor, append_value: torch.Tensor, 
 
 
 def _int32(name: str, t: torch.Tensor, n: int, what: str) -> None:
-    if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous() or (n >= 0 and t.numel() != n):
+    if t.dtype is not torch.int32 or t.dim() != 1 or not t.is_contiguous() or (n >= 0 and t.numel() != n):
         raise RuntimeError(f"{what}: {name} must be a contiguous int32 tensor" + (f" of {n} elements" if n >= 0 else ""))
 
 
 def _tables(block_tables: torch.Tensor, n: int, what: str) -> None:
-    if block_tables.dtype != torch.int32 or block_tables.dim() != 2 or block_tables.shape[0] != n:
+    if block_tables.dtype is not torch.int32 or block_tables.dim() != 2 or block_tables.size(0) != n:
         raise RuntimeError(f"{what}: block_tables must be an int32 tensor [{n}, blocks]")
-    if (block_tables.shape[1] > 1 and block_tables.stride(1) != 1) or (n > 1 and block_tables.stride(0) < block_tables.shape[1]):
+    width = block_tables.size(1)
+    if (width > 1 and block_tables.stride(1) != 1) or (n > 1 and block_tables.stride(0) < width):
         raise RuntimeError(f"{what}: the rows of block_tables must have unit inner stride and must not overlap")
 
 
@@ -155,13 +156,10 @@ def batch_layout(query_lens: torch.Tensor, context_lens: torch.Tensor, block_tab
         # one allocation each for the two types; the parts of either one after the other
         parts = [n + 1, n, n + 1, n * width, n, T]
         ints = torch.empty(sum(parts), dtype=torch.int32, device=dev)
-        longs = torch.empty(2, T, dtype=torch.int64, device=dev)
-        out = BatchLayout(*torch.split_with_sizes(ints, parts), *longs.unbind(0))
-        at, pointers = ints.data_ptr(), []
-        for k in parts:
-            pointers.append(at)
-            at += 4 * k
-        out._for = (sizes, (*pointers, longs.data_ptr(), longs.data_ptr() + 8 * T), parts[3])
+        longs = torch.empty(2 * T, dtype=torch.int64, device=dev)
+        # ("unsafe": without the bookkeeping of autograd for views, which integers have no use for)
+        out = BatchLayout(*torch.unsafe_split_with_sizes(ints, parts), *torch.unsafe_split_with_sizes(longs, [T, T]))
+        out._for = (sizes, tuple(map(torch.Tensor.data_ptr, out)), n * width)
     elif getattr(out, "_for", None) is None or out._for[0] != sizes or out._for[1][0] != out[0].data_ptr():
         N.require_current(*out)
         for name, t, k in zip(BatchLayout._fields, out, (n + 1, n, n + 1, -1, n, T)):
@@ -171,7 +169,7 @@ def batch_layout(query_lens: torch.Tensor, context_lens: torch.Tensor, block_tab
         for t in out[6:]:
             if t.dtype != torch.int64 or t.shape != (T,) or not t.is_contiguous():
                 raise RuntimeError(f"{what}: out.positions and out.kv_slots must be contiguous int64 tensors of {T} elements")
-        out._for = (sizes, tuple(t.data_ptr() for t in out), out.kv_indices.numel())
+        out._for = (sizes, tuple(map(torch.Tensor.data_ptr, out)), out.kv_indices.numel())
     _, (qo, kv, indptr, indices, last, req, pos, slot), capacity = out._for
     N.check(N.lib().sb200_batch_layout(query_lens.data_ptr(), context_lens.data_ptr(), block_tables.data_ptr(), _table_stride(block_tables),
                                        n, width, int(page_size), int(num_pages), T, qo, kv, indptr, indices, capacity, last, req, pos,
