@@ -90,34 +90,57 @@ __device__ void simt_many(const AttnArgs& a, float* smem, AttnWalk walk) {
       for (int i = 0; i < CT; ++i) acc[j][i] = make_float4(0.f, 0.f, 0.f, 0.f);
     }
     const int pos_first = p.t.pos0 + a.by_group.div(p.t.row0), pos_last = p.hi - 1;
+    const int warp_lo = __shfl_sync(0xffffffffu, pos[0], 0), warp_hi = __shfl_sync(0xffffffffu, pos[3], 31);  // of the warp's rows
     const int k0 = max(p.lo, (p.t.blk_lo + p.b0) * kAttnBlock) & ~(M::KEYS - 1), k1 = min(p.hi, (p.t.blk_lo + p.b1) * kAttnBlock);
-    float4 next_k[PER], next_v[PER];  // this thread's share of the next step
-    auto ask = [&](int kb) {
+    // Lane l knows the pages of keys l, l + 32 of the step after the next, so that the loads of the next one (this thread's share:
+    // next_k, next_v; real: whether its i-th row is one) wait for nothing.
+    AttnAhead ahead[M::KEYS / 32];
+    float4 next_k[PER], next_v[PER];
+    uint32_t real = 0;
+    auto look_up = [&](int kb) {
 #pragma unroll
-      for (int i = 0; i < PER; ++i) {
-        const int j = i * kSimtThreads + tid, r = j / VPR, v = j - r * VPR, key = kb + r;
-        const int at = key >= p.lo && key < p.hi ? attn_key_row(a, p.t.page_at, key) : -1;
-        next_k[i] = next_v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (at >= 0) {
-          const float* src = cache + (int64_t)at * ldc + p.head * HD + v * 4;
-          next_k[i] = *reinterpret_cast<const float4*>(src);
-          next_v[i] = *reinterpret_cast<const float4*>(src + a.page_size * ldc);
-        }
+      for (int h = 0; h < M::KEYS / 32; ++h) {
+        const int key = kb + h * 32 + (tid & 31);
+        ahead[h].ask(a, p.t.page_at, key, key >= p.lo && key < k1);
       }
     };
-    if (k0 < k1) ask(k0);
+    auto ask = [&]() {
+      int rows[M::KEYS / 32];
+#pragma unroll
+      for (int h = 0; h < M::KEYS / 32; ++h) rows[h] = ahead[h].row(a);
+      real = 0;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const int j = i * kSimtThreads + tid, r = j / VPR, v = j - r * VPR;
+        static_assert(32 % (kSimtThreads / VPR) == 0, "the rows of one i are in one half");
+        const int at = __shfl_sync(0xffffffffu, rows[i * (kSimtThreads / VPR) / 32], r & 31);
+        if (at >= 0) real |= 1u << i;
+        const float* src = cache + (int64_t)max(at, 0) * ldc + p.head * HD + v * 4;
+        next_k[i] = *reinterpret_cast<const float4*>(src);
+        next_v[i] = *reinterpret_cast<const float4*>(src + a.page_size * ldc);
+      }
+    };
+    if (k0 < k1) {
+      look_up(k0);
+      ask();
+      look_up(k0 + M::KEYS);
+    }
     for (int kb = k0; kb < k1; kb += M::KEYS) {
       __syncthreads();
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
         const int j = i * kSimtThreads + tid, r = j / VPR, v = j - r * VPR;
-        *reinterpret_cast<float4*>(sk + r * M::LD + v * 4) = next_k[i];
-        *reinterpret_cast<float4*>(sv + r * HD + v * 4) = next_v[i];
+        const float4 none = make_float4(0.f, 0.f, 0.f, 0.f);
+        *reinterpret_cast<float4*>(sk + r * M::LD + v * 4) = (real >> i) & 1u ? next_k[i] : none;
+        *reinterpret_cast<float4*>(sv + r * HD + v * 4) = (real >> i) & 1u ? next_v[i] : none;
       }
       __syncthreads();
-      if (kb + M::KEYS < k1) ask(kb + M::KEYS);
+      if (kb + M::KEYS < k1) {
+        ask();
+        look_up(kb + 2 * M::KEYS);
+      }
       float s[4][KT] = {};
-#pragma unroll 2
+#pragma unroll 4
       for (int c = 0; c < HD; c += 4) {
         float4 x[4], y[KT];
 #pragma unroll
@@ -157,22 +180,13 @@ __device__ void simt_many(const AttnArgs& a, float* smem, AttnWalk walk) {
       for (int i = 0; i < KT; ++i)
         *reinterpret_cast<float4*>(sp + (cg + 16 * i) * M::LDP + rg * 4) = make_float4(s[0][i], s[1][i], s[2][i], s[3][i]);
       __syncwarp();  // the rows of a warp are its own
-      if (all) {
-#pragma unroll 4
-        for (int k = 0; k < M::KEYS; ++k) {
-          const float4 w = *reinterpret_cast<const float4*>(sp + k * M::LDP + rg * 4);
-#pragma unroll
-          for (int i = 0; i < CT; ++i) {
-            const float4 v = *reinterpret_cast<const float4*>(sv + k * HD + cg * 4 + 64 * i);
-            acc[0][i].x += w.x * v.x; acc[0][i].y += w.x * v.y; acc[0][i].z += w.x * v.z; acc[0][i].w += w.x * v.w;
-            acc[1][i].x += w.y * v.x; acc[1][i].y += w.y * v.y; acc[1][i].z += w.y * v.z; acc[1][i].w += w.y * v.w;
-            acc[2][i].x += w.z * v.x; acc[2][i].y += w.z * v.y; acc[2][i].z += w.z * v.z; acc[2][i].w += w.z * v.w;
-            acc[3][i].x += w.w * v.x; acc[3][i].y += w.w * v.y; acc[3][i].z += w.w * v.z; acc[3][i].w += w.w * v.w;
-          }
-        }
-      } else {  // a key that a row does not see contributes nothing to it, whatever its value holds
+      // Keys that all rows of the warp see, and around them those that only some see: such a key contributes nothing to the others,
+      // whatever its value holds.  (One by one through every step that has any: the chunk of 256 and 32 decodes of above take 43 us then.)
+      const int see = min(M::KEYS, max(0, warp_hi + 1 - kb)), see_lo = a.window > 0 ? min(see, max(0, warp_lo - a.window + 1 - kb)) : 0;
+      const int mid = a.window > 0 ? min(see, max(see_lo, warp_hi - a.window + 1 - kb)) : 0, mid_end = min(see, max(mid, warp_lo + 1 - kb));
+      auto one_by_one = [&](int k, int end) {
 #pragma unroll 1
-        for (int k = 0; k < M::KEYS; ++k) {
+        for (; k < end; ++k) {
           const float* w = sp + k * M::LDP + rg * 4;
 #pragma unroll
           for (int i = 0; i < CT; ++i) {
@@ -184,7 +198,21 @@ __device__ void simt_many(const AttnArgs& a, float* smem, AttnWalk walk) {
             }
           }
         }
+      };
+      one_by_one(see_lo, mid);
+#pragma unroll 4
+      for (int k = mid; k < mid_end; ++k) {
+        const float4 w = *reinterpret_cast<const float4*>(sp + k * M::LDP + rg * 4);
+#pragma unroll
+        for (int i = 0; i < CT; ++i) {
+          const float4 v = *reinterpret_cast<const float4*>(sv + k * HD + cg * 4 + 64 * i);
+          acc[0][i].x += w.x * v.x; acc[0][i].y += w.x * v.y; acc[0][i].z += w.x * v.z; acc[0][i].w += w.x * v.w;
+          acc[1][i].x += w.y * v.x; acc[1][i].y += w.y * v.y; acc[1][i].z += w.y * v.z; acc[1][i].w += w.y * v.w;
+          acc[2][i].x += w.z * v.x; acc[2][i].y += w.z * v.y; acc[2][i].z += w.z * v.z; acc[2][i].w += w.z * v.w;
+          acc[3][i].x += w.w * v.x; acc[3][i].y += w.w * v.y; acc[3][i].z += w.w * v.z; acc[3][i].w += w.w * v.w;
+        }
       }
+      one_by_one(mid_end, see);
       __syncwarp();
     }
 #pragma unroll
