@@ -27,8 +27,8 @@ struct PlanArgs {
 __device__ __forceinline__ void unit_cost(const AttnShape& sh, int kind, int nrows, int* block, int* fixed, int* least) {
   const bool wide = sh.head_dim > 64;
   if (sh.dtype == SB200_F32) {
-    *block = (kind == ATTN_MANY ? 1300 : 150) * sh.head_dim / 64;
-    *fixed = 200;
+    *block = (kind == ATTN_MANY ? 1200 : 150) * sh.head_dim / 64;
+    *fixed = kind == ATTN_MANY ? 350 : 200;
     *least = 1;
   } else if (kind == ATTN_MANY) {
     *block = nrows > 128 ? (wide ? 192 : 170) : (wide ? 170 : 150);
@@ -39,6 +39,21 @@ __device__ __forceinline__ void unit_cost(const AttnShape& sh, int kind, int nro
     *fixed = wide ? 260 : 220;
     *least = 2;
   }
+}
+
+// A unit as a whole.  fp32 tiles of many rows go 64 keys (or 32) at a time: a half of the first or last block that no row sees is not
+// done.  (A chunk of 256 tokens with 32 decodes: the last worker done after 37 us, most of them after 27, with whole blocks.)
+__device__ __forceinline__ long long unit_time(const AttnShape& sh, const AttnTile& d, int block, int fixed, int* lead) {
+  *lead = 0;
+  long long t = (long long)d.nblk * block + fixed;
+  if (sh.dtype == SB200_F32 && d.kind == ATTN_MANY && d.nblk > 0) {
+    const int tok0 = d.row0 / sh.group, tok1 = (d.row0 + d.nrows - 1) / sh.group;
+    const int hi = max(0, d.pos0 + tok1 + 1), lo = sh.window > 0 ? max(0, d.pos0 + tok0 + 1 - sh.window) : 0;
+    if (lo - d.blk_lo * kAttnBlock >= kAttnBlock / 2) *lead = block / 2;
+    t -= *lead;
+    if ((d.blk_lo + d.nblk) * kAttnBlock - hi >= kAttnBlock / 2) t -= block / 2;
+  }
+  return t;
 }
 
 constexpr long long kShareMany = 200, kShareFew = 150, kJoinMany = 500, kJoinFew = 250;
@@ -150,7 +165,8 @@ attn_plan_kernel(const PlanArgs a) {
       dst[1] = make_int4(d.pos0, d.page_at, d.blk_lo, d.nblk);
       int block, fixed, least;
       unit_cost(sh, d.kind, d.nrows, &block, &fixed, &least);
-      c = ((long long)d.nblk * block + fixed) * sh.kv_heads;
+      int lead;
+      c = unit_time(sh, d, block, fixed, &lead) * sh.kv_heads;
     }
     const long long at = carry + scan_block(c, red, &total);
     if (t < tiles) {
@@ -184,7 +200,8 @@ attn_plan_kernel(const PlanArgs a) {
       near_blocks[threadIdx.x] = d.nblk;
       near_cost[threadIdx.x] = block;
       near_fixed[threadIdx.x] = fixed;
-      atomicMax(&largest, (int)min((long long)d.nblk * block + fixed, 1ll << 30));
+      int lead;
+      atomicMax(&largest, (int)min(unit_time(sh, d, block, fixed, &lead), 1ll << 30));
     }
     __syncthreads();
     const int lane = threadIdx.x & 31, k = threadIdx.x >> 5;
@@ -238,9 +255,10 @@ attn_plan_kernel(const PlanArgs a) {
       const AttnTile d = a.plan.tiles[lo];
       int block, fixed, least;
       unit_cost(sh, d.kind, d.nrows, &block, &fixed, &least);
-      const long long unit = (long long)d.nblk * block + fixed, rem = x - (lo < kNearTiles ? near[lo] : a.plan.cost[lo]);
+      int lead;
+      const long long unit = unit_time(sh, d, block, fixed, &lead), rem = x - (lo < kNearTiles ? near[lo] : a.plan.cost[lo]);
       int head = (int)(rem / unit);
-      const long long in = rem - head * unit;
+      const long long in = rem - head * unit + lead;
       int blk = in <= fixed / 2 ? 0 : (int)min((in - fixed / 2 + block / 2) / block, (long long)d.nblk);
       // no piece of less than `least` blocks: the cut moves to the end of the unit it is near to
       if (blk < least) blk = 0;
