@@ -335,6 +335,44 @@ def test_repeats_agree_and_shared_pages():
             assert torch.equal(attention_ops.paged_attention(c["q"], c["cache"], plan, 0.09), first)
 
 
+@pytest.mark.parametrize("dtype,hd", [(torch.bfloat16, 128), (torch.float16, 64), (torch.float32, 128)])
+def test_values_before_and_behind_the_window(dtype, hd):
+    """Values that are not finite at keys that leave the window inside a tile, that enter it there, and at both."""
+    from sarathi_serve_b200 import attention_ops
+    c = make(17, dtype, 8, 2, hd, 16, [(150, 300), (1, 700), (40, 90), (3, 250)])
+    for r, keys in enumerate(((170, 299, 401, 449), (500, 612), (0, 60, 111), (120, 121, 252))):
+        for i, j in enumerate(keys):
+            c["cache"][c["table"][r, j // 16], 1, j % 16, i % 2, 5 * i:5 * i + 3] = (math.nan, math.inf)[i % 2]
+    plan, _ = plan_of(c, window=130)
+    check(c, attention_ops.paged_attention(c["q"], c["cache"], plan, 0.1), 0.1, window=130)
+
+
+@pytest.mark.parametrize("heads,hd", [(71, 64), (128, 128), (300, 64)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_many_heads_on_one(dtype, heads, hd):
+    """Groups wider than a tile of few rows, and than one of many: a token alone fills it; q with its heads apart."""
+    from sarathi_serve_b200 import attention_ops
+    c = make(18, dtype, heads, 1, hd, 16, [(1, 260), (3, 17), (1, 0), (2, 130)])
+    plan, _ = plan_of(c)
+    q = c["q"].unflatten(1, (heads, hd))
+    check(c, attention_ops.paged_attention(q, c["cache"], plan, 0.1), 0.1)
+
+
+@pytest.mark.parametrize("dtype,requests", [(torch.bfloat16, 3000), (torch.float32, 1500), (torch.float16, 8192)])
+def test_thousands_of_requests(dtype, requests):
+    """More tiles than the plan keeps near; the most requests that there can be."""
+    from sarathi_serve_b200 import attention_ops
+    g = torch.Generator().manual_seed(requests)
+    now = torch.randint(0, 24, (requests,), generator=g).tolist()
+    c = make(19, dtype, 2, 1, 64, 8, [(1, n) for n in now])
+    plan, _ = plan_of(c)
+    out = attention_ops.paged_attention(c["q"], c["cache"], plan, 0.125)
+    few = list(range(0, requests, max(1, requests // 150)))
+    part = dict(c, batch=[c["batch"][r] for r in few], total=len(few), q=c["q"][few], table=c["table"][few])
+    check(part, out[few], 0.125)
+    assert torch.isfinite(out).all()
+
+
 # ------------------------------------------------------------------ block tables and layout
 def layout_by_hand(query, context, table, page, pages, T):
     n, width = table.shape
