@@ -510,7 +510,10 @@ extern "C" int sb200_attention_plan(void* plan, int64_t plan_bytes, const sb200_
   a.max_tokens = shape->max_tokens;
   a.sh = sh;
   const size_t smem = 2 * (size_t)(num_requests + 1) * sizeof(int);
-  if (smem > 48 * 1024) SB_CUDA(cudaFuncSetAttribute(attn_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  // (What the most requests need, once: the limit without it is on this and the kernel's static 16 KB together, and a limit that
+  // follows each call's own size would be lowered under another thread's launch.)
+  static std::atomic<uint64_t> allowed{0};
+  SB_CUDA(allow_smem(reinterpret_cast<const void*>(attn_plan_kernel), 2 * (SB200_MAX_REQUESTS + 1) * (int)sizeof(int), &allowed));
   SB_CUDA(launch_dependent(attn_plan_kernel, dim3(1), dim3(kPlanThreads), smem, (cudaStream_t)stream, a));
   return SB200_OK;
 }

@@ -266,6 +266,8 @@ template <int W, int R> static bool any_meet(const Range (&written)[W], const Ra
   return false;
 }
 
+// (Each kernel is allowed what kMaxRequests need, once: the limit without that counts its static shared memory too, and a limit that
+// follows each call's own size would be lowered under another thread's launch.)
 static size_t layout_smem(int n, int arrays) { return (size_t)arrays * (n + 1) * sizeof(int); }
 
 extern "C" int sb200_resize_block_tables(int32_t* block_tables, int64_t ld, int32_t* num_blocks, const int32_t* seq_lens,
@@ -290,8 +292,8 @@ extern "C" int sb200_resize_block_tables(int32_t* block_tables, int64_t ld, int3
   // Eight CTAs where the tables could hold so many pages that a prompt's worth of them may move in one step.
   const int ctas = (int64_t)num_requests * width > 16384 ? 8 : 1;
   const size_t smem = layout_smem(num_requests, 4);
-  if (smem > 48 * 1024)
-    SB_CUDA(cudaFuncSetAttribute(resize_tables_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  static std::atomic<uint64_t> allowed{0};
+  SB_CUDA(allow_smem(reinterpret_cast<const void*>(resize_tables_kernel), (int)layout_smem(kMaxRequests, 4), &allowed));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(ctas);
   cfg.blockDim = dim3(kTablesThreads);
@@ -341,8 +343,8 @@ extern "C" int sb200_batch_layout(const int32_t* query_lens, const int32_t* cont
   int64_t ctas = (items + kLayoutThreads - 1) / kLayoutThreads;
   if (ctas > sm_count()) ctas = sm_count();
   const size_t smem = layout_smem(num_requests, 2);
-  if (smem > 48 * 1024)
-    SB_CUDA(cudaFuncSetAttribute(batch_layout_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  static std::atomic<uint64_t> allowed{0};
+  SB_CUDA(allow_smem(reinterpret_cast<const void*>(batch_layout_kernel), (int)layout_smem(kMaxRequests, 2), &allowed));
   SB_CUDA(launch_dependent(batch_layout_kernel, dim3((unsigned)ctas), dim3(kLayoutThreads), smem, (cudaStream_t)stream, a));
   return SB200_OK;
 }
