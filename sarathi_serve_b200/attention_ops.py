@@ -45,21 +45,21 @@ class AttentionPlan:
         self.buffer = torch.empty(plan_bytes, dtype=torch.uint8, device=device)
         self.workspace = torch.empty(lib.sb200_attention_workspace_bytes(self._shape), dtype=torch.uint8, device=device)
         self.kv_indices: Optional[torch.Tensor] = None
-        self._stream: Optional[torch.cuda.Stream] = None
-        self._stream_ptr: Optional[int] = None
+        # the stream of the last call; so far the one that the buffers belong to
+        self._stream = torch.cuda.current_stream(self.buffer.device)
+        self._stream_ptr: int = self._stream.cuda_stream
 
-    def stream(self) -> Optional[int]:
+    def stream(self) -> int:
         """The current stream, behind whatever the plan's calls have queued on the one they used last.  (A kernel that read a plan
         that is still being written would follow numbers that mean nothing.)  Not while a graph is captured: its replays are the
         caller's to order."""
         here = N.stream_ptr()
         if here != self._stream_ptr and not torch.cuda.is_current_stream_capturing():
             now = torch.cuda.current_stream()
-            if self._stream is not None:
-                now.wait_stream(self._stream)
-                for t in (self.buffer, self.workspace, self.kv_indices):
-                    if t is not None:
-                        t.record_stream(now)
+            now.wait_stream(self._stream)
+            for t in (self.buffer, self.workspace, self.kv_indices):
+                if t is not None:
+                    t.record_stream(now)
             self._stream, self._stream_ptr = now, here
         return here
 
@@ -67,7 +67,8 @@ class AttentionPlan:
                kv_lens: Optional[torch.Tensor] = None, kv_indptr: Optional[torch.Tensor] = None,
                kv_indices: Optional[torch.Tensor] = None) -> "AttentionPlan":
         """Plan the step of ``layout`` (or of the four arrays given by name).  The plan keeps ``kv_indices`` and reads it in
-        every ``paged_attention`` of the step; the others are read here only."""
+        every ``paged_attention`` of the step; the others are read here only.  A layout that was made on another stream must be
+        waited for there, as any tensor."""
         if layout is not None:
             qo_indptr, kv_lens, kv_indptr, kv_indices = layout[:4]
         if qo_indptr is None or kv_lens is None or kv_indptr is None or kv_indices is None:
@@ -80,7 +81,11 @@ class AttentionPlan:
         N.check(N.lib().sb200_attention_plan(self.buffer.data_ptr(), self.buffer.numel(), self._shape, qo_indptr.data_ptr(),
                                              kv_lens.data_ptr(), kv_indptr.data_ptr(), n, kv_indices.numel(), self.stream()),
                 "attention_plan")
-        self.kv_indices = kv_indices
+        if kv_indices is not self.kv_indices:
+            # The plan lets go of it at some later update, when this stream may still be reading it.
+            if not torch.cuda.is_current_stream_capturing():
+                kv_indices.record_stream(self._stream)
+            self.kv_indices = kv_indices
         return self
 
 

@@ -1,0 +1,106 @@
+"""Streams and lifetimes of what an attention plan keeps, without a GPU: the library and the streams are stand-ins that write down
+what is asked of them."""
+import contextlib
+
+import pytest
+import torch
+
+from sarathi_serve_b200 import _native as N
+from sarathi_serve_b200 import attention_ops
+
+
+class Stream:
+    def __init__(self, number):
+        self.cuda_stream, self.waited = number, []
+
+    def wait_stream(self, other):
+        self.waited.append(other)
+
+
+class Library:
+    def __getattr__(self, name):
+        return (lambda *a: 256) if name.endswith("_bytes") else (lambda *a: 0)
+
+
+class Machine:
+    """The current stream, and which memory was recorded on which one."""
+
+    def __init__(self):
+        self.streams = [Stream(0), Stream(7), Stream(9)]
+        self.now, self.recorded, self.capturing = self.streams[0], [], False
+
+    @contextlib.contextmanager
+    def on(self, stream):
+        before, self.now = self.now, stream
+        yield
+        self.now = before
+
+    def has(self, t, stream):
+        return any(at == t.untyped_storage().data_ptr() and s is stream for at, s in self.recorded)
+
+
+@pytest.fixture
+def machine(monkeypatch):
+    m = Machine()
+    monkeypatch.setattr(N, "lib", Library)
+    monkeypatch.setattr(N, "require_current", lambda *t: None)
+    monkeypatch.setattr(N, "stream_ptr", lambda: m.now.cuda_stream)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: m.now)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: m.capturing)
+    monkeypatch.setattr(torch.Tensor, "record_stream", lambda t, s: m.recorded.append((t.untyped_storage().data_ptr(), s)))
+    return m
+
+
+def plan():
+    return attention_ops.AttentionPlan(2, 1, 64, 16, torch.float16, 4, 8, device=torch.device("cpu"))
+
+
+def arrays():
+    i = lambda n: torch.zeros(n, dtype=torch.int32)
+    return dict(qo_indptr=i(3), kv_lens=i(2), kv_indptr=i(3), kv_indices=i(6))
+
+
+def test_a_list_of_pages_is_recorded_where_it_is_read(machine):
+    """Lists made on a side stream, the plan always on the main one: each list stays until the main stream has read it."""
+    p = plan()
+    lists = [arrays() for _ in range(3)]
+    for a in lists:
+        p.update(**a)
+    assert all(machine.has(a["kv_indices"], machine.streams[0]) for a in lists)
+
+
+def test_a_plan_used_first_on_another_stream_than_it_was_made_on(machine):
+    """Its memory may still be in use by what the first stream did before, and may be given away while the second one works."""
+    main, side, _ = machine.streams
+    p = plan()
+    with machine.on(side):
+        p.update(**arrays())
+    assert side.waited == [main]
+    assert all(machine.has(t, side) for t in (p.buffer, p.workspace, p.kv_indices))
+
+
+def test_a_plan_that_moves_between_streams(machine):
+    main, side, third = machine.streams
+    p = plan()
+    a, b = arrays(), arrays()
+    p.update(**a)
+    with machine.on(side):
+        p.stream()
+        assert side.waited == [main] and machine.has(a["kv_indices"], side)
+        p.update(**b)
+    with machine.on(third):
+        p.stream()
+    assert third.waited == [side] and machine.has(b["kv_indices"], side) and machine.has(b["kv_indices"], third)
+    assert not machine.has(a["kv_indices"], third)
+
+
+def test_a_captured_call_leaves_order_and_lifetimes_to_the_caller(machine):
+    main, side, _ = machine.streams
+    p = plan()
+    p.update(**arrays())
+    machine.recorded.clear()
+    machine.capturing = True
+    with machine.on(side):
+        p.update(**arrays())
+    machine.capturing = False
+    assert not machine.recorded and not side.waited and p.stream() == main.cuda_stream
