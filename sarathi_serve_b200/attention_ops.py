@@ -7,7 +7,7 @@ step can be captured into a CUDA graph and replayed with other lengths; ``paged_
 from __future__ import annotations
 
 import ctypes
-from typing import Optional
+from typing import List, Optional
 
 import torch
 
@@ -45,6 +45,7 @@ class AttentionPlan:
         self.buffer = torch.empty(plan_bytes, dtype=torch.uint8, device=device)
         self.workspace = torch.empty(lib.sb200_attention_workspace_bytes(self._shape), dtype=torch.uint8, device=device)
         self.kv_indices: Optional[torch.Tensor] = None
+        self.beside: List[torch.Tensor] = []  # what else the plan's user reads on its streams: kept from reuse like the plan's own
         # the stream of the last call; so far the one that the buffers belong to
         self._stream = torch.cuda.current_stream(self.buffer.device)
         self._stream_ptr: int = self._stream.cuda_stream
@@ -57,7 +58,7 @@ class AttentionPlan:
         if here != self._stream_ptr and not torch.cuda.is_current_stream_capturing():
             now = torch.cuda.current_stream()
             now.wait_stream(self._stream)
-            for t in (self.buffer, self.workspace, self.kv_indices):
+            for t in (self.buffer, self.workspace, self.kv_indices, *self.beside):
                 if t is not None:
                     t.record_stream(now)
             self._stream, self._stream_ptr = now, here

@@ -40,6 +40,9 @@ class PagedAttentionWrapper:
         self.block_tables = torch.full((max_requests, max_blocks), -1, **ints)
         self.layout = kv_cache_ops.batch_layout(self.query_lens, self.context_lens, self.block_tables, page_size, num_pages, max_tokens)
         self.plan.update(self.layout)
+        # (the layout's arrays are parts of two allocations)
+        self.plan.beside = [self.query_lens, self.context_lens, self.block_tables, self.layout.qo_indptr, self.layout.positions,
+                            *self.kv_caches]
         self.num_tokens = max_tokens
         self._appended: Optional[int] = None
 

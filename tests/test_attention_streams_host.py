@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from sarathi_serve_b200 import _native as N
-from sarathi_serve_b200 import attention_ops
+from sarathi_serve_b200 import attention_ops, attention_wrapper
 
 
 class Stream:
@@ -104,3 +104,15 @@ def test_a_captured_call_leaves_order_and_lifetimes_to_the_caller(machine):
         p.update(**arrays())
     machine.capturing = False
     assert not machine.recorded and not side.waited and p.stream() == main.cuda_stream
+
+
+def test_a_wrapper_that_is_used_on_another_stream_than_it_was_made_on(machine):
+    """All that its kernels read there stays until they have: caches, layout, the step's lengths and tables."""
+    main, side, _ = machine.streams
+    w = attention_wrapper.PagedAttentionWrapper(2, 1, 64, 16, 5, 2, torch.float16, 4, 8, 3, device=torch.device("cpu"))
+    i = lambda *s: torch.ones(*s, dtype=torch.int32)
+    with machine.on(side):
+        w.begin_forward(i(2), i(2), i(2, 1), 4)
+    assert side.waited == [main]
+    for t in (*w.kv_caches, *w.layout, w.query_lens, w.context_lens, w.block_tables, w.plan.buffer, w.plan.workspace):
+        assert machine.has(t, side)
