@@ -95,9 +95,11 @@ class PagedAttentionWrapper:
 
     def fused_kv_append(self, layer_cache_idx: int):
         """(paged cache, slots) for the qkv projection's epilogue: the layer stores its own keys and values."""
+        cache = self.kv_caches[layer_cache_idx]
+        N.require_current(cache)
         self.plan.stream()
         self._appended = layer_cache_idx
-        return self.kv_caches[layer_cache_idx], self.layout.kv_slots[:self.num_tokens]
+        return cache, self.layout.kv_slots[:self.num_tokens]
 
     def forward(self, query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, layer_cache_idx: int, softmax_scale: float = 1.0,
                 layer_id: Optional[int] = None) -> torch.Tensor:
@@ -106,6 +108,7 @@ class PagedAttentionWrapper:
         if T > self.max_tokens:
             raise RuntimeError(f"PagedAttentionWrapper: {T} rows, made for at most {self.max_tokens}")
         cache = self.kv_caches[layer_cache_idx]
+        N.require_current(query, key, value, cache)
         self.plan.stream()
         if self._appended != layer_cache_idx:
             kv_cache_ops.append_rows(cache, key, value, self.layout.kv_slots[:T])

@@ -18,8 +18,13 @@ class Stream:
 
 
 class Library:
+    def __init__(self):
+        self.calls = []
+
     def __getattr__(self, name):
-        return (lambda *a: 256) if name.endswith("_bytes") else (lambda *a: 0)
+        if name.endswith("_bytes"):
+            return lambda *a: 256
+        return lambda *a: self.calls.append(name) or 0
 
 
 class Machine:
@@ -28,6 +33,7 @@ class Machine:
     def __init__(self):
         self.streams = [Stream(0), Stream(7), Stream(9)]
         self.now, self.recorded, self.capturing = self.streams[0], [], False
+        self.library, self.device = Library(), 0
 
     @contextlib.contextmanager
     def on(self, stream):
@@ -42,8 +48,10 @@ class Machine:
 @pytest.fixture
 def machine(monkeypatch):
     m = Machine()
-    monkeypatch.setattr(N, "lib", Library)
-    monkeypatch.setattr(N, "require_current", lambda *t: None)
+    monkeypatch.setattr(N, "lib", lambda: m.library)
+    monkeypatch.setattr(N, "require_cuda", lambda *t: None)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: m.device)
+    monkeypatch.setattr(torch.Tensor, "get_device", lambda t: 0)
     monkeypatch.setattr(N, "stream_ptr", lambda: m.now.cuda_stream)
     monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: m.now)
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: m.capturing)
@@ -116,3 +124,18 @@ def test_a_wrapper_that_is_used_on_another_stream_than_it_was_made_on(machine):
     assert side.waited == [main]
     for t in (*w.kv_caches, *w.layout, w.query_lens, w.context_lens, w.block_tables, w.plan.buffer, w.plan.workspace):
         assert machine.has(t, side)
+
+
+def test_a_wrapper_on_another_current_device_refuses_its_calls(machine):
+    """Nothing is launched there, neither the append before the attention nor anything else, and the plan's stream stays."""
+    w = attention_wrapper.PagedAttentionWrapper(2, 1, 64, 16, 5, 2, torch.float16, 4, 8, 3, device=torch.device("cpu"))
+    i = lambda *s: torch.ones(*s, dtype=torch.int32)
+    w.begin_forward(i(2), i(2), i(2, 1), 4)
+    machine.library.calls.clear()
+    machine.device = 1
+    q, k = torch.zeros(4, 128, dtype=torch.float16), torch.zeros(4, 64, dtype=torch.float16)
+    with machine.on(machine.streams[1]):
+        for call in (lambda: w.fused_kv_append(0), lambda: w.forward(q, k, k, 0), lambda: w.begin_forward(i(2), i(2), i(2, 1), 4)):
+            with pytest.raises(RuntimeError, match="current device"):
+                call()
+    assert not machine.library.calls and not machine.streams[1].waited
