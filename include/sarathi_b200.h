@@ -280,7 +280,7 @@ typedef struct sb200_attention_shape {
  * sum_j exp(scale q . k[j]).  Scores, maxima, sums and outputs are fp32 until the one rounding at the end; fp16 / bf16
  * round the probabilities once more, for the second product.  A row that sees no key is zero (lse -inf).  Rows that belong to no
  * request are left as they were, or cleared if zero_rows_behind.  Pages outside [0, num_pages) read as zeros.
- * out must not overlap q (columns of one buffer may interleave if ldq = ldo) or the cache.
+ * out must not overlap q (columns of one buffer may interleave if ldq = ldo) or the cache, nor lse any of the three.
  * workspace (sb200_attention_workspace_bytes): parts of rows whose keys are shared out; written before it is read in every
  * call.  A plan and a workspace serve one call at a time: not two streams at once.  `status` (device word): as sb200_gemm_colpar.
  * Replaces: BatchPrefillWithPagedKVCacheWrapper.plan / run,

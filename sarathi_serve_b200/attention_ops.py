@@ -96,8 +96,8 @@ def paged_attention(q: torch.Tensor, paged_kv_cache: torch.Tensor, plan: Attenti
     have been appended before.  q: [tokens, heads * head_dim] (or [tokens, heads, head_dim]); its rows may be a strided view of
     the fused qkv buffer.  Rows that belong to no request are zero in a result that is allocated here (-inf in ``lse``); in an
     ``out`` that is given they, and their ``lse``, are left as they were.  ``out`` may be strided like q, but must not overlap q or
-    the cache.  ``lse``: optional fp32 [tokens, heads], the natural
-    logarithm of the softmax denominators."""
+    the cache.  ``lse``: optional fp32 [tokens, heads], the natural logarithm of the softmax denominators; it must not overlap any of
+    the three."""
     N.require_current(q, paged_kv_cache, out, lse, plan.buffer)
     if plan.kv_indices is None:
         raise RuntimeError("paged_attention: the plan has not been updated with a step")

@@ -463,6 +463,13 @@ static bool rows_meet(const void* x, uint64_t ldx, const void* y, uint64_t ldy, 
   return apart < row || apart > ldx - row;
 }
 
+// Does a range meet any of `rows` rows of `row` bytes, ldx bytes apart?  (The gaps between them may hold it.)
+static bool range_meets_rows(const void* r, uint64_t n, const void* x, uint64_t ldx, uint64_t rows, uint64_t row) {
+  const uint64_t a = reinterpret_cast<uintptr_t>(r), b = reinterpret_cast<uintptr_t>(x);
+  const uint64_t i = a < b + row ? 0 : (a - b - row) / ldx + 1;  // the first row that ends behind the range's start
+  return i < rows && b + i * ldx < a + n;
+}
+
 static int slot_rows(const AttnShape& sh) { return sh.rows_many > sh.rows_few ? sh.rows_many : sh.rows_few; }
 
 template <typename T>
@@ -541,6 +548,11 @@ extern "C" int sb200_paged_attention(void* out, int64_t ldo, float* lse, const v
   const uint64_t cache_bytes = (uint64_t)num_pages * 2 * sh.page_size * sh.kv_heads * sh.head_dim * es;
   SB_CHECK_ARG(!rows_meet(q, ldq * es, out, ldo * es, num_tokens, row * es) && !ranges_meet(out, out_bytes, cache, cache_bytes),
                "paged_attention: out must not overlap q or the cache");
+  const uint64_t lse_bytes = (uint64_t)num_tokens * sh.heads * sizeof(float);
+  SB_CHECK_ARG(!lse || (!range_meets_rows(lse, lse_bytes, out, ldo * es, num_tokens, row * es) &&
+                        !range_meets_rows(lse, lse_bytes, q, ldq * es, num_tokens, row * es) &&
+                        !ranges_meet(lse, lse_bytes, cache, cache_bytes)),
+               "paged_attention: lse must not overlap out, q or the cache");
   AttnArgs a = {};
   plan_view(const_cast<void*>(plan), tiles_cap(sh, shape), &a.plan);
   a.q = q; a.ldq = ldq; a.out = out; a.ldo = ldo; a.lse = lse; a.cache = cache;
