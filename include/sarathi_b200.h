@@ -275,7 +275,7 @@ typedef struct sb200_attention_shape {
  * sb200_batch_layout makes them: once a step, for all layers of this shape.  `plan` (sb200_attention_plan_bytes bytes) is
  * read by every sb200_paged_attention of the step.
  * sb200_paged_attention: out[t, h, :] = sum_j softmax_j(scale q[t, h] . k[j]) v[j].  q and out: [num_tokens, num_heads *
- * head_dim], rows ldq / ldo elements apart (views of the fused qkv buffer are fine); cache: [num_pages, 2, page_size,
+ * head_dim], rows ldq / ldo elements apart (views of the fused qkv buffer are fine; q spans less than 64 GiB); cache: [num_pages, 2, page_size,
  * num_kv_heads, head_dim]; kv_indices as planned.  lse: NULL or fp32 [num_tokens, num_heads], the natural logarithm of
  * sum_j exp(scale q . k[j]).  Scores, maxima, sums and outputs are fp32 until the one rounding at the end; fp16 / bf16
  * round the probabilities once more, for the second product.  A row that sees no key is zero (lse -inf).  Rows that belong to no

@@ -539,6 +539,9 @@ extern "C" int sb200_paged_attention(void* out, int64_t ldo, float* lse, const v
   SB_CHECK_ARG(out && q && plan && cache && (kv_indices || num_kv_indices == 0), "paged_attention: null pointer");
   SB_CHECK_ARG(ldq >= row && ldo >= row && aligned16(q) && aligned16(out) && aligned16(cache) && (ldq * es) % 16 == 0 && (ldo * es) % 16 == 0,
                "paged_attention: rows of q and out must be 16-byte aligned and at least %lld elements apart", (long long)row);
+  // (the kernels address the rows of q by 32-bit numbers of 16 bytes, the last of which stands for no row)
+  SB_CHECK_ARG(ldq <= (int64_t)((uint64_t)UINT32_MAX * 16 / es) / num_tokens && ldo <= INT64_MAX / es / num_tokens,
+               "paged_attention: %lld rows of q or out are too far apart (%lld, %lld)", (long long)num_tokens, (long long)ldq, (long long)ldo);
   SB_CHECK_ARG(num_pages > 0 && num_kv_indices >= 0 && num_pages * 2 * sh.page_size <= INT32_MAX, "paged_attention: bad cache of %lld pages",
                (long long)num_pages);
   SB_CHECK_ARG(workspace && aligned16(workspace) && workspace_bytes >= sb200_attention_workspace_bytes(shape),

@@ -52,3 +52,16 @@ def test_lse_between_rows_as_found_by_trying_them_all():
         lse = out + 4 * rng.randint(-200, T * ldo // 2 + 200)
         meet = any(lse < out + i * ldo * 2 + 2048 and out + i * ldo * 2 < lse + T * 32 for i in range(T))
         assert said(attention(s, T=T, ldo=ldo, lse=lse), b"lse must not overlap") == meet, (T, ldo, lse - out)
+
+
+@without_gpu
+def test_rows_too_far_apart():
+    """Offsets of q rows are kept in 32 bits, in units of 16 bytes: 64 GiB, which a strided view of a large buffer can pass."""
+    for dtype, es in ((2, 2), (0, 4)):
+        s = shape(dtype=dtype, tokens=1 << 20)
+        T = 1 << 20
+        far = ((1 << 32) - 1) * 16 // es // T // 8 * 8
+        assert not said(attention(s, T=T, ldq=far, q=1 << 50), b"too far apart")
+        assert said(attention(s, T=T, ldq=far + 8, q=1 << 50), b"too far apart")
+        assert said(attention(s, T=2, ldq=1 << 62, q=1 << 50), b"too far apart")
+        assert said(attention(s, T=8, ldo=1 << 61), b"too far apart")
