@@ -151,7 +151,7 @@ attn_plan_kernel(const PlanArgs a) {
       // no more tokens than the listed pages have room for, whatever the length says
       const long long at0 = min((long long)max(0, a.kv_indptr[lo]), (long long)a.num_kv_indices);
       const long long at1 = min((long long)max(0, a.kv_indptr[lo + 1]), (long long)a.num_kv_indices);
-      const long long room = min(max(0ll, at1 - at0) * sh.page_size, 1ll << 30);
+      const long long room = min(max(0ll, at1 - at0) * sh.page_size, (long long)kAttnMaxKeys);
       const int len = (int)min((long long)max(0, a.kv_lens[lo]), room);
       d.pos0 = len - q;
       d.page_at = (int)at0;
@@ -414,7 +414,7 @@ static int attn_shape(const sb200_attention_shape* s, AttnShape* sh, const char*
   sh->head_dim = s->head_dim;
   sh->page_size = s->page_size;
   sh->dtype = s->dtype;
-  sh->window = s->window;
+  sh->window = s->window < kAttnMaxKeys ? s->window : 0;  // (a wider one hides nothing; position - window stays within 32 bits)
   // Tiles of 256 rows on tcgen05 fetch keys in boxes of whole swizzle atoms (8 rows); pages that are no multiple of 8, and
   // heads of 256, whose two outputs and scores do not fit TMEM together, stay with tiles of 16 rows.
   const bool many = s->dtype != SB200_F32 && s->head_dim <= 128 && s->page_size % 8 == 0;

@@ -19,6 +19,7 @@
 namespace sb200 {
 
 constexpr int kAttnBlock = 128;       // keys of a block
+constexpr int kAttnMaxKeys = 1 << 30; // of a request; positions are below
 constexpr int kAttnMaxWorkers = 256;  // (B200: 148 SMs)
 
 // How the rows of a tile are computed.
