@@ -179,5 +179,16 @@ def require_current(*tensors: torch.Tensor) -> None:
             raise RuntimeError(f"sarathi_serve_b200: a tensor is on cuda:{t.get_device()}, the current device is cuda:{here}")
 
 
+INT_MAX = 2 ** 31 - 1
+
+
+def int32(name: str, v, what: str) -> int:
+    """A number for a C int: ctypes would keep the low 32 bits of a larger one and say nothing."""
+    v = int(v)
+    if not -INT_MAX <= v <= INT_MAX:
+        raise RuntimeError(f"{what}: {name} = {v} does not fit 32 bits")
+    return v
+
+
 def ptr(t):
     return None if t is None else t.data_ptr()

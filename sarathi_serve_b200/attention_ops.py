@@ -30,8 +30,10 @@ class AttentionPlan:
                  max_tokens: int, window: int = 0, device: Optional[torch.device] = None):
         if dtype not in N._DTYPE_ID:
             raise RuntimeError(f"AttentionPlan: unsupported dtype {dtype}")
-        self.shape = N.AttentionShape(num_heads, num_kv_heads, head_dim, page_size, N._DTYPE_ID[dtype], int(window or 0), max_requests,
-                                      max_tokens)
+        window = min(int(window or 0), N.INT_MAX)  # (no request is that long)
+        self.shape = N.AttentionShape(*[N.int32(n, v, "AttentionPlan") for n, v in (
+            ("num_heads", num_heads), ("num_kv_heads", num_kv_heads), ("head_dim", head_dim), ("page_size", page_size),
+            ("dtype", N._DTYPE_ID[dtype]), ("window", window), ("max_requests", max_requests), ("max_tokens", max_tokens))])
         self._shape = ctypes.byref(self.shape)
         lib = N.lib()
         plan_bytes = lib.sb200_attention_plan_bytes(self._shape)
@@ -41,7 +43,7 @@ class AttentionPlan:
             device = torch.device("cuda", torch.cuda.current_device())
         self.dtype = dtype
         self.num_heads, self.num_kv_heads, self.head_dim, self.page_size = num_heads, num_kv_heads, head_dim, page_size
-        self.max_requests, self.max_tokens, self.window = max_requests, max_tokens, int(window or 0)
+        self.max_requests, self.max_tokens, self.window = max_requests, max_tokens, window
         self.buffer = torch.empty(plan_bytes, dtype=torch.uint8, device=device)
         self.workspace = torch.empty(lib.sb200_attention_workspace_bytes(self._shape), dtype=torch.uint8, device=device)
         self.kv_indices: Optional[torch.Tensor] = None

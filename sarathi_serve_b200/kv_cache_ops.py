@@ -34,7 +34,7 @@ def slots(batch_indices: torch.Tensor, positions: torch.Tensor, kv_indices: torc
     if out is None:
         out = torch.empty(n, dtype=torch.int64, device=batch_indices.device)
     N.check(N.lib().sb200_kv_cache_slots(N.ptr(out), N.ptr(batch_indices), N.ptr(positions), N.ptr(kv_indices),
-                                         N.ptr(kv_indptr), n, int(page_size), N.stream_ptr()), "kv_cache_slots")
+                                         N.ptr(kv_indptr), n, N.int32("page_size", page_size, "kv_cache_ops.slots"), N.stream_ptr()), "kv_cache_slots")
     return out
 
 
@@ -109,7 +109,7 @@ def resize_block_tables(block_tables: torch.Tensor, num_blocks: torch.Tensor, se
         _int32("granted", granted, n, what)
     N.check(N.lib().sb200_resize_block_tables(N.ptr(block_tables), _table_stride(block_tables), N.ptr(num_blocks), N.ptr(seq_lens),
                                               N.ptr(free_blocks), N.ptr(num_free), N.ptr(granted), n, block_tables.shape[1],
-                                              free_blocks.numel(), int(page_size), N.stream_ptr()), what)
+                                              free_blocks.numel(), N.int32("page_size", page_size, what), N.stream_ptr()), what)
     return granted
 
 
@@ -172,6 +172,6 @@ def batch_layout(query_lens: torch.Tensor, context_lens: torch.Tensor, block_tab
         out._for = (sizes, tuple(map(torch.Tensor.data_ptr, out)), out.kv_indices.numel())
     _, (qo, kv, indptr, indices, last, req, pos, slot), capacity = out._for
     N.check(N.lib().sb200_batch_layout(query_lens.data_ptr(), context_lens.data_ptr(), block_tables.data_ptr(), _table_stride(block_tables),
-                                       n, width, int(page_size), int(num_pages), T, qo, kv, indptr, indices, capacity, last, req, pos,
+                                       n, width, N.int32("page_size", page_size, what), int(num_pages), T, qo, kv, indptr, indices, capacity, last, req, pos,
                                        slot, N.stream_ptr()), what)
     return out

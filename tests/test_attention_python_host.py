@@ -1,12 +1,12 @@
-"""Streams and lifetimes of what an attention plan keeps, without a GPU: the library and the streams are stand-ins that write down
-what is asked of them."""
+"""Python side of the attention plan, its wrapper and the layout, without a GPU: streams, lifetimes, devices, arguments.  The library and
+the streams are stand-ins that write down what is asked of them."""
 import contextlib
 
 import pytest
 import torch
 
 from sarathi_serve_b200 import _native as N
-from sarathi_serve_b200 import attention_ops, attention_wrapper
+from sarathi_serve_b200 import attention_ops, attention_wrapper, kv_cache_ops
 
 
 class Stream:
@@ -139,3 +139,23 @@ def test_a_wrapper_on_another_current_device_refuses_its_calls(machine):
             with pytest.raises(RuntimeError, match="current device"):
                 call()
     assert not machine.library.calls and not machine.streams[1].waited
+
+
+def test_numbers_that_do_not_fit_32_bits(machine):
+    """The library takes C ints, of which ctypes would keep the low half."""
+    make = lambda **k: attention_ops.AttentionPlan(**{**dict(num_heads=2, num_kv_heads=1, head_dim=64, page_size=16, dtype=torch.float16,
+                                                             max_requests=4, max_tokens=8, device=torch.device("cpu")), **k})
+    for name in ("num_heads", "num_kv_heads", "head_dim", "page_size", "max_requests", "max_tokens"):
+        with pytest.raises(RuntimeError, match=name):
+            make(**{name: 2 ** 32 + 64})
+    with pytest.raises(RuntimeError, match="window"):
+        make(window=-2 ** 32 + 5)
+    assert make(window=2 ** 32 + 100).shape.window == make(window=2 ** 63 - 1).shape.window == 2 ** 31 - 1   # (wide, not 100 and -1)
+    assert make(window=None).shape.window == 0 and make(window=100).shape.window == 100
+    i = lambda *s: torch.zeros(*s, dtype=torch.int32)
+    for call in (lambda: kv_cache_ops.batch_layout(i(2), i(2), i(2, 3), 2 ** 32 + 16, 9, 8),
+                 lambda: kv_cache_ops.resize_block_tables(i(2, 3), i(2), i(2), i(9), i(1), 2 ** 32 + 16),
+                 lambda: kv_cache_ops.slots(i(2), i(2), i(3), i(3), 2 ** 32 + 16)):
+        with pytest.raises(RuntimeError, match="page_size"):
+            call()
+    assert not machine.library.calls
