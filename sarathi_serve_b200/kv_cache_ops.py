@@ -125,8 +125,8 @@ class _BatchArrays(NamedTuple):
 
 
 class BatchLayout(_BatchArrays):
-    """Index arrays of a step (see ``batch_layout``).  ``_for``: the sizes and device that ``batch_layout`` made or checked them
-    for, with their addresses, so that a step that writes them again need not look at eight tensors."""
+    """Index arrays of a step (see ``batch_layout``).  ``_for``: the sizes, device, addresses and lengths that ``batch_layout`` made or
+    checked them for, so that a step that writes the same arrays again need not look at eight types, shapes and strides."""
     _for = None
 
 
@@ -151,16 +151,17 @@ def batch_layout(query_lens: torch.Tensor, context_lens: torch.Tensor, block_tab
     T, width, dev = int(num_tokens), block_tables.shape[1], query_lens.device
     if T < 0:
         raise RuntimeError(f"{what}: num_tokens is negative")
-    sizes = (n, width, T, dev)
-    if out is None:
+    made = out is None
+    if made:
         # one allocation each for the two types; the parts of either one after the other
         parts = [n + 1, n, n + 1, n * width, n, T]
         ints = torch.empty(sum(parts), dtype=torch.int32, device=dev)
         longs = torch.empty(2 * T, dtype=torch.int64, device=dev)
         # ("unsafe": without the bookkeeping of autograd for views, which integers have no use for)
         out = BatchLayout(*torch.unsafe_split_with_sizes(ints, parts), *torch.unsafe_split_with_sizes(longs, [T, T]))
-        out._for = (sizes, tuple(map(torch.Tensor.data_ptr, out)), n * width)
-    elif getattr(out, "_for", None) is None or out._for[0] != sizes or out._for[1][0] != out[0].data_ptr():
+    at, lengths = [*map(torch.Tensor.data_ptr, out)], [*map(torch.Tensor.numel, out)]
+    this = (n, width, T, dev, at, lengths)
+    if not made and out._for != this:
         N.require_current(*out)
         for name, t, k in zip(BatchLayout._fields, out, (n + 1, n, n + 1, -1, n, T)):
             _int32("out." + name, t, k, what)
@@ -169,9 +170,9 @@ def batch_layout(query_lens: torch.Tensor, context_lens: torch.Tensor, block_tab
         for t in out[6:]:
             if t.dtype != torch.int64 or t.shape != (T,) or not t.is_contiguous():
                 raise RuntimeError(f"{what}: out.positions and out.kv_slots must be contiguous int64 tensors of {T} elements")
-        out._for = (sizes, tuple(map(torch.Tensor.data_ptr, out)), out.kv_indices.numel())
-    _, (qo, kv, indptr, indices, last, req, pos, slot), capacity = out._for
+    out._for = this
+    qo, kv, indptr, indices, last, req, pos, slot = at
     N.check(N.lib().sb200_batch_layout(query_lens.data_ptr(), context_lens.data_ptr(), block_tables.data_ptr(), _table_stride(block_tables),
-                                       n, width, N.int32("page_size", page_size, what), int(num_pages), T, qo, kv, indptr, indices, capacity, last, req, pos,
-                                       slot, N.stream_ptr()), what)
+                                       n, width, N.int32("page_size", page_size, what), int(num_pages), T, qo, kv, indptr, indices,
+                                       lengths[3], last, req, pos, slot, N.stream_ptr()), what)
     return out

@@ -159,3 +159,32 @@ def test_numbers_that_do_not_fit_32_bits(machine):
         with pytest.raises(RuntimeError, match="page_size"):
             call()
     assert not machine.library.calls
+
+
+def test_a_layout_whose_arrays_were_exchanged(machine):
+    """What is written is what the tuple holds now, whichever of its tensors got other memory or another length since."""
+    written = []
+    machine.library.sb200_batch_layout = lambda *a: written.append(a) or 0
+    i = lambda *s: torch.zeros(*s, dtype=torch.int32)
+    step = lambda out=None: kv_cache_ops.batch_layout(i(2), i(2), i(2, 3), 16, 9, 8, out=out)
+    lay = step()
+    arrays = lambda: [*(x for x in written[-1][9:13]), *(x for x in written[-1][14:18])]
+    assert arrays() == [t.data_ptr() for t in lay]
+    assert step(lay) is lay and arrays() == [t.data_ptr() for t in lay]
+    for k, name in enumerate(lay._fields):
+        old = lay[k].data_ptr()
+        lay[k].data = torch.zeros_like(lay[k])
+        assert lay[k].data_ptr() != old
+        step(lay)
+        assert arrays() == [t.data_ptr() for t in lay], name
+        whole = lay[k].data
+        lay[k].data = whole[:-1]
+        with pytest.raises(RuntimeError, match="out."):
+            step(lay)
+        lay[k].data = whole
+        step(lay)
+    wide = lay._replace(kv_indices=i(10))
+    step(wide)
+    assert arrays() == [t.data_ptr() for t in wide] and written[-1][13] == 10
+    with pytest.raises(RuntimeError, match="kv_indices"):
+        step(lay._replace(kv_indices=i(5)))
