@@ -315,10 +315,10 @@ attn_join_kernel(const AttnArgs a) {
   constexpr int kRows = kJoinValues / HD, kBatch = 4;
   __shared__ int first[kAttnMaxWorkers + 1];
   T* out = reinterpret_cast<T*>(a.out);
-  const int units = __ldcg(&a.plan.starts[0].units);
+  const int units = attn_clamp(__ldcg(&a.plan.starts[0].units), 0, a.workers);  // (what comes from the plan: see attn_piece)
   for (int i = threadIdx.x; i <= a.workers; i += kJoinThreads) first[i] = __ldcg(a.plan.cut_first + i);  // (behind `units`: anything)
   __syncthreads();
-  const int groups = first[units];
+  const int groups = min(first[units], a.workers * (a.slot_rows * HD / kJoinValues));
   int lo = 0;
   int4 u, v;  // the cut unit of group g
   auto look_up = [&](int g) {
@@ -336,7 +336,7 @@ attn_join_kernel(const AttnArgs a) {
   if ((int)blockIdx.x < groups) look_up(blockIdx.x);
   grid_dependency_begin();
   if (a.zero_behind) {
-    const int rows0 = min(a.plan.starts[0].rows, a.num_tokens), per_row = a.kv_heads * a.group * HD;
+    const int rows0 = attn_clamp(a.plan.starts[0].rows, 0, a.num_tokens), per_row = a.kv_heads * a.group * HD;
     for (int t = rows0 + blockIdx.x; t < a.num_tokens; t += gridDim.x) {
       for (int i = threadIdx.x; i < per_row; i += kJoinThreads) out[t * a.ldo + i] = DT<T>::from_f(0.f);
       if (a.lse)
@@ -346,9 +346,11 @@ attn_join_kernel(const AttnArgs a) {
   }
   for (int g = blockIdx.x; g < groups; g += gridDim.x) {
     if (g != (int)blockIdx.x) look_up(g);
-    const AttnCut c = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+    AttnCut c = {attn_clamp(u.x, 0, a.num_tokens), attn_clamp(u.y, 0, a.num_tokens * a.group), attn_clamp(u.z, 0, a.slot_rows), u.w,
+                 attn_clamp(v.x, 0, a.kv_heads - 1), attn_clamp(v.y, 0, 2 * a.workers - 1), v.z, 0};
+    c.pieces = min(c.pieces, 2 * a.workers - c.slot);
     const int r = (g - first[lo]) * kRows + threadIdx.x % kRows, col4 = threadIdx.x / kRows;
-    if (r >= min(c.nrows, max(0, (a.num_tokens - c.q_row) * a.group - c.row0))) continue;
+    if ((unsigned)r >= (unsigned)min(c.nrows, max(0, (a.num_tokens - c.q_row) * a.group - c.row0))) continue;
     float m = -INFINITY, base = 0.f, sum = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int i = 0; i < c.pieces; i += kBatch) {
@@ -576,6 +578,11 @@ extern "C" int sb200_paged_attention(void* out, int64_t ldo, float* lse, const v
   a.scale_log2 = scale * 1.4426950408889634f;
   a.zero_behind = zero_rows_behind;
   const int workers = a.workers = attn_workers();
+  a.rows_many = sh.rows_many;
+  a.rows_few = sh.rows_few;
+  a.many_cap = sh.few_limit < INT32_MAX ? a.plan.tiles_cap : 0;
+  const int64_t listed = min(num_kv_indices * sh.page_size, (int64_t)kAttnMaxKeys);
+  a.blocks = (int)((listed + kAttnBlock - 1) / kAttnBlock);
   cudaStream_t s = (cudaStream_t)stream;
   if (int rc = sh.dtype == SB200_F32 ? run_attn_simt(sh.head_dim, a, workers, s)
                                      : run_attn_tc(sh.dtype, sh.head_dim, a, sh, workers, s))

@@ -78,7 +78,7 @@ struct FastDiv {
     while ((1ll << s) < d) ++s;
     return FastDiv{(uint32_t)((1ull << (31 + s)) / (uint32_t)d + 1), 31 + s, (uint32_t)d};
   }
-  __device__ __forceinline__ int div(int n) const { return (int)(((uint64_t)(uint32_t)n * mul) >> shift); }
+  __host__ __device__ __forceinline__ int div(int n) const { return (int)(((uint64_t)(uint32_t)n * mul) >> shift); }
 };
 
 struct AttnArgs {
@@ -94,6 +94,9 @@ struct AttnArgs {
   int64_t num_kv_indices;
   int num_pages, num_tokens;
   int workers;
+  int rows_many, rows_few;  // of a tile, at most
+  int many_cap;             // tiles of many rows, at most (0: this shape has none)
+  int blocks;               // of a request, at most: no more than all listed pages hold
   int kv_heads, group, page_size, window, slot_rows;
   FastDiv by_group, by_page;
   float scale_log2;    // scale * log2(e): scores in powers of two
@@ -113,29 +116,65 @@ __device__ __forceinline__ float4* attn_part(const AttnArgs& a, int head_dim, in
   return reinterpret_cast<float4*>(a.part_o + (int64_t)slot * a.slot_rows * head_dim) + (col4 * stride + row);
 }
 
-// Walks a worker's share of the line.
+__host__ __device__ __forceinline__ int attn_clamp(int v, int lo, int hi) { return v < lo ? lo : v > hi ? hi : v; }
+
+// The piece of tile t that begins at `cur`, in a share that ends at `end`; `most`: rows of its kind of tile, `slot`: of the share's next
+// piece that is not a whole unit.
+// What comes from the plan is held to what the call's own arguments allow.  Calls that share a plan follow one another, and then
+// nothing changes here; if a caller lets them overlap all the same (graphs on two streams, the C interface), or hands over the plan of
+// another shape, the numbers are wrong but no address is.
+__host__ __device__ __forceinline__ AttnPiece attn_piece(const AttnArgs& a, AttnTile t, int4 cur, int4 end, int most, int* slot) {
+  AttnPiece p;
+  t.q_row = attn_clamp(t.q_row, 0, a.num_tokens);
+  t.row0 = attn_clamp(t.row0, 0, a.num_tokens * a.group);
+  t.nrows = attn_clamp(t.nrows, 0, most);
+  t.pos0 = attn_clamp(t.pos0, -kAttnMaxKeys, kAttnMaxKeys);
+  t.page_at = t.page_at < 0 ? 0 : t.page_at;
+  t.blk_lo = attn_clamp(t.blk_lo, 0, a.blocks);
+  t.nblk = attn_clamp(t.nblk, 0, a.blocks - t.blk_lo);
+  p.t = t;
+  p.stride = t.nrows;
+  p.head = attn_clamp(cur.y, 0, a.kv_heads - 1);
+  p.b0 = attn_clamp(cur.z, 0, t.nblk);
+  p.b1 = cur.x == end.x && cur.y == end.y ? attn_clamp(end.z, p.b0, t.nblk) : t.nblk;
+  p.slot = p.b0 > 0 || p.b1 < t.nblk ? attn_clamp((*slot)++, 0, 2 * a.workers - 1) : -1;
+  // q may have fewer rows than the plan was made for (tokens x group stays below 2^30)
+  p.t.nrows = attn_clamp((a.num_tokens - t.q_row) * a.group - t.row0, 0, t.nrows);
+  const int first = a.by_group.div(t.row0), last = a.by_group.div(t.row0 + (p.t.nrows > 0 ? p.t.nrows - 1 : 0));
+  p.hi = t.pos0 + last + 1 < 0 ? 0 : t.pos0 + last + 1;
+  p.lo = a.window > 0 && t.pos0 + first + 1 > a.window ? t.pos0 + first + 1 - a.window : 0;
+  return p;
+}
+
+// Walks a worker's share of the line.  How many pieces it finds follows from the share's two ends alone, which all warps of a CTA have
+// from one copy in shared memory; a piece's tile is the same for all lanes of a warp.  So waits for each other hold up even where the
+// plan changes meanwhile (see attn_piece).
 struct AttnWalk {
   int4 cur, end;
-  AttnTile tile;  // of cur
-  int many, slot;
-  __device__ __forceinline__ AttnWalk(const AttnArgs& a, int w) {
-    const int4* s = reinterpret_cast<const int4*>(a.plan.starts + w);
-    const int4 x = s[0], u = s[1], v = s[2], e = s[3];
-    end = reinterpret_cast<const int4*>(a.plan.starts + w + 1)[0];
-    cur = x;
-    tile = AttnTile{u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
-    many = e.x;
-    slot = e.y;
+  int word;  // lane i, i + 8, ...: the i-th number of the tile at `cur`, asked for when the one before was taken
+  int many, slot, most;
+  // s: the worker's AttnStart and the first 16 bytes of the next one (attn_share)
+  __device__ __forceinline__ AttnWalk(const AttnArgs& a, const int4* s) {
+    cur = s[0];
+    end = s[4];
+    cur.x = attn_clamp(cur.x, 0, a.plan.tiles_cap);
+    end.x = attn_clamp(end.x, 0, a.plan.tiles_cap);
+    end.y = attn_clamp(end.y, 0, a.kv_heads);
+    many = attn_clamp(s[3].x, 0, a.many_cap);
+    slot = s[3].y;
+    word = reinterpret_cast<const int*>(s + 1)[threadIdx.x & 7];
+    most = 0;
   }
   __device__ __forceinline__ void fetch(const AttnArgs& a) {
-    if (!more()) return;
-    const int4* src = reinterpret_cast<const int4*>(a.plan.tiles + cur.x);
-    const int4 u = src[0], v = src[1];
-    tile = AttnTile{u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+    if (more()) word = reinterpret_cast<const int*>(a.plan.tiles + min(cur.x, a.plan.tiles_cap - 1))[threadIdx.x & 7];
   }
   // Only the tiles of many rows, or the others.
-  __device__ __forceinline__ void only_many() { if (end.x >= many) end = make_int4(many, 0, 0, 0); }
+  __device__ __forceinline__ void only_many(const AttnArgs& a) {
+    most = a.rows_many;
+    if (end.x >= many) end = make_int4(many, 0, 0, 0);
+  }
   __device__ __forceinline__ void only_few(const AttnArgs& a) {
+    most = a.rows_few;
     if (cur.x < many) {
       // pieces that are passed over keep their slots: the first, and the last if the share ends among them
       if (more() && cur.z > 0) ++slot;
@@ -146,20 +185,19 @@ struct AttnWalk {
   __device__ __forceinline__ bool more() const {
     return cur.x < end.x || (cur.x == end.x && (cur.y < end.y || (cur.y == end.y && cur.z < end.z)));
   }
+  // Called by whole warps.
   __device__ __forceinline__ bool next(const AttnArgs& a, AttnPiece* p) {
     if (!more()) return false;
-    p->t = tile;
-    p->stride = tile.nrows;
-    p->head = cur.y;
-    p->b0 = cur.z;
-    p->b1 = cur.x == end.x && cur.y == end.y ? end.z : p->t.nblk;
-    const bool head_cut = p->b0 > 0, tail_cut = p->b1 < p->t.nblk;
-    p->slot = head_cut || tail_cut ? slot++ : -1;
-    // q may have fewer rows than the plan was made for (tokens x group stays below 2^30)
-    p->t.nrows = min(p->t.nrows, max(0, (a.num_tokens - p->t.q_row) * a.group - p->t.row0));
-    const int first = a.by_group.div(p->t.row0), last = a.by_group.div(p->t.row0 + max(p->t.nrows, 1) - 1);
-    p->hi = max(0, p->t.pos0 + last + 1);
-    p->lo = a.window > 0 ? max(0, p->t.pos0 + first + 1 - a.window) : 0;
+    AttnTile t;
+    t.q_row = __shfl_sync(0xffffffffu, word, 0);
+    t.row0 = __shfl_sync(0xffffffffu, word, 1);
+    t.nrows = __shfl_sync(0xffffffffu, word, 2);
+    t.kind = 0;  // (the walk goes over one kind only)
+    t.pos0 = __shfl_sync(0xffffffffu, word, 4);
+    t.page_at = __shfl_sync(0xffffffffu, word, 5);
+    t.blk_lo = __shfl_sync(0xffffffffu, word, 6);
+    t.nblk = __shfl_sync(0xffffffffu, word, 7);
+    *p = attn_piece(a, t, cur, end, most, &slot);
     if (cur.y + 1 < a.kv_heads) {
       cur = make_int4(cur.x, cur.y + 1, 0, 0);
     } else {
@@ -169,6 +207,12 @@ struct AttnWalk {
     return true;
   }
 };
+
+// The CTA's share: five times 16 bytes of the plan, read once for all of its threads.
+__device__ __forceinline__ void attn_share(const AttnArgs& a, int4* to) {
+  if (threadIdx.x < 5) to[threadIdx.x] = reinterpret_cast<const int4*>(a.plan.starts + blockIdx.x)[threadIdx.x];
+  __syncthreads();
+}
 
 // Cache row (of kv_heads * head_dim elements) of a key, or -1 where its page is not one of the cache's: such a page reads
 // as zeros, so that a bad table cannot reach outside.  The value is page_size rows further.
@@ -196,7 +240,7 @@ struct AttnAhead {
 };
 
 // Where row r of a piece's tile goes: (token row, q head).
-__device__ __forceinline__ void attn_row(const AttnArgs& a, const AttnPiece& p, int r, int* token, int* head, int* pos) {
+__host__ __device__ __forceinline__ void attn_row(const AttnArgs& a, const AttnPiece& p, int r, int* token, int* head, int* pos) {
   const int row = p.t.row0 + r, tok = a.by_group.div(row);
   *token = p.t.q_row + tok;
   *head = p.head * a.group + (row - tok * a.group);

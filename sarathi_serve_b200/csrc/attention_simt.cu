@@ -66,9 +66,17 @@ __device__ void simt_many(const AttnArgs& a, float* smem, AttnWalk walk) {
   const float* q = reinterpret_cast<const float*>(a.q);
   const float* cache = reinterpret_cast<const float*>(a.cache);
   const int64_t ldc = (int64_t)a.kv_heads * HD;
+  // The keys of a piece, as its first warp sees them: every step below waits for all warps (two pieces' in turn: the next one's
+  // are written when not all may have read these).
+  __shared__ int2 ends[2];
+  int turn = 0;
   AttnPiece p;
   while (walk.next(a, &p)) {
+    if (tid == 0)
+      ends[turn] = make_int2(max(p.lo, (p.t.blk_lo + p.b0) * kAttnBlock) & ~(M::KEYS - 1), min(p.hi, (p.t.blk_lo + p.b1) * kAttnBlock));
     __syncthreads();  // the previous piece has been read
+    const int k0 = ends[turn].x, k1 = ends[turn].y;
+    turn ^= 1;
     for (int i = tid; i < kSimtRows * VPR; i += kSimtThreads) {
       const int r = i / VPR, v = i - r * VPR;
       int token, head, pos;
@@ -91,7 +99,6 @@ __device__ void simt_many(const AttnArgs& a, float* smem, AttnWalk walk) {
     }
     const int pos_first = p.t.pos0 + a.by_group.div(p.t.row0), pos_last = p.hi - 1;
     const int warp_lo = __shfl_sync(0xffffffffu, pos[0], 0), warp_hi = __shfl_sync(0xffffffffu, pos[3], 31);  // of the warp's rows
-    const int k0 = max(p.lo, (p.t.blk_lo + p.b0) * kAttnBlock) & ~(M::KEYS - 1), k1 = min(p.hi, (p.t.blk_lo + p.b1) * kAttnBlock);
     // Lane l knows the pages of keys l, l + 32 of the step after the next, so that the loads of the next one (this thread's share:
     // next_k, next_v; real: whether its i-th row is one) wait for nothing.
     AttnAhead ahead[M::KEYS / 32];
@@ -424,9 +431,10 @@ attn_simt_kernel(const __grid_constant__ AttnArgs a) {
   ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();  // (the join reads the plan at once)
   extern __shared__ float smem_f[];
-  if ((int)blockIdx.x >= a.workers) return;
-  AttnWalk walk(a, blockIdx.x), few = walk;
-  walk.only_many();
+  __shared__ int4 share[5];
+  attn_share(a, share);
+  AttnWalk walk(a, share), few = walk;
+  walk.only_many(a);
   simt_many<HD>(a, smem_f, walk);
   __syncthreads();
   few.only_few(a);

@@ -29,7 +29,7 @@ template <int HD> struct Few {
   static constexpr int RING = WARPS * STAGES * 2 * HALF;
   static constexpr int JOIN_ROWS = 8;                   // rows that the warps hand over at a time
   static constexpr int JOIN = WARPS * JOIN_ROWS * HD * 4;
-  static constexpr int STATS = 2 * WARPS * kFewRows * 4;
+  static constexpr int STATS = 2 * WARPS * kFewRows * 4 + 16;
   static constexpr int SMEM = RING + JOIN + STATS;
 };
 
@@ -190,7 +190,7 @@ template <int HD> struct FewSteps {
   AttnWalk walk;
   AttnPiece p;
   int key, end;   // next step of the current piece, and where it ends
-  __device__ __forceinline__ FewSteps(const AttnArgs& a, int worker) : walk(a, worker), key(0), end(0) { walk.only_few(a); }
+  __device__ __forceinline__ FewSteps(const AttnArgs& a, const int4* share) : walk(a, share), key(0), end(0) { walk.only_few(a); }
   __device__ __forceinline__ bool next_piece(const AttnArgs& a, int warp) {
     if (!walk.next(a, &p)) return false;
     key = (max(p.lo, (p.t.blk_lo + p.b0) * kAttnBlock) & ~(kFewKeys - 1)) + warp * kFewKeys;
@@ -200,7 +200,7 @@ template <int HD> struct FewSteps {
 };
 
 template <typename T, int HD>
-__device__ void few_share(const AttnArgs& a, uint8_t* smem, int worker) {
+__device__ void few_share(const AttnArgs& a, uint8_t* smem, const int4* share) {
   using F = Few<HD>;
   constexpr int CPR = HD / 8;              // 16-byte pieces of a key
   constexpr int KPI = 32 / CPR > 0 ? 32 / CPR : 1;  // keys that one copy instruction of the warp covers
@@ -213,12 +213,13 @@ __device__ void few_share(const AttnArgs& a, uint8_t* smem, int worker) {
   const uint32_t sq = ptx::smem_u32(join + warp * 8 * HD);
   float* stat_m = reinterpret_cast<float*>(smem + F::RING + F::JOIN);   // [warp][16]
   float* stat_l = stat_m + F::WARPS * kFewRows;
+  int* rows_word = reinterpret_cast<int*>(stat_l + F::WARPS * kFewRows);  // rows of the piece, as the first warp sees them
   const T* cache = reinterpret_cast<const T*>(a.cache);
   const int64_t ldc = (int64_t)a.kv_heads * HD;
   constexpr int kStep = F::WARPS * kFewKeys;
 
   // loads: one step ahead of the copies the pages of the keys are asked for (lane i: key i of the step)
-  FewSteps<HD> ld(a, worker);
+  FewSteps<HD> ld(a, share);
   bool more = true;
   AttnAhead next;
   int head_next = 0;
@@ -253,7 +254,7 @@ __device__ void few_share(const AttnArgs& a, uint8_t* smem, int worker) {
 #pragma unroll 1
   for (int i = 0; i < F::STAGES - 1; ++i) load();
 
-  FewSteps<HD> st(a, worker);
+  FewSteps<HD> st(a, share);
   int get = 0;
   while (st.next_piece(a, warp)) {
     const AttnPiece& p = st.p;
@@ -375,7 +376,9 @@ __device__ void few_share(const AttnArgs& a, uint8_t* smem, int worker) {
       stat_l[warp * kFewRows + g] = l0; stat_l[warp * kFewRows + g + 8] = l1;
     }
     static_assert(F::JOIN_ROWS == 8, "rows g, then rows g + 8");
-    for (int pass = 0; pass * 8 < max(p.t.nrows, 1); ++pass) {
+    if (threadIdx.x == 0) *rows_word = p.t.nrows;
+    int all_rows = 1;  // (the same for all warps: they wait for each other in every pass)
+    for (int pass = 0; pass * 8 < all_rows; ++pass) {
       if (pass * 8 + g < p.t.nrows) {
         float* dst = join + (warp * 8 + g) * HD + 2 * t4;
 #pragma unroll
@@ -383,6 +386,7 @@ __device__ void few_share(const AttnArgs& a, uint8_t* smem, int worker) {
           *reinterpret_cast<float2*>(dst + i * 8) = pass ? make_float2(o[i][2], o[i][3]) : make_float2(o[i][0], o[i][1]);
       }
       few_barrier(F::WARPS * 32);
+      all_rows = *rows_word;
       const int rows = min(8, p.t.nrows - pass * 8);
       constexpr int N = HD / 32;
       for (int rr = warp; rr < rows; rr += F::WARPS) {  // a warp per row, N columns a lane
@@ -513,8 +517,9 @@ __device__ __forceinline__ void many_load(const AttnArgs& a, const CUtensorMap* 
       }
     }
   }
-  if (!ok) {
-    // given up: wait (with a limit) for the copies that are still on their way before the CTA may end
+  {
+    // wait (with a limit) for the copies that are still on their way before the CTA may end: those of a walk that was given up, or
+    // of which another warp has seen less
     __shared__ int never;
     if (lane == 0) never = 0;
     __syncwarp();
@@ -668,8 +673,7 @@ __device__ __forceinline__ void many_multiply(const AttnArgs& a, uint8_t* smem, 
       for (int s = 0; s < 2; ++s)
         if (s == 0 || both) wait_p(s, 1);
   }
-  ok = __all_sync(0xffffffffu, *abort_flag == 0);
-  if (!ok) {  // given up: what has been issued may still read shared memory and write TMEM
+  {  // what has been issued may still read shared memory and write TMEM (under the other warps' last stores)
     __shared__ int never;
     if (lane == 0) never = 0;
     __syncwarp();
@@ -889,7 +893,9 @@ attn_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUten
   if constexpr (HD == 256) {
     ptx::grid_dependency_wait();
     ptx::grid_launch_dependents();
-    few_share<T, HD>(a, smem, blockIdx.x);
+    __shared__ int4 share[5];
+    attn_share(a, share);
+    few_share<T, HD>(a, smem, share);
   } else {
     // Barriers and TMEM before the wait, whether the share will need them or not: under the end of the kernel before.
     __shared__ __align__(8) ManySync sy;
@@ -911,8 +917,10 @@ attn_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUten
     ptx::tc_fence_after();
     ptx::grid_dependency_wait();
     ptx::grid_launch_dependents();  // (the TMEM is ours, and the plan that the join reads at once is complete)
-    AttnWalk walk(a, blockIdx.x);
-    walk.only_many();
+    __shared__ int4 share[5];
+    attn_share(a, share);
+    AttnWalk walk(a, share);
+    walk.only_many(a);
     const bool many = walk.more();  // the same for the whole CTA
     __syncwarp();
     if (warp >= 8) {
@@ -938,7 +946,7 @@ attn_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUten
         __syncthreads();
         if (sy.abort_word && threadIdx.x == 0 && a.status) atomicCAS(a.status, 0u, (uint32_t)CS_TIMEOUT_MBARRIER);
       }
-      few_share<T, HD>(a, smem, blockIdx.x);
+      few_share<T, HD>(a, smem, share);
     }
   }
 }
