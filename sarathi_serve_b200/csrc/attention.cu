@@ -374,7 +374,7 @@ attn_join_kernel(const AttnArgs a) {
       for (int k = 0; k < kBatch; ++k) {
         const float wt = exp2f(l[k] - base);
         sum += wt;
-        if (wt != 0.f) {  // (0: a piece that this row sees nothing of)
+        if (i + k < c.pieces) {  // (a piece that this row sees nothing of holds zeros; one that it sees counts, however small its weight)
           acc.x += wt * o[k].x; acc.y += wt * o[k].y; acc.z += wt * o[k].z; acc.w += wt * o[k].w;
         }
       }

@@ -188,7 +188,7 @@ __device__ void simt_many(const AttnArgs& a, float* smem, AttnWalk walk) {
         *reinterpret_cast<float4*>(sp + (cg + 16 * i) * M::LDP + rg * 4) = make_float4(s[0][i], s[1][i], s[2][i], s[3][i]);
       __syncwarp();  // the rows of a warp are its own
       // Keys that all rows of the warp see, and around them those that only some see: such a key contributes nothing to the others,
-      // whatever its value holds.  (One by one through every step that has any: the chunk of 256 and 32 decodes of above take 43 us then.)
+      // whatever its value holds.  (Not: whose probability is 0.  A value that is not finite reaches every row that sees it.)  (One by one through every step that has any: the chunk of 256 and 32 decodes of above take 43 us then.)
       const int see = min(M::KEYS, max(0, warp_hi + 1 - kb)), see_lo = a.window > 0 ? min(see, max(0, warp_lo - a.window + 1 - kb)) : 0;
       const int mid = a.window > 0 ? min(see, max(see_lo, warp_hi - a.window + 1 - kb)) : 0, mid_end = min(see, max(mid, warp_lo + 1 - kb));
       auto one_by_one = [&](int k, int end) {
@@ -201,7 +201,8 @@ __device__ void simt_many(const AttnArgs& a, float* smem, AttnWalk walk) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
               const float x = w[j];
-              if (x != 0.f) { acc[j][i].x += x * v.x; acc[j][i].y += x * v.y; acc[j][i].z += x * v.z; acc[j][i].w += x * v.w; }
+              const int key = kb + k;
+              if (key <= pos[j] && (a.window == 0 || key > pos[j] - a.window)) { acc[j][i].x += x * v.x; acc[j][i].y += x * v.y; acc[j][i].z += x * v.z; acc[j][i].w += x * v.w; }
             }
           }
         }
@@ -369,7 +370,8 @@ __device__ void simt_few(const AttnArgs& a, float* smem, const AttnWalk& walk) {
 #pragma unroll
         for (int r = 0; r < R; ++r) {
           const float w = s[t][r];
-          if (all || w != 0.f) {  // a key that the row does not see contributes nothing, whatever its value holds
+          const int key = st.key + t * KPW + mine;
+          if (all || (key <= pos[r] && (a.window == 0 || key > pos[r] - a.window))) {  // a key that the row does not see contributes nothing, whatever its value holds
             o[r][0].x += w * x.x; o[r][0].y += w * x.y; o[r][0].z += w * x.z; o[r][0].w += w * x.w;
             o[r][1].x += w * y.x; o[r][1].y += w * y.y; o[r][1].z += w * y.z; o[r][1].w += w * y.w;
           }
@@ -410,9 +412,7 @@ __device__ void simt_few(const AttnArgs& a, float* smem, const AttnWalk& walk) {
       const float base = top == -INFINITY ? 0.f : top;
 #pragma unroll
       for (int w = 0; w < kFew32Warps; ++w) {
-        const float mw = stat_m[w * R + warp];
-        if (mw == -INFINITY) { sum += stat_l[w * R + warp]; continue; }
-        const float f = exp2f(mw - base);
+        const float mw = stat_m[w * R + warp], f = mw == -INFINITY ? 0.f : exp2f(mw - base);
         sum += f * stat_l[w * R + warp];
 #pragma unroll
         for (int j = 0; j < N; ++j) acc[j] += f * join[(w * R + warp) * HD + lane * N + j];

@@ -398,9 +398,7 @@ __device__ void few_share(const AttnArgs& a, uint8_t* smem, const int4* share) {
         float l = 0.f, acc[N] = {};
 #pragma unroll
         for (int w = 0; w < F::WARPS; ++w) {
-          const float mw = stat_m[w * kFewRows + r];
-          if (mw == -INFINITY) { l += stat_l[w * kFewRows + r]; continue; }
-          const float f = pow2(mw - base);
+          const float mw = stat_m[w * kFewRows + r], f = mw == -INFINITY ? 0.f : pow2(mw - base);
           l += f * stat_l[w * kFewRows + r];
 #pragma unroll
           for (int j = 0; j < N; ++j) acc[j] += f * join[(w * 8 + rr) * HD + lane * N + j];
