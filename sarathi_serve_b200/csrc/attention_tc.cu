@@ -12,8 +12,8 @@
 // Many rows (prompt chunks): tiles of 256 rows on tcgen05, see "many rows" below.
 //
 // Scores, maxima, sums and outputs are fp32.  Probabilities are rounded to the 16 bits of the values, as both tensor instructions
-// want both operands of one type: that is at most half a step of each, like one more rounding of each value.  The sum that the
-// result is divided by is that of the unrounded ones.
+// want both operands of one type: that is at most half a step of each, like one more rounding of each value (fp16 below 2^-21 of the
+// largest: 2^-32 of it, see kHeadroom).  The sum that the result is divided by is that of the unrounded ones.
 #include "attention.cuh"
 #include "gemm_host.cuh"
 
@@ -118,6 +118,11 @@ __device__ __forceinline__ void few_barrier(int threads) {
 // 2^8, which 16 bits hold as well as numbers below 1, and the output need not be rescaled.
 constexpr float kLazy = 8.f;
 
+// Probabilities are made 2^kHeadroom times as large (the sums with them, so the result is the same): fp16 has no full precision below
+// 2^-14, and one key that outweighs the others by more than that would coarsen theirs (20000 keys of 2^-19.3 beside one: 0.7 % off).
+// With kLazy they reach 2^15 and no more, which fp16 holds.
+template <typename T> constexpr float kHeadroom = DT<T>::id == SB200_F16 ? 7.f : 0.f;
+
 // Lane i of a quad has row i's four pieces; afterwards v[j] is piece i of row j.
 __device__ __forceinline__ void turn_quad(uint4 (&v)[4], int lane4) {
   auto swap = [&](uint4& x, uint4& y, int mask, bool upper) {  // the upper lane gives x and takes y's place
@@ -135,7 +140,7 @@ __device__ __forceinline__ void turn_quad(uint4 (&v)[4], int lane4) {
 }
 
 // What a product with P = 0 cannot do is to leave out a value that is not finite.  Called by a warp for a row of which some columns
-// came out not finite; o: this lane's columns lane * HD / 32 ..., m: the maximum that the row's sum was made with.  Only keys that
+// came out not finite; o: this lane's columns lane * HD / 32 ..., m: what was taken from the scores in the row's sum.  Only keys that
 // the tile has and the row does not see can have spoilt it: if one of them is not finite in such a column, the column is
 // made again, key by key (true is returned); if none is, the result stands.  So a value that is not finite costs the rows that see
 // it a look at their tile's last keys, and only the rows of its own tile before it the long way.
@@ -341,7 +346,7 @@ __device__ void few_share(const AttnArgs& a, uint8_t* smem, const int4* share) {
 #pragma unroll
         for (int i = 0; i < NT; ++i) { o[i][0] *= f0; o[i][1] *= f0; o[i][2] *= f1; o[i][3] *= f1; }
       }
-      const float b0 = m0 == -INFINITY ? 0.f : m0, b1 = m1 == -INFINITY ? 0.f : m1;
+      const float b0 = (m0 == -INFINITY ? 0.f : m0) - kHeadroom<T>, b1 = (m1 == -INFINITY ? 0.f : m1) - kHeadroom<T>;
       uint32_t pf[4];
 #pragma unroll
       for (int n = 0; n < 2; ++n) {
@@ -394,7 +399,7 @@ __device__ void few_share(const AttnArgs& a, uint8_t* smem, const int4* share) {
         float m = -INFINITY;
 #pragma unroll
         for (int w = 0; w < F::WARPS; ++w) m = fmaxf(m, stat_m[w * kFewRows + r]);
-        const float base = m == -INFINITY ? 0.f : m;
+        float base = m == -INFINITY ? 0.f : m;
         float l = 0.f, acc[N] = {};
 #pragma unroll
         for (int w = 0; w < F::WARPS; ++w) {
@@ -403,6 +408,7 @@ __device__ void few_share(const AttnArgs& a, uint8_t* smem, const int4* share) {
 #pragma unroll
           for (int j = 0; j < N; ++j) acc[j] += f * join[(w * 8 + rr) * HD + lane * N + j];
         }
+        base -= kHeadroom<T>;
         bool fine = true;
 #pragma unroll
         for (int j = 0; j < N; ++j) fine = fine && fabsf(acc[j]) < INFINITY;
@@ -734,7 +740,7 @@ __device__ __forceinline__ void many_softmax(const AttnArgs& a, uint8_t* smem, M
       uint32_t prob[32];
       f32x2 sum0, sum1;
       auto exponentials = [&](int part) {
-        const float base = m == -INFINITY ? 0.f : -m * scale;
+        const float base = kHeadroom<T> - (m == -INFINITY ? 0.f : m * scale);
         const f32x2 sc = pair(scale, scale), bs = pair(base, base);
 #pragma unroll
         for (int i = 0; i < 32; ++i) {
@@ -795,7 +801,7 @@ __device__ __forceinline__ void many_softmax(const AttnArgs& a, uint8_t* smem, M
     const bool some = l > 0.f || l != l;
     const float inv = p.slot < 0 ? attn_inverse(l, pos) : some ? 1.f / l : 0.f;
     const int64_t at = (int64_t)p.slot * a.slot_rows + r;
-    const float base2 = m == -INFINITY ? 0.f : m * scale;
+    const float base2 = (m == -INFINITY ? 0.f : m * scale) - kHeadroom<T>;
     bool fine = true;
     const long long mine = real ? token * a.ldo + head * HD : -1;  // where this thread's row goes
     long long quad_off[4];                                         // and those of its four lanes

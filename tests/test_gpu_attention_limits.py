@@ -46,3 +46,45 @@ def test_values_that_are_not_finite_under_weights_that_vanish(dtype, hd, window)
                     c["cache"][c["table"][r, lo // 16], 1, lo % 16, 1, 5] = (math.nan, math.inf)[at % 2]
             plan, _ = plan_of(c, window)
             check(c, attention_ops.paged_attention(c["q"], c["cache"], plan, 0.1), 0.1, window)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("hd,page", [(64, 16), (128, 16), (256, 16), (128, 12)])
+@pytest.mark.parametrize("batch", [[(1, 20000), (3, 9000)], [(200, 5000), (1, 300)]], ids=["decodes", "chunk"])
+def test_one_key_that_outweighs_thousands(dtype, hd, page, batch):
+    """One key has a value of 0 and a score 10 to 15 above the others', whose probabilities (2^-14 to 2^-22 of it) make the result.
+    Tolerance: that of test_gpu_attention.py, but what fp16 loses below its full precision is 2^-32 of the largest a key (at worst
+    2^-25 of 2^-7)."""
+    from sarathi_serve_b200 import attention_ops
+    heads, scale = 4, 1.0
+    u = torch.finfo(dtype).eps / 2
+    for sink in (0, 100):
+        c = make(23, dtype, heads, 1, hd, page, batch, cache_fill=0.0)
+        c["q"].zero_()
+        a = (10 + 5 * torch.rand(c["T"], heads, generator=torch.Generator().manual_seed(5))).to(dtype).cuda()
+        c["q"][:, ::hd] = a / 8
+        plan, _ = plan_of(c)
+        want = []
+        for r, (new, before) in enumerate(batch):
+            n = new + before
+            where = torch.arange(n, device="cuda")
+            pages = c["table"][r].long()[where // page]
+            c["cache"][pages, 0, where % page] = 0
+            c["cache"][pages[sink], 0, sink % page, 0, 0] = 8.0
+            c["cache"][pages, 1, where % page] = c["cache"][pages, 1, where % page].abs().clamp(max=2.0)
+            c["cache"][pages[sink], 1, sink % page] = 0
+            v = c["cache"][pages, 1, where % page][:, 0].double()
+            row = sum(b[0] for b in batch[:r])
+            s = torch.zeros(new, heads, n, dtype=torch.float64, device="cuda")
+            s[:, :, sink] = (c["q"][row:row + new, ::hd].double() * 8)
+            s.masked_fill_((where > before + torch.arange(new, device="cuda")[:, None])[:, None], -math.inf)
+            res = torch.softmax(s, 2) @ v
+            delta = (hd + 16) * 2.0 ** -24 * 16 + 2.0 ** -21
+            tol = (2 * u + 2 * delta + 2 * (n + 16) * 2.0 ** -24) * res + (n * 2.0 ** -32 * 2 + 2.0 ** -25 if dtype == torch.float16 else 0)
+            want.append((res, tol))
+        lse = torch.zeros(c["T"], heads, device="cuda")
+        out = attention_ops.paged_attention(c["q"], c["cache"], plan, scale, lse=lse).view(-1, heads, hd).double()
+        res, tol = (torch.cat(x) for x in zip(*want))
+        worst = ((out - res).abs() / tol).max().item()
+        assert worst <= 1, f"{worst:.2f} times the tolerance"
+        check(c, out.view(-1, heads * hd), scale, lse=lse)
