@@ -294,7 +294,7 @@ attn_plan_kernel(const PlanArgs a) {
     s.tile = d;
     s.many = tiles_many;
     s.slot = slot;
-    s.rows = a.n ? max(0, min(a.qo_indptr[a.n], a.max_tokens)) : 0;
+    s.rows = a.n ? max(0, min(a.qo_indptr[w == 1 ? 0 : a.n], a.max_tokens)) : 0;
     s.units = units;
     const int4* src = reinterpret_cast<const int4*>(&s);
     int4* dst = reinterpret_cast<int4*>(a.plan.starts + w);
@@ -304,7 +304,7 @@ attn_plan_kernel(const PlanArgs a) {
 
 // Joins the pieces of cut units: o = sum_p 2^(l_p - m) o_p / sum_p 2^(l_p - m) with l_p the log2 of piece p's sum, in the
 // order of the keys.  The cut units' rows are dealt out in groups of 1024 values, four a thread: neighbouring lanes have neighbouring
-// rows, which is how the slots are laid out.  Also clears the rows of q that belong to no request, when asked to.  Bound by
+// rows, which is how the slots are laid out.  Also clears the rows that belong to no request, when asked to.  Bound by
 // latency: the groups' prefix sums, the unit and its pieces (sums and outputs of four at a time) are three loads after one another:
 // 2 to 4 us for decodes, 20 with a cut unit of 256 rows on every SM.
 // What it reads of the plan it reads ahead of its wait: the attention kernel lets it start only when its own wait is over, and the plan
@@ -336,8 +336,10 @@ attn_join_kernel(const AttnArgs a) {
   if ((int)blockIdx.x < groups) look_up(blockIdx.x);
   grid_dependency_begin();
   if (a.zero_behind) {
-    const int rows0 = attn_clamp(a.plan.starts[0].rows, 0, a.num_tokens), per_row = a.kv_heads * a.group * HD;
-    for (int t = rows0 + blockIdx.x; t < a.num_tokens; t += gridDim.x) {
+    const int ahead = attn_clamp(a.plan.starts[1].rows, 0, a.num_tokens);
+    const int behind = attn_clamp(a.plan.starts[0].rows, ahead, a.num_tokens), per_row = a.kv_heads * a.group * HD;
+    for (int row = blockIdx.x; row < ahead + a.num_tokens - behind; row += gridDim.x) {
+      const int t = row < ahead ? row : row - ahead + behind;
       for (int i = threadIdx.x; i < per_row; i += kJoinThreads) out[t * a.ldo + i] = DT<T>::from_f(0.f);
       if (a.lse)
         for (int i = threadIdx.x; i < a.kv_heads * a.group; i += kJoinThreads)

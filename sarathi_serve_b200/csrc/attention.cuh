@@ -42,7 +42,7 @@ struct alignas(16) AttnStart {
   AttnTile tile;  // of `at`
   int many;       // tiles of many rows (they come before the others)
   int slot;       // of its first piece that is not a whole unit; slots of one unit follow one another in the order of the keys
-  int rows;       // rows of q that belong to a request
+  int rows;       // of the first worker: the row of q behind the last request's; of the second: the first request's first row
   int units;      // cut units
 };
 

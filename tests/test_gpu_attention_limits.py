@@ -88,3 +88,23 @@ def test_one_key_that_outweighs_thousands(dtype, hd, page, batch):
         worst = ((out - res).abs() / tol).max().item()
         assert worst <= 1, f"{worst:.2f} times the tolerance"
         check(c, out.view(-1, heads * hd), scale, lse=lse)
+
+
+@pytest.mark.parametrize("dtype,hd", [(torch.bfloat16, 128), (torch.float16, 256), (torch.float32, 64)])
+def test_rows_ahead_of_the_first_request(dtype, hd):
+    """Offsets that start behind row 0: the rows ahead belong to no request, as those behind the last one's."""
+    from sarathi_serve_b200 import attention_ops
+    c = make(24, dtype, 4, 2, hd, 16, [(20, 3), (1, 200), (140, 0)], pad=9)
+    plan, lay = plan_of(c)
+    plan.update(qo_indptr=lay.qo_indptr + 5, kv_lens=lay.kv_lens, kv_indptr=lay.kv_indptr, kv_indices=lay.kv_indices)
+    part = dict(c, q=c["q"][5:166])
+    lse = torch.full((c["T"], 4), 7.0, device="cuda")
+    out = attention_ops.paged_attention(c["q"], c["cache"], plan, 0.1, lse=lse)
+    check(part, out[5:], 0.1, lse=lse[5:])
+    for rows in (slice(0, 5), slice(166, c["T"])):
+        assert (out[rows] == 0).all() and (lse[rows] == -math.inf).all()
+    given, lse = torch.full_like(out, 3.0), torch.full_like(lse, 7.0)
+    attention_ops.paged_attention(c["q"], c["cache"], plan, 0.1, out=given, lse=lse)
+    assert torch.equal(given[5:166], out[5:166])
+    for rows in (slice(0, 5), slice(166, c["T"])):
+        assert (given[rows] == 3).all() and (lse[rows] == 7).all()
