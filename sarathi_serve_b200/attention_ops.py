@@ -51,6 +51,7 @@ class AttentionPlan:
         # the stream of the last call; so far the one that the buffers belong to
         self._stream = torch.cuda.current_stream(self.buffer.device)
         self._stream_ptr: int = self._stream.cuda_stream
+        self._streams = {self._stream_ptr}  # those that the plan's own memory is kept for
 
     def stream(self) -> int:
         """The current stream, behind whatever the plan's calls have queued on the one they used last.  (A kernel that read a plan
@@ -60,9 +61,12 @@ class AttentionPlan:
         if here != self._stream_ptr and not torch.cuda.is_current_stream_capturing():
             now = torch.cuda.current_stream()
             now.wait_stream(self._stream)
-            for t in (self.buffer, self.workspace, self.kv_indices, *self.beside):
-                if t is not None:
+            if here not in self._streams:
+                self._streams.add(here)
+                for t in (self.buffer, self.workspace, *self.beside):
                     t.record_stream(now)
+            if self.kv_indices is not None:
+                self.kv_indices.record_stream(now)
             self._stream, self._stream_ptr = now, here
         return here
 

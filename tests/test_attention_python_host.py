@@ -126,6 +126,19 @@ def test_a_wrapper_that_is_used_on_another_stream_than_it_was_made_on(machine):
         assert machine.has(t, side)
 
 
+def test_a_wrapper_that_goes_back_and_forth_between_streams(machine):
+    """Every change waits for the stream before; its memory is recorded once a stream, not every time."""
+    main, side, _ = machine.streams
+    w = attention_wrapper.PagedAttentionWrapper(2, 1, 64, 16, 5, 40, torch.float16, 4, 8, 3, device=torch.device("cpu"))
+    i = lambda *s: torch.ones(*s, dtype=torch.int32)
+    for _ in range(5):
+        for stream in (side, main):
+            with machine.on(stream):
+                w.begin_forward(i(2), i(2), i(2, 1), 4)
+    assert side.waited == [main] * 5 and main.waited == [side] * 5
+    assert all(machine.has(t, side) for t in w.kv_caches) and len(machine.recorded) < 40 + 20
+
+
 def test_a_wrapper_on_another_current_device_refuses_its_calls(machine):
     """Nothing is launched there, neither the append before the attention nor anything else, and the plan's stream stays."""
     w = attention_wrapper.PagedAttentionWrapper(2, 1, 64, 16, 5, 2, torch.float16, 4, 8, 3, device=torch.device("cpu"))
