@@ -23,7 +23,7 @@ struct PlanArgs {
 // What a block of keys, and a unit apart from its blocks, costs a CTA, in hundredths of a microsecond, and the least blocks of a
 // piece.  Fitted to when the CTAs ended in 17 steps, most of them mixed, their keys in HBM: 0.2 us a block more for many rows than where
 // every SM does them, a window's masks at both ends 2 us a unit.  Few rows count at the share of HBM that an SM has when all of them
-// stream.
+// stream (3 % less than fitted then, as a unit starts faster since: 512 rows with 100 decodes 187 -> 179 us).
 __device__ __forceinline__ void unit_cost(const AttnShape& sh, int kind, int nrows, int* block, int* fixed, int* least) {
   const bool wide = sh.head_dim > 64;
   if (sh.dtype == SB200_F32) {
@@ -35,8 +35,8 @@ __device__ __forceinline__ void unit_cost(const AttnShape& sh, int kind, int nro
     *fixed = (wide ? 508 : 480) + (sh.window > 0 ? 200 : 0);
     *least = 2;
   } else {
-    *block = sh.head_dim == 256 ? 300 : wide ? 150 : 100;
-    *fixed = wide ? 260 : 220;
+    *block = sh.head_dim == 256 ? 290 : wide ? 145 : 97;
+    *fixed = wide ? 250 : 215;
     *least = 2;
   }
 }
@@ -348,11 +348,12 @@ attn_join_kernel(const AttnArgs a) {
   }
   for (int g = blockIdx.x; g < groups; g += gridDim.x) {
     if (g != (int)blockIdx.x) look_up(g);
-    AttnCut c = {attn_clamp(u.x, 0, a.num_tokens), attn_clamp(u.y, 0, a.num_tokens * a.group), attn_clamp(u.z, 0, a.slot_rows), u.w,
-                 attn_clamp(v.x, 0, a.kv_heads - 1), attn_clamp(v.y, 0, 2 * a.workers - 1), v.z, 0};
-    c.pieces = min(c.pieces, 2 * a.workers - c.slot);
+    const AttnCut c = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
     const int r = (g - first[lo]) * kRows + threadIdx.x % kRows, col4 = threadIdx.x / kRows;
-    if ((unsigned)r >= (unsigned)min(c.nrows, max(0, (a.num_tokens - c.q_row) * a.group - c.row0))) continue;
+    const bool fine = (unsigned)c.q_row <= (unsigned)a.num_tokens && (unsigned)c.row0 <= (unsigned)(a.num_tokens * a.group) &&
+                      (unsigned)c.nrows <= (unsigned)a.slot_rows && (unsigned)c.head < (unsigned)a.kv_heads &&
+                      (unsigned)c.slot <= (unsigned)(2 * a.workers) && (unsigned)c.pieces <= (unsigned)(2 * a.workers - c.slot);
+    if (!fine || (unsigned)r >= (unsigned)min(c.nrows, max(0, (a.num_tokens - c.q_row) * a.group - c.row0))) continue;
     float m = -INFINITY, base = 0.f, sum = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int i = 0; i < c.pieces; i += kBatch) {

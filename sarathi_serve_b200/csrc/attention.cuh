@@ -116,33 +116,32 @@ __device__ __forceinline__ float4* attn_part(const AttnArgs& a, int head_dim, in
   return reinterpret_cast<float4*>(a.part_o + (int64_t)slot * a.slot_rows * head_dim) + (col4 * stride + row);
 }
 
+__host__ __device__ __forceinline__ int attn_min(int a, int b) { return a < b ? a : b; }
+__host__ __device__ __forceinline__ int attn_max(int a, int b) { return a > b ? a : b; }
 __host__ __device__ __forceinline__ int attn_clamp(int v, int lo, int hi) { return v < lo ? lo : v > hi ? hi : v; }
 
 // The piece of tile t that begins at `cur`, in a share that ends at `end`; `most`: rows of its kind of tile, `slot`: of the share's next
 // piece that is not a whole unit.
 // What comes from the plan is held to what the call's own arguments allow.  Calls that share a plan follow one another, and then
 // nothing changes here; if a caller lets them overlap all the same (graphs on two streams, the C interface), or hands over the plan of
-// another shape, the numbers are wrong but no address is.
-__host__ __device__ __forceinline__ AttnPiece attn_piece(const AttnArgs& a, AttnTile t, int4 cur, int4 end, int most, int* slot) {
+// another shape, the numbers are wrong but no address is: rows are rows of q, there are no more steps than keys listed, and the page of
+// a key, wherever its number comes from, is looked up within the list and checked.  (Only what addresses need: this code is in six
+// places, and what it costs is fetching it.  With a clamp for each number three chunks of 1500 take 2 us of 88 more.)
+__host__ __device__ __forceinline__ AttnPiece attn_piece(const AttnArgs& a, const AttnTile& t, int4 cur, int4 end, int most, int* slot) {
   AttnPiece p;
-  t.q_row = attn_clamp(t.q_row, 0, a.num_tokens);
-  t.row0 = attn_clamp(t.row0, 0, a.num_tokens * a.group);
-  t.nrows = attn_clamp(t.nrows, 0, most);
-  t.pos0 = attn_clamp(t.pos0, -kAttnMaxKeys, kAttnMaxKeys);
-  t.page_at = t.page_at < 0 ? 0 : t.page_at;
-  t.blk_lo = attn_clamp(t.blk_lo, 0, a.blocks);
-  t.nblk = attn_clamp(t.nblk, 0, a.blocks - t.blk_lo);
+  const bool tail_cut = cur.x == end.x && cur.y == end.y;
   p.t = t;
-  p.stride = t.nrows;
-  p.head = attn_clamp(cur.y, 0, a.kv_heads - 1);
-  p.b0 = attn_clamp(cur.z, 0, t.nblk);
-  p.b1 = cur.x == end.x && cur.y == end.y ? attn_clamp(end.z, p.b0, t.nblk) : t.nblk;
-  p.slot = p.b0 > 0 || p.b1 < t.nblk ? attn_clamp((*slot)++, 0, 2 * a.workers - 1) : -1;
+  p.head = cur.y;
+  p.b0 = cur.z;
+  p.b1 = attn_max(cur.z, attn_min(tail_cut ? end.z : t.nblk, cur.z + a.blocks));
+  p.slot = tail_cut || cur.z > 0 ? (*slot)++ : -1;
+  p.stride = attn_min(t.nrows, most);
   // q may have fewer rows than the plan was made for (tokens x group stays below 2^30)
-  p.t.nrows = attn_clamp((a.num_tokens - t.q_row) * a.group - t.row0, 0, t.nrows);
-  const int first = a.by_group.div(t.row0), last = a.by_group.div(t.row0 + (p.t.nrows > 0 ? p.t.nrows - 1 : 0));
-  p.hi = t.pos0 + last + 1 < 0 ? 0 : t.pos0 + last + 1;
-  p.lo = a.window > 0 && t.pos0 + first + 1 > a.window ? t.pos0 + first + 1 - a.window : 0;
+  const bool rows = (unsigned)t.q_row <= (unsigned)a.num_tokens && (unsigned)t.row0 <= (1u << 30);
+  p.t.nrows = rows ? attn_max(0, attn_min(p.stride, (a.num_tokens - t.q_row) * a.group - t.row0)) : 0;
+  const int first = a.by_group.div(t.row0), last = a.by_group.div(t.row0 + attn_max(p.t.nrows, 1) - 1);
+  p.hi = attn_max(0, t.pos0 + last + 1);
+  p.lo = a.window > 0 ? attn_min(attn_max(0, t.pos0 + first + 1 - a.window), kAttnMaxKeys) : 0;
   return p;
 }
 
@@ -157,16 +156,16 @@ struct AttnWalk {
   __device__ __forceinline__ AttnWalk(const AttnArgs& a, const int4* s) {
     cur = s[0];
     end = s[4];
-    cur.x = attn_clamp(cur.x, 0, a.plan.tiles_cap);
-    end.x = attn_clamp(end.x, 0, a.plan.tiles_cap);
-    end.y = attn_clamp(end.y, 0, a.kv_heads);
+    // (as attn_piece: these hold the tile, the head, the block and the two slots of a share)
+    cur = make_int4(max(cur.x, 0), attn_clamp(cur.y, 0, a.kv_heads - 1), attn_clamp(cur.z, 0, kAttnMaxKeys / kAttnBlock), 0);
+    if (end.x >= a.plan.tiles_cap) end = make_int4(a.plan.tiles_cap, 0, 0, 0);
     many = attn_clamp(s[3].x, 0, a.many_cap);
-    slot = s[3].y;
+    slot = attn_clamp(s[3].y, 0, 2 * a.workers - 2);
     word = reinterpret_cast<const int*>(s + 1)[threadIdx.x & 7];
     most = 0;
   }
   __device__ __forceinline__ void fetch(const AttnArgs& a) {
-    if (more()) word = reinterpret_cast<const int*>(a.plan.tiles + min(cur.x, a.plan.tiles_cap - 1))[threadIdx.x & 7];
+    if (more()) word = reinterpret_cast<const int*>(a.plan.tiles + cur.x)[threadIdx.x & 7];
   }
   // Only the tiles of many rows, or the others.
   __device__ __forceinline__ void only_many(const AttnArgs& a) {
@@ -230,7 +229,7 @@ struct AttnAhead {
   __device__ __forceinline__ void ask(const AttnArgs& a, int page_at, int key, bool seen) {
     const int p = a.by_page.div(max(key, 0));
     const long long at = (long long)page_at + p;
-    seen = seen && at < a.num_kv_indices;
+    seen = seen && at >= 0 && at < a.num_kv_indices;
     page = seen ? a.kv_indices[at] : -1;
     slot = seen ? key - p * a.page_size : -1;
   }

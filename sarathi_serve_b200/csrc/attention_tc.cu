@@ -494,7 +494,7 @@ __device__ __forceinline__ void many_load(const AttnArgs& a, const CUtensorMap* 
     auto page_of = [&](int b) {
       const int key = key_of(b);
       const long long at = (long long)p.t.page_at + a.by_page.div(key);
-      return b < p.b1 && lane < boxes && key < p.hi && at < a.num_kv_indices ? a.kv_indices[at] : -1;
+      return b < p.b1 && lane < boxes && key < p.hi && at >= 0 && at < a.num_kv_indices ? a.kv_indices[at] : -1;
     };
     int next = page_of(p.b0);
     for (int b = p.b0; ok && b < p.b1; ++b) {
