@@ -282,7 +282,7 @@ typedef struct sb200_attention_shape {
  * request are left as they were, or cleared if zero_rows_behind.  Pages outside [0, num_pages) read as zeros.
  * out must not overlap q (columns of one buffer may interleave if ldq = ldo) or the cache, nor lse any of the three.
  * workspace (sb200_attention_workspace_bytes): parts of rows whose keys are shared out; written before it is read in every
- * call.  A plan and a workspace serve one call at a time: not two streams at once.  `status` (device word): as sb200_gemm_colpar.
+ * call.  A plan and a workspace serve one call at a time: not two streams at once (calls that overlap give wrong numbers).  `status` (device word): as sb200_gemm_colpar.
  * Replaces: BatchPrefillWithPagedKVCacheWrapper.plan / run,
  * sarathi/model_executor/attention/flashinfer_attention_wrapper.py:240-299. */
 int64_t sb200_attention_plan_bytes(const sb200_attention_shape* shape);

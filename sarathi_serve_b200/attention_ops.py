@@ -22,9 +22,9 @@ class AttentionPlan:
     ``num_heads`` / ``num_kv_heads``: of this rank; ``window``: a token sees itself and the ``window - 1`` tokens before it (0:
     all of them).  ``max_requests`` and ``max_tokens`` bound the steps the plan is updated with.  A plan serves one step at a
     time: a call on another stream than the one before waits for that one, and the graphs that captured such calls belong on one
-    stream (or ordered by events).  A graph keeps reading
-    the ``kv_indices`` that the plan had when it was captured: write later steps' layouts to the same arrays
-    (``batch_layout(..., out=)``)."""
+    stream (or ordered by events): replays that overlap give wrong numbers.  A graph keeps reading the ``kv_indices`` that the plan had
+    when it was captured: write later steps' layouts to the same arrays (``batch_layout(..., out=)``), on the stream that reads them or
+    ordered with it, as that call is none of the plan's."""
 
     def __init__(self, num_heads: int, num_kv_heads: int, head_dim: int, page_size: int, dtype: torch.dtype, max_requests: int,
                  max_tokens: int, window: int = 0, device: Optional[torch.device] = None):

@@ -23,7 +23,7 @@ struct PlanArgs {
 // What a block of keys, and a unit apart from its blocks, costs a CTA, in hundredths of a microsecond, and the least blocks of a
 // piece.  Fitted to when the CTAs ended in 17 steps, most of them mixed, their keys in HBM: 0.2 us a block more for many rows than where
 // every SM does them, a window's masks at both ends 2 us a unit.  Few rows count at the share of HBM that an SM has when all of them
-// stream (3 % less than fitted then, as a unit starts faster since: 512 rows with 100 decodes 187 -> 179 us).
+// stream (3 % less than fitted then, as a unit starts faster since: 512 rows with 100 decodes 187 -> 182 us).
 __device__ __forceinline__ void unit_cost(const AttnShape& sh, int kind, int nrows, int* block, int* fixed, int* least) {
   const bool wide = sh.head_dim > 64;
   if (sh.dtype == SB200_F32) {
@@ -420,8 +420,10 @@ static int attn_shape(const sb200_attention_shape* s, AttnShape* sh, const char*
   sh->page_size = s->page_size;
   sh->dtype = s->dtype;
   sh->window = s->window < kAttnMaxKeys ? s->window : 0;  // (a wider one hides nothing; position - window stays within 32 bits)
-  // Tiles of 256 rows on tcgen05 fetch keys in boxes of whole swizzle atoms (8 rows); pages that are no multiple of 8, and
-  // heads of 256, whose two outputs and scores do not fit TMEM together, stay with tiles of 16 rows.
+  // Tiles of 256 rows on tcgen05 fetch keys in boxes of whole swizzle atoms (8 rows), and hold scores and outputs of two halves in TMEM.
+  // Pages that are no multiple of 8, and heads of 256, of which TMEM has room for one half (128 + 256 columns) only, stay with tiles of
+  // 16 rows: a tenth of the rate in long chunks (2000 tokens at 8000, 32 heads on 8: 266 us with heads of 128 and pages of 16, 2232 with pages of
+  // 12, 4754 with heads of 256).
   const bool many = s->dtype != SB200_F32 && s->head_dim <= 128 && s->page_size % 8 == 0;
   const bool f32 = s->dtype == SB200_F32;
   sh->rows_many = f32 ? 64 : many ? 256 : 16;
